@@ -540,6 +540,114 @@ typedef struct MgbsMlpNoAllocArgs {
 int mgbs_mlp_score_noalloc(const MgbsMlpNoAllocArgs* args, const uint8_t* children, int32_t rows, uint32_t* scores,
                            int32_t* err_out_host, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators for training and serving scorers.  No counterparts in the reference.  Device pointers unless a comment
+ * says otherwise, on the current device; each call enqueues on `stream`, allocates nothing, keeps nothing, and may be
+ * captured in a graph.  Workspaces are the caller's and belong to one call at a time.  Equal calls give equal bits.
+ * ---------------------------------------------------------------------------------------------------------------- */
+#define MGBS_DT_BF16 0
+#define MGBS_DT_F16 1
+#define MGBS_DT_F32 2
+
+/* RMS norm of every query and key head with a learned gain, and the rotation by position:
+ *   y = R(position) (gain * x / sqrt(mean(x^2) + eps)),
+ * R turns the pairs (i, i + head_dim/2), or (2i, 2i+1) when interleaved, by position * freq_i.  x and y are
+ * [batch, tokens, heads, head_dim] with any strides (elements) for the first three and 1 for the last; y may be x.
+ * Backward: q, k are the forward's inputs, dq_out / dk_out the gradients of its outputs, q_out / k_out take the
+ * gradients of q and k, dq_gain / dk_gain [head_dim] those of the gains. */
+typedef struct MgbsQkNormArgs {
+  int32_t dtype;         /* MGBS_DT_* of q, k and their gradients */
+  int32_t head_dim;      /* even, 2 .. 256 */
+  int32_t heads_q, heads_k;
+  int32_t interleaved;
+  int32_t position_bits; /* 0: a token's index is its position; 32 / 64: element size of positions */
+  int64_t batch, tokens; /* batch * tokens < 2^31 */
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3], dq_out_stride[3], dk_out_stride[3]; /* batch, token, head */
+  int64_t position_stride[2]; /* batch, token */
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const float* q_gain;   /* [head_dim] */
+  const float* k_gain;
+  const uint64_t* phase; /* [head_dim / 2]: round(2^64 * freq_i / (2 pi)), the turn per position */
+  const void* positions; /* int32 / int64 */
+  const void* dq_out;    /* backward only, as all below */
+  const void* dk_out;
+  float* dq_gain;
+  float* dk_gain;
+  float* workspace;      /* mgbs_qk_norm_rope_backward_workspace(head_dim) bytes */
+  float eps;
+  int32_t reserved;
+} MgbsQkNormArgs;
+int mgbs_sizeof_qk_norm_args(void);
+int mgbs_qk_norm_rope(const MgbsQkNormArgs* args, void* stream);
+int64_t mgbs_qk_norm_rope_backward_workspace(int32_t head_dim);
+int mgbs_qk_norm_rope_backward(const MgbsQkNormArgs* args, void* stream);
+
+/* Softmax attention with a learned bias per head and distance bucket:
+ *   out_i = sum_j softmax_j(scale q_i . k_j + table[bucket(j - i), head]) v_j.
+ * Query heads share key heads in runs of heads / heads_kv.  With lengths, tokens of a sequence from its length on are
+ * no keys, are never read, and their outputs and gradients are 0; causal leaves only keys j <= i.  Strides in
+ * elements (batch, token, head), the last dimension 1; q, k, v, dout on 16-byte boundaries (base and strides).
+ * out, dq, dk, dv are contiguous. */
+typedef struct MgbsRelAttentionArgs {
+  int32_t dtype;     /* MGBS_DT_BF16 or MGBS_DT_F16: q, k, v, table, out and all gradients */
+  int32_t head_dim;  /* 32 or 64 */
+  int32_t heads, heads_kv;
+  int64_t batch, tokens; /* tokens <= 2^20 */
+  int64_t q_stride[3], k_stride[3], v_stride[3], dout_stride[3];
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* table;         /* [num_buckets, heads] contiguous */
+  const int32_t* bucket_map; /* [2 * max_distance + 1]: bucket of key minus query, from -max_distance on; the ends' buckets hold for all further ones */
+  const int32_t* bucket_order; /* [2 * max_distance + 1]: the map's places, sorted by bucket */
+  const int32_t* bucket_start; /* [num_buckets + 1]: where each bucket's places begin in bucket_order */
+  const int32_t* lengths;    /* [batch] or null */
+  void* out;
+  float* stats;      /* [batch, heads, tokens, 2] softmax statistics, or null: needed for a backward call when tokens > 64 or
+                      * heads != heads_kv, written by the forward and read by the backward */
+  int32_t num_buckets, max_distance; /* 1 .. 512, 1 .. 1024 */
+  int32_t causal;
+  float scale;       /* > 0 */
+  const void* dout;  /* backward only, as all below */
+  void* dq;
+  void* dk;
+  void* dv;
+  void* dtable;      /* [num_buckets, heads] */
+  void* workspace;   /* mgbs_rel_attention_backward_workspace() bytes, 16-byte aligned */
+} MgbsRelAttentionArgs;
+int mgbs_sizeof_rel_attention_args(void);
+int mgbs_rel_attention(const MgbsRelAttentionArgs* args, void* stream);
+int64_t mgbs_rel_attention_backward_workspace(const MgbsRelAttentionArgs* args);
+/* out and stats are those of the forward call on the same inputs. */
+int mgbs_rel_attention_backward(const MgbsRelAttentionArgs* args, void* stream);
+
+/* Distillation from a teacher's top entries.  Per row, with p = softmax(teacher / temperature) over the held entries
+ * (those whose index lies in [0, width)): loss = sum_k p_k (log p_k - log softmax(logits / temperature)[index_k]);
+ * grad = row_weight * dloss/dlogits.  An index given twice counts with both probabilities; a row that holds no entry
+ * (or only entries at -inf) has loss 0 and gradient 0. */
+#define MGBS_DISTILL_MAX_ENTRIES 1024
+typedef struct MgbsDistillArgs {
+  int32_t dtype;       /* MGBS_DT_* of logits and grad */
+  int32_t entries;     /* 1 .. MGBS_DISTILL_MAX_ENTRIES */
+  int64_t rows;
+  int32_t width;       /* row length of the logits */
+  int32_t index_bits;  /* 32 or 64 */
+  int64_t row_stride, grad_stride, teacher_stride, index_stride; /* elements; the last dimension has stride 1 */
+  const void* logits;
+  const float* teacher;
+  const void* index;
+  const float* row_weight; /* [rows] or null (1); only for grad */
+  float* loss;             /* [rows] */
+  void* grad;              /* null: loss only */
+  float temperature;       /* > 0 */
+  int32_t reserved;
+} MgbsDistillArgs;
+int mgbs_sizeof_distill_args(void);
+int mgbs_distill_top_logits(const MgbsDistillArgs* args, void* stream);
+
 /* Host-side helpers with the device's exact arithmetic (data_loader.hash_state_cpu, data_loader.py:192-213). */
 uint64_t mgbs_hash64_host(const uint8_t* state, int32_t n);
 uint64_t mgbs_fingerprint64_host(const uint8_t* state, int32_t n);

@@ -2,4 +2,4 @@
 
 from . import puzzles  # noqa: F401
 
-__all__ = ["puzzles", "beam_engine", "records"]
+__all__ = ["puzzles", "beam_engine", "records", "scorers", "operators"]
