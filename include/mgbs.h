@@ -479,6 +479,10 @@ typedef struct MgbsTfLayer {
    * e4m3 tensor that feeds it (LN1 output, attention output, LN2 output, GELU output). */
   const float* cs_qkv; const float* cs_o; const float* cs_1; const float* cs_2;
   float inv_y1, inv_att, inv_y2, inv_hid;
+  /* Optional (null: absent).  q_gain, k_gain [32] f32: queries and keys go through mgbs_qk_norm_rope before the attention,
+   * with the encoder's rotary_phase.  rel_table [rel_buckets, 8] bf16: the attention is mgbs_rel_attention (dtype 0). */
+  const float* q_gain; const float* k_gain;
+  const void* rel_table;
 } MgbsTfLayer;
 typedef struct MgbsTfConfig {
   int32_t state_len, state_stride, num_values, d_model, heads, ffn, layers, encoders;
@@ -499,7 +503,12 @@ typedef struct MgbsTfConfig {
   float* q;     /* f32 [max_states] */
   int32_t* err;
   int32_t dtype; /* GEMM operand type: 0 = bf16, 1 = e4m3 (float32 accumulation, residual stream and softmax either way) */
-  int32_t reserved;
+  float qk_eps;  /* of the layers' query and key norm */
+  const uint64_t* rotary_phase[MGBS_TF_MAX_ENCODERS]; /* [16], with q_gain; zeros turn nothing */
+  const int32_t* rel_map;    /* with rel_table: bucket_map, bucket_order and bucket_start of MgbsRelAttentionArgs */
+  const int32_t* rel_order;
+  const int32_t* rel_start;
+  int32_t rel_buckets, rel_distance;
 } MgbsTfConfig;
 typedef struct MgbsTf MgbsTf;
 int mgbs_sizeof_tf_config(void);

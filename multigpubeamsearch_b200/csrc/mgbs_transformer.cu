@@ -18,6 +18,7 @@
 #include <new>
 
 #include "mgbs.h"
+#include "mgbs_counted.cuh"
 #include "mgbs_tc.cuh"
 
 namespace mgbs {
@@ -631,6 +632,9 @@ int mgbs_tf_create(const MgbsTfConfig* cfg, MgbsTf** out) {
       if (!L.ln1_g || !L.ln1_b || !L.wqkv || !L.bqkv || !L.wo || !L.bo || !L.ln2_g || !L.ln2_b || !L.w1 || !L.b1 ||
           !L.w2 || !L.b2)
         rc = MGBS_ERR_ARG;
+      if (!rc && ((!L.q_gain != !L.k_gain) || (L.q_gain && !c.rotary_phase[e]))) rc = MGBS_ERR_ARG;
+      if (!rc && L.rel_table && c.dtype != 0) rc = MGBS_ERR_UNSUPPORTED;
+      if (!rc && L.rel_table && (!c.rel_map || !c.rel_order || !c.rel_start)) rc = MGBS_ERR_ARG;
       if (!rc && c.dtype == 1 && (!L.cs_qkv || !L.cs_o || !L.cs_1 || !L.cs_2)) rc = MGBS_ERR_ARG;
       if (!rc) rc = mgbs::make_map(&t->tm_wqkv[e][l], L.wqkv, 768, 256, mgbs::BN, eb);
       if (!rc) rc = mgbs::make_map(&t->tm_wo[e][l], L.wo, 256, 256, mgbs::BN, eb);
@@ -657,6 +661,39 @@ int mgbs_tf_create(const MgbsTfConfig* cfg, MgbsTf** out) {
 int mgbs_tf_destroy(MgbsTf* t) {
   delete t;
   return 0;
+}
+
+// The layer's queries and keys normalised and rotated in place in the qkv buffer.
+static int tf_norm_rope(const MgbsTfConfig& c, const MgbsTfLayer& L, int encoder, const uint32_t* count_dev, int64_t first, void* stream) {
+  MgbsQkNormArgs a = {};
+  a.dtype = MGBS_DT_BF16;
+  a.head_dim = 32; a.heads_q = a.heads_k = 8;
+  a.batch = c.micro_batch; a.tokens = c.state_len;
+  const int64_t stride[3] = {(int64_t)c.state_len * 768, 768, 32};
+  for (int i = 0; i < 3; ++i) a.q_stride[i] = a.k_stride[i] = a.q_out_stride[i] = a.k_out_stride[i] = stride[i];
+  __nv_bfloat16* qkv = reinterpret_cast<__nv_bfloat16*>(c.qkv);
+  a.q = a.q_out = qkv;
+  a.k = a.k_out = qkv + 256;
+  a.q_gain = L.q_gain; a.k_gain = L.k_gain; a.phase = c.rotary_phase[encoder];
+  a.eps = c.qk_eps;
+  return mgbs::qk_norm_rope_counted(&a, count_dev, first, stream);
+}
+
+static int tf_rel_attention(const MgbsTfConfig& c, const MgbsTfLayer& L, const uint32_t* count_dev, int64_t first, void* stream) {
+  MgbsRelAttentionArgs a = {};
+  a.dtype = MGBS_DT_BF16;
+  a.head_dim = 32; a.heads = a.heads_kv = 8;
+  a.batch = c.micro_batch; a.tokens = c.state_len;
+  const int64_t stride[3] = {(int64_t)c.state_len * 768, 768, 32};
+  for (int i = 0; i < 3; ++i) a.q_stride[i] = a.k_stride[i] = a.v_stride[i] = stride[i];
+  const __nv_bfloat16* qkv = reinterpret_cast<const __nv_bfloat16*>(c.qkv);
+  a.q = qkv; a.k = qkv + 256; a.v = qkv + 512;
+  a.table = L.rel_table;
+  a.bucket_map = c.rel_map; a.bucket_order = c.rel_order; a.bucket_start = c.rel_start;
+  a.num_buckets = c.rel_buckets; a.max_distance = c.rel_distance;
+  a.out = c.att;
+  a.scale = 0.17677669529663687f;  // 1 / sqrt(32)
+  return mgbs::rel_attention_counted(&a, count_dev, first, stream);
 }
 
 int mgbs_tf_enqueue(void* user, const uint8_t* children, const uint32_t* count_dev, uint32_t* scores, void* stream) {
@@ -690,11 +727,24 @@ int mgbs_tf_enqueue(void* user, const uint8_t* children, const uint32_t* count_d
           k_tf_layernorm<1><<<ew_grid, 256, 0, st>>>(c.x, count_dev, T, off, t->mb_rows, L.ln1_g, L.ln1_b, c.y, L.inv_y1);
           g.col_scale = L.cs_qkv;
           k_tf_gemm<TF_EPI_STORE, 1><<<gg, gb, TF_SMEM, st>>>(t->tm_y, t->tm_wqkv[e][l], t->tm_qkv_st, g);
+          if (L.q_gain) {
+            const int rc = tf_norm_rope(c, L, e, count_dev, mb * c.micro_batch, stream);
+            if (rc) return rc;
+          }
           k_tf_attention<1><<<t->sms * 2, TF_ATT_WARPS * 32, TF_ATT_SMEM, st>>>(qkv, count_dev, T, off, t->mb_rows, c.att, L.inv_att);
         } else {
           k_tf_layernorm<0><<<ew_grid, 256, 0, st>>>(c.x, count_dev, T, off, t->mb_rows, L.ln1_g, L.ln1_b, c.y, 1.f);
           k_tf_gemm<TF_EPI_STORE, 0><<<gg, gb, TF_SMEM, st>>>(t->tm_y, t->tm_wqkv[e][l], t->tm_qkv_st, g);
-          k_tf_attention<0><<<t->sms * 2, TF_ATT_WARPS * 32, TF_ATT_SMEM, st>>>(qkv, count_dev, T, off, t->mb_rows, c.att, 1.f);
+          if (L.q_gain) {
+            const int rc = tf_norm_rope(c, L, e, count_dev, mb * c.micro_batch, stream);
+            if (rc) return rc;
+          }
+          if (L.rel_table) {
+            const int rc = tf_rel_attention(c, L, count_dev, mb * c.micro_batch, stream);
+            if (rc) return rc;
+          } else {
+            k_tf_attention<0><<<t->sms * 2, TF_ATT_WARPS * 32, TF_ATT_SMEM, st>>>(qkv, count_dev, T, off, t->mb_rows, c.att, 1.f);
+          }
         }
         g.n_total = 256; g.k_total = 256; g.bias = L.bo;
         if (f8) {

@@ -14,7 +14,7 @@ from typing import Any, Dict, List, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, operators
 from .records import unpack_payload  # noqa: F401  (re-exported for callers of the engine)
 
 MAX_MODELS = 4
@@ -538,6 +538,13 @@ class MLPActionScorer(torch.nn.Module):
             x = torch.nn.functional.gelu(lin(x))
         return self.out(x)
 
+    def distillation_loss(self, states_u8: torch.Tensor, teacher_values: torch.Tensor, teacher_moves: torch.Tensor,
+                          temperature: float = 1.0) -> torch.Tensor:
+        """Mean divergence (operators.distill_top_logits) of this scorer's move values from a teacher's best moves on the
+        same states: ``teacher_values`` and ``teacher_moves`` [B, entries], e.g. the topk of a wide ensemble's values;
+        moves outside [0, fanout) are padding.  Larger is better on both sides.  CUDA only."""
+        return operators.distill_top_logits(self(states_u8), teacher_values, teacher_moves, temperature=temperature).mean()
+
 
 class QuantizedActionScorer(torch.nn.Module):
     """16-bit quantiser around a base scorer (scorers.QuantizedActionScorer, scorers.py:38-53): "sigmoid_u16" =
@@ -702,7 +709,8 @@ E4M3_MAX = 448.0
 class MgbsTfLayer(C.Structure):
     _fields_ = ([(name, C.c_void_p) for name in _LAYER_FIELDS]
                 + [(name, C.c_void_p) for name in ("cs_qkv", "cs_o", "cs_1", "cs_2")]
-                + [(name, C.c_float) for name in ("inv_y1", "inv_att", "inv_y2", "inv_hid")])
+                + [(name, C.c_float) for name in ("inv_y1", "inv_att", "inv_y2", "inv_hid")]
+                + [(name, C.c_void_p) for name in ("q_gain", "k_gain", "rel_table")])
 
 
 class MgbsTfConfig(C.Structure):
@@ -716,7 +724,10 @@ class MgbsTfConfig(C.Structure):
         ("w_head", C.c_void_p * TF_MAX_ENCODERS),
         ("layer", (MgbsTfLayer * TF_MAX_LAYERS) * TF_MAX_ENCODERS),
         ("x", C.c_void_p), ("y", C.c_void_p), ("qkv", C.c_void_p), ("att", C.c_void_p), ("hid", C.c_void_p),
-        ("q", C.c_void_p), ("err", C.c_void_p), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("q", C.c_void_p), ("err", C.c_void_p), ("dtype", C.c_int32), ("qk_eps", C.c_float),
+        ("rotary_phase", C.c_void_p * TF_MAX_ENCODERS),
+        ("rel_map", C.c_void_p), ("rel_order", C.c_void_p), ("rel_start", C.c_void_p),
+        ("rel_buckets", C.c_int32), ("rel_distance", C.c_int32),
     ]
 
 
@@ -739,7 +750,14 @@ class TransformerValueScorer:
     e4m3 activations (LayerNorm output, attention output, GELU output) with one scale per tensor.  The activation
     scales come from bounds that hold for every input (a LayerNorm row has L2 norm 16 before its gain, so
     |row . w| <= (16 max|gain| + |shift|) |w|), not from calibration data; q, k, v stay bf16 for the attention
-    kernel.  ``dtype="nvfp4_weights"`` rounds the same matrices to the NVFP4 grid and runs them on the bf16 path."""
+    kernel.  ``dtype="nvfp4_weights"`` rounds the same matrices to the NVFP4 grid and runs them on the bf16 path.
+
+    Encoders may bring relative positions (TransformerValueNet.encoder_weights has them all): layers with ``q_gain`` and
+    ``k_gain`` [32] normalise queries and keys per head (``qk_eps`` of the encoder, 1e-6 by default) and rotate them by
+    position (``rotary_base`` of the encoder; None turns nothing), operators.qk_norm_rope; layers with ``rel_table``
+    [num_buckets, 8] add a learned bias by distance (``rel_buckets`` of the encoder: (num_buckets, max_distance), (32, 128)
+    by default), operators.relative_attention, its table held in bfloat16 and not available with ``dtype="fp8"``.  All
+    encoders share qk_eps and rel_buckets."""
 
     def __init__(self, encoders: Sequence[Dict], state_len: int, state_stride: int, num_values: int, max_rows: int,
                  micro_batch: int = 32768, score_offset: float = -150.0, device=None, dtype: str = "bf16"):
@@ -829,6 +847,7 @@ class TransformerValueScorer:
                     dst.w1, dst.cs_1 = e4m3(L["w1"], s_y2)
                     dst.w2, dst.cs_2 = e4m3(L["w2"], s_hid)
                     dst.inv_y1, dst.inv_att, dst.inv_y2, dst.inv_hid = 1 / s_y1, 1 / s_att, 1 / s_y2, 1 / s_hid
+        self._relative_positions(cfg, encoders, dev, fp8, f32)
         act = torch.uint8 if fp8 else torch.bfloat16
         self.x = torch.zeros((rows_pad, d), dtype=torch.float32, device=dev)
         self.y = torch.zeros((rows_pad, d), dtype=act, device=dev)
@@ -844,6 +863,41 @@ class TransformerValueScorer:
         h = C.c_void_p()
         _lib.check(self.lib.mgbs_tf_create(C.byref(cfg), C.byref(h)), "TransformerValueScorer")
         self._h = h
+
+    def _relative_positions(self, cfg, encoders, dev, fp8, f32) -> None:
+        """Query/key norm, rotation and distance biases of the encoders that bring them."""
+        shared = {(float(w.get("qk_eps", 1e-6)), tuple(w.get("rel_buckets", (32, 128)))) for w in encoders}
+        if len(shared) != 1:
+            raise RuntimeError("all encoders must share qk_eps and rel_buckets")
+        eps, (num_buckets, max_distance) = shared.pop()
+        for e, w in enumerate(encoders):
+            for li, L in enumerate(w["layers"]):
+                dst = cfg.layer[e][li]
+                if ("q_gain" in L) != ("k_gain" in L):
+                    raise RuntimeError("a layer has q_gain and k_gain or neither")
+                if "q_gain" in L:
+                    if np.shape(L["q_gain"]) != (32,) or np.shape(L["k_gain"]) != (32,):
+                        raise RuntimeError("q_gain and k_gain must be [32]")
+                    dst.q_gain, dst.k_gain = f32(L["q_gain"]), f32(L["k_gain"])
+                    if not cfg.rotary_phase[e]:
+                        base = w.get("rotary_base", 10000.0)
+                        rotary = operators.RotaryFrequencies(32, device=dev, **({"inv_freq": [0.0] * 16} if base is None else {"base": base}))
+                        self._keep.append(rotary.phase)
+                        cfg.rotary_phase[e] = rotary.phase.data_ptr()
+                if "rel_table" in L:
+                    if fp8:
+                        raise RuntimeError('rel_table is not available with dtype="fp8"')
+                    if np.shape(L["rel_table"]) != (num_buckets, 8):
+                        raise RuntimeError(f"rel_table must be [{num_buckets}, 8]")
+                    table = torch.from_numpy(np.ascontiguousarray(L["rel_table"], dtype=np.float32)).to(dev).to(torch.bfloat16).contiguous()
+                    self._keep.append(table)
+                    dst.rel_table = table.data_ptr()
+                    if not cfg.rel_map:
+                        plan = operators.RelativeBuckets(num_buckets, max_distance, device=dev)
+                        self._keep.append(plan)
+                        cfg.rel_map, cfg.rel_order, cfg.rel_start = plan.map.data_ptr(), plan.order.data_ptr(), plan.start.data_ptr()
+                        cfg.rel_buckets, cfg.rel_distance = num_buckets, max_distance
+        cfg.qk_eps = eps
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -877,3 +931,73 @@ class TransformerValueScorer:
 
     def error_code(self) -> int:
         return int(self.err.item())
+
+
+class TransformerValueNet(torch.nn.Module):
+    """Trainable form of one encoder of TransformerValueScorer with relative positions: uint8 states [B, >= state_len] ->
+    float32 values [B].  Per layer x += W_o attention(LN1 x), x += W2 gelu(W1 LN2 x), where queries and keys are
+    normalised per head and rotated by position (operators.qk_norm_rope) and the attention has a learned bias per head
+    and distance bucket (operators.relative_attention); d_model 256, 8 heads.  The residual stream and all norms are
+    float32, the matrix products and the attention take bfloat16.  CUDA only.  ``encoder_weights()`` is the dictionary
+    that TransformerValueScorer loads."""
+
+    D, HEADS, EPS = 256, 8, 1e-6
+
+    def __init__(self, state_len: int, num_values: int, layers: int = 4, ffn: int = 1024, rotary_base: Optional[float] = 10000.0,
+                 rel_buckets: Sequence[int] = (32, 128), std: float = 0.02):
+        super().__init__()
+        d = self.D
+        if not 1 <= state_len <= 64 or not 1 <= layers <= TF_MAX_LAYERS or ffn % 256 or ffn < 256:
+            raise RuntimeError(f"state_len 1..64, layers 1..{TF_MAX_LAYERS}, ffn a multiple of 256")
+        self.state_len, self.num_values, self.rotary_base, self.rel_buckets = int(state_len), int(num_values), rotary_base, tuple(rel_buckets)
+
+        def g(*shape):
+            return torch.nn.Parameter(torch.randn(shape) * std)
+
+        def const(value, *shape):
+            return torch.nn.Parameter(torch.full(shape, float(value)))
+
+        self.tok_emb, self.pos_emb = g(num_values, d), g(state_len, d)
+        self.layers = torch.nn.ModuleList()
+        for _ in range(layers):
+            layer = torch.nn.Module()
+            for name, p in (("ln1_g", const(1, d)), ("ln1_b", const(0, d)), ("wqkv", g(3 * d, d)), ("bqkv", const(0, 3 * d)), ("wo", g(d, d)),
+                            ("bo", const(0, d)), ("ln2_g", const(1, d)), ("ln2_b", const(0, d)), ("w1", g(ffn, d)), ("b1", const(0, ffn)),
+                            ("w2", g(d, ffn)), ("b2", const(0, d)), ("q_gain", const(1, 32)), ("k_gain", const(1, 32)),
+                            ("rel_table", const(0, self.rel_buckets[0], self.HEADS))):
+                layer.register_parameter(name, p)
+            self.layers.append(layer)
+        self.lnf_g, self.lnf_b, self.w_head, self.b_head = const(1, d), const(0, d), g(d), const(0)
+        self._plans: Dict[torch.device, Any] = {}
+
+    def _plan(self, device):
+        if device not in self._plans:
+            freq = {"inv_freq": [0.0] * 16} if self.rotary_base is None else {"base": self.rotary_base}
+            self._plans[device] = (operators.RotaryFrequencies(32, device=device, **freq), operators.RelativeBuckets(*self.rel_buckets, device=device))
+        return self._plans[device]
+
+    def forward(self, states_u8: torch.Tensor) -> torch.Tensor:
+        F, d, bf = torch.nn.functional, self.D, torch.bfloat16
+        s = states_u8[:, : self.state_len].long()
+        batch, tokens = s.shape
+        rotary, buckets = self._plan(states_u8.device)
+        x = self.tok_emb[s] + self.pos_emb
+
+        def linear(y, w, b):
+            return F.linear(y.to(bf), w.to(bf), b.to(bf))
+
+        for L in self.layers:
+            qkv = linear(F.layer_norm(x, (d,), L.ln1_g, L.ln1_b), L.wqkv, L.bqkv).view(batch, tokens, 3, self.HEADS, 32)
+            q, k = operators.qk_norm_rope(qkv[:, :, 0], qkv[:, :, 1], L.q_gain, L.k_gain, rotary, eps=self.EPS)
+            att = operators.relative_attention(q, k, qkv[:, :, 2], L.rel_table.to(bf), buckets)
+            x = x + linear(att.reshape(batch, tokens, d), L.wo, L.bo)
+            x = x + linear(F.gelu(linear(F.layer_norm(x, (d,), L.ln2_g, L.ln2_b), L.w1, L.b1)), L.w2, L.b2)
+        return F.layer_norm(x, (d,), self.lnf_g, self.lnf_b).mean(1) @ self.w_head + self.b_head
+
+    def encoder_weights(self) -> Dict[str, Any]:
+        """The weights as TransformerValueScorer takes them (float32 arrays)."""
+        names = _LAYER_FIELDS + ("q_gain", "k_gain", "rel_table")
+        return {"tok_emb": _np(self.tok_emb), "pos_emb": _np(self.pos_emb), "lnf_g": _np(self.lnf_g), "lnf_b": _np(self.lnf_b),
+                "w_head": _np(self.w_head), "b_head": np.float32(self.b_head.item()), "qk_eps": self.EPS,
+                "rotary_base": self.rotary_base, "rel_buckets": self.rel_buckets,
+                "layers": [{n: _np(getattr(L, n)) for n in names} for L in self.layers]}

@@ -769,6 +769,28 @@ def _e4m3_tensor(x: np.ndarray, bound: float) -> np.ndarray:
     return round_e4m3(x * np.float32(1.0 / scale)) * scale
 
 
+def _norm_rotate(x: np.ndarray, gain: np.ndarray, base, eps: float) -> np.ndarray:
+    """Heads [..., tokens, hd] over their root mean square, times the gain, with the pairs (i, i + hd/2) turned by
+    token * base^(-2 i / hd) (base None: not turned)."""
+    hd = x.shape[-1]
+    x = x / np.sqrt((x.astype(np.float64) ** 2).mean(axis=-1, keepdims=True) + eps) * gain
+    z = x[..., : hd // 2] + 1j * x[..., hd // 2:]
+    if base is not None:
+        z = z * np.exp(1j * np.arange(x.shape[-2])[:, None] * float(base) ** (-np.arange(hd // 2) * 2.0 / hd))
+    return np.concatenate([z.real, z.imag], axis=-1).astype(np.float32)
+
+
+def _relative_buckets(tokens: int, num_buckets: int, max_distance: int) -> np.ndarray:
+    """Bucket of (query, key): per side half the buckets for single distances, the rest in equal factors up to
+    max_distance; keys after the query in the upper half."""
+    side = num_buckets // 2
+    exact = side // 2
+    off = np.arange(tokens)[None, :] - np.arange(tokens)[:, None]
+    n = np.abs(off)
+    grown = np.floor(np.log(np.maximum(n, 1) / exact) / np.log(max_distance / exact) * (side - exact) + 1e-9)
+    return np.where(n < exact, n, np.minimum(exact + grown, side - 1)).astype(np.int64) + side * (off > 0)
+
+
 def transformer_forward(states: np.ndarray, encoders: Sequence[Dict], heads: int = 8, e4m3: bool = False) -> np.ndarray:
     """float32 pre-LayerNorm transformer encoder ensemble on token states; mean over members.
 
@@ -807,7 +829,11 @@ def transformer_forward(states: np.ndarray, encoders: Sequence[Dict], heads: int
             if e4m3:
                 qkv = round_bf16(qkv.astype(np.float32))
             q, k, v = (qkv[..., i * d:(i + 1) * d].reshape(c, t, heads, hd).transpose(0, 2, 1, 3) for i in range(3))
+            if "q_gain" in L:
+                q, k = (_norm_rotate(x_, L[g], w.get("rotary_base", 10000.0), w.get("qk_eps", 1e-6)) for x_, g in ((q, "q_gain"), (k, "k_gain")))
             att = (q @ k.transpose(0, 1, 3, 2)) / np.float32(np.sqrt(hd))
+            if "rel_table" in L:
+                att = att + L["rel_table"][_relative_buckets(t, *w.get("rel_buckets", (32, 128)))].transpose(2, 0, 1)
             att = att - att.max(axis=-1, keepdims=True)
             att = np.exp(att)
             if e4m3:

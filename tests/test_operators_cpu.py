@@ -156,3 +156,11 @@ def test_empty_calls_do_nothing():
 def test_error_names():
     with pytest.raises(RuntimeError, match="too large"):
         _lib.check(ERR_TOO_LARGE, "relative_attention")
+
+
+def test_transformer_config_mirrors():
+    from multigpubeamsearch_b200 import scorers
+
+    lib = ops._load()
+    lib.mgbs_sizeof_tf_config.restype = C.c_int
+    assert lib.mgbs_sizeof_tf_config() == C.sizeof(scorers.MgbsTfConfig)
