@@ -5,8 +5,10 @@
 //
 // What bounds it: bytes (x read, y written; backward x, dy read, dx written).  A group of lanes owns one head vector,
 // each lane eight pairs, so that both members of a pair are in one lane, loads and stores are 16 bytes wide and the
-// only exchange is the sum of squares.  Sines and cosines are shared by all heads of a token: the block computes them
-// once per token into shared memory while the loads of the vectors are in flight.
+// only exchange is the sum of squares.  The lanes of a token's query and key heads are the columns of a block: a thread
+// stays in its column and walks over tokens, several in flight at a time, so that its gains stay in registers and
+// nothing is divided per vector.  Sines and cosines are shared by all heads of a token through shared memory: once per
+// block where positions do not depend on the sequence and fit, else once per step.
 //
 // Angles: position * freq / (2 pi) is taken modulo one turn as a 64-bit integer product (freq comes as 2^64 times
 // its turns per position), exact for any 64-bit position: no table, no range limit, no loss at far positions.
@@ -25,7 +27,7 @@ struct QkTensor {
   const float* gain;
   int64_t xs[3], ys[3], ds[3];  // strides of x, y (dx) and dy in elements: batch, token, head
   int32_t heads;
-  int32_t flat;  // every tensor's batch stride is tokens * token stride
+  int32_t pad;
 };
 struct QkArgs {
   QkTensor t[2];  // queries, keys
@@ -36,18 +38,24 @@ struct QkArgs {
   int64_t count_offset;
   int32_t pos_bits;  // 0 = token index, 32 or 64 = element size of positions
   int32_t batch, tokens, head_dim, lanes;  // lanes: per head vector, a power of two
-  int32_t tile;                            // tokens per block iteration
+  int32_t cols;      // columns (lanes of a token's heads) per block, blockIdx.y picks which
+  int32_t step;      // tokens side by side in a block
+  int32_t step_b, step_t;  // step = step_b * tokens + step_t
+  int32_t span;      // tokens per block and turn of its loop: step, or step times the tokens in flight per thread
   float eps;
-  float* partial;  // backward: [2][gridDim.x][head_dim] sums of the gain gradients
+  float* partial;    // backward: [blocks][2][head_dim] sums of the gains' gradients
 };
 
 constexpr int QK_THREADS = 256;
-constexpr int QK_ITEMS = 2;  // vectors parts in flight per thread
 
 // The 16 elements of a lane (8 pairs): a[i], b[i].
 template <typename T, bool INTER, bool VEC> struct PairIo {
   static constexpr int R = (int)sizeof(T);  // 16-byte registers of a lane: 16 * sizeof(T) / 16
   uint4 raw[R];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < R; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
   __device__ __forceinline__ void load(const T* p, int chunk, int half) {
     if (VEC) {
       const uint4* lo = reinterpret_cast<const uint4*>(p + (INTER ? 16 * chunk : 8 * chunk));
@@ -103,37 +111,46 @@ __device__ __forceinline__ int64_t qk_batch(const QkArgs& g) {
   return left < 0 ? 0 : (left < g.batch ? left : g.batch);
 }
 
-// (cos, sin) of the tile's tokens: cs[token][pair].
-__device__ __forceinline__ void qk_angles(const QkArgs& g, uint32_t first, uint32_t count, float2* cs) {
-  const uint32_t half = g.head_dim / 2;
-  for (uint32_t i = threadIdx.x; i < count * half; i += QK_THREADS) {
-    const uint32_t tok = i / half, pair = i - tok * half;
-    const uint32_t n = first + tok, b = n / (uint32_t)g.tokens, t = n - b * (uint32_t)g.tokens;
+// A thread's pairs of a run of tokens: i = thread, thread + threads, ...; only the first is divided.
+struct QkPairs {
+  uint32_t tok, pair, add_tok, add_pair, half;
+  __device__ __forceinline__ explicit QkPairs(uint32_t half_) : half(half_) {
+    tok = threadIdx.x / half;
+    pair = threadIdx.x - tok * half;
+    add_tok = blockDim.x / half;
+    add_pair = blockDim.x - add_tok * half;
+  }
+};
+
+// (cos, sin) of `count` tokens from token `first` of all sequences on: cs[token][pair].  For 16-bit results the fast sine
+// and cosine (absolute error 2^-21 on one turn) are far below their rounding.
+template <bool FAST> __device__ __forceinline__ void qk_angles(const QkArgs& g, QkPairs p, uint32_t first, uint32_t count, float2* cs) {
+  while (p.tok < count) {
+    const uint32_t n = first + p.tok, b = n / (uint32_t)g.tokens, t = n - b * (uint32_t)g.tokens;
     const int64_t at = (int64_t)b * g.pos_sb + (int64_t)t * g.pos_st;
     const int64_t pos = g.pos_bits == 64 ? static_cast<const int64_t*>(g.positions)[at]
                         : g.pos_bits == 32 ? (int64_t) static_cast<const int32_t*>(g.positions)[at] : (int64_t)t;
-    const uint64_t turns = (uint64_t)pos * g.phase[pair];  // modulo one turn = 2^64
+    const float turns = (float)(int32_t)(((uint64_t)pos * __ldg(g.phase + p.pair)) >> 32);  // modulo one turn: signed, 2^-32 each
     float s, c;
-    sincospif((float)(int32_t)(turns >> 32) * 4.656612873077393e-10f, &s, &c);  // 2^-31: signed half turns
-    cs[i] = make_float2(c, s);
+    if (FAST) __sincosf(turns * 1.4629180792671596e-9f, &s, &c);  // 2 pi / 2^32
+    else sincospif(turns * 4.656612873077393e-10f, &s, &c);       // 2^-31: half turns
+    cs[p.tok * p.half + p.pair] = make_float2(c, s);
+    p.tok += p.add_tok;
+    p.pair += p.add_pair;
+    if (p.pair >= p.half) { p.pair -= p.half; ++p.tok; }
   }
 }
 
-__device__ __forceinline__ const float4* qk_cs(const float2* cs, uint32_t tok, int half, int chunk) {
-  return reinterpret_cast<const float4*>(cs + tok * half + chunk * 8);
-}
-
 // Rotation coefficients of a lane's eight pairs; pairs past `half` read nothing.
-template <bool VEC> __device__ __forceinline__ void qk_read_cs(const float2* cs, uint32_t tok, int half, int chunk, float (&c)[8], float (&s)[8]) {
+template <bool VEC> __device__ __forceinline__ void qk_read_cs(const float2* cs, int chunk, int half, float (&c)[8], float (&s)[8]) {
   if (VEC) {
-    const float4* p = qk_cs(cs, tok, half, chunk);
+    const float4* p = reinterpret_cast<const float4*>(cs + chunk * 8);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { const float4 f = p[i]; c[2 * i] = f.x; s[2 * i] = f.y; c[2 * i + 1] = f.z; s[2 * i + 1] = f.w; }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = 8 * chunk + i < half;
-      const float2 f = in ? cs[tok * half + chunk * 8 + i] : make_float2(0.f, 0.f);
+      const float2 f = 8 * chunk + i < half ? cs[chunk * 8 + i] : make_float2(0.f, 0.f);
       c[i] = f.x; s[i] = f.y;
     }
   }
@@ -148,199 +165,152 @@ template <bool INTER> __device__ __forceinline__ void qk_gains(const float* gain
   }
 }
 
-__device__ __forceinline__ int64_t qk_offset(const QkArgs& g, int flat, const int64_t (&s)[3], uint32_t n, int head) {
-  if (flat) return (int64_t)n * s[1] + head * s[2];
-  const uint32_t b = n / (uint32_t)g.tokens;
-  return (int64_t)b * s[0] + (int64_t)(n - b * (uint32_t)g.tokens) * s[1] + head * s[2];
-}
-
 __device__ __forceinline__ float group_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Queries and keys of a token are one run of heads, so both share the token's angles.
-template <typename T, bool INTER, bool VEC>
-__global__ void __launch_bounds__(QK_THREADS) k_qk_norm_rope(const __grid_constant__ QkArgs g) {
-  extern __shared__ __align__(16) float2 cs[];
+// BWD 0: y from x.  BWD 1: dx from x and dy, and the block's sums of the gains' gradients.  U tokens in flight per thread.
+// SHARED: the angles of all `tokens` positions are kept for the whole block.
+template <typename T, bool INTER, bool VEC, int U, bool BWD, bool SHARED>
+__global__ void __launch_bounds__(QK_THREADS, BWD ? 2 : 3) k_qk_norm_rope(const __grid_constant__ QkArgs g) {
+  extern __shared__ __align__(16) float2 angles[];
+  float2* cs = angles;
+  int odd = 0;
+  using Io = PairIo<T, INTER, VEC>;
   const uint32_t total = (uint32_t)(qk_batch(g) * g.tokens);
   const int half = g.head_dim / 2, lanes = g.lanes;
-  const int chunk = threadIdx.x & (lanes - 1);
-  const bool busy = chunk * 8 < half;
-  const uint32_t row = (uint32_t)(g.t[0].heads + g.t[1].heads) * lanes;  // lanes of one token
-  const float inv_d = 1.f / (float)g.head_dim;
-  for (uint64_t first = (uint64_t)blockIdx.x * g.tile; first < total; first += (uint64_t)gridDim.x * g.tile) {
-    const uint32_t count = min((uint32_t)g.tile, total - (uint32_t)first);
-    const uint32_t items = count * row;
-    for (uint32_t base = 0; base < items; base += QK_THREADS * QK_ITEMS) {
-      PairIo<T, INTER, VEC> io[QK_ITEMS];
-      uint32_t tok[QK_ITEMS];
-      int head[QK_ITEMS];
-#pragma unroll
-      for (int u = 0; u < QK_ITEMS; ++u) {
-        const uint32_t i = base + u * QK_THREADS + threadIdx.x;
-        tok[u] = i / row;
-        head[u] = (int)((i - tok[u] * row) / lanes);
-        const int which = head[u] >= g.t[0].heads;
-        head[u] = i < items && busy ? head[u] : -1;
-        if (head[u] >= 0) {
-          const QkTensor& t = g.t[which];
-          io[u].load(static_cast<const T*>(t.x) + qk_offset(g, t.flat, t.xs, (uint32_t)first + tok[u], head[u] - (which ? g.t[0].heads : 0)), chunk, half);
-        } else {
-#pragma unroll
-          for (int r = 0; r < PairIo<T, INTER, VEC>::R; ++r) io[u].raw[r] = make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-      if (base == 0) {
-        __syncthreads();  // the tile before has been read
-        qk_angles(g, (uint32_t)first, count, cs);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int u = 0; u < QK_ITEMS; ++u) {
-        float a[8], b[8], ss = 0.f;
-        io[u].get(a, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-        ss = group_sum(ss, lanes);
-        if (head[u] < 0) continue;
-        const float r = rsqrtf(ss * inv_d + g.eps);
-        const int which = head[u] >= g.t[0].heads;
-        const QkTensor& t = g.t[which];
-        float ga[8], gb[8], c[8], s[8];
-        qk_gains<INTER>(t.gain, chunk, half, ga, gb);
-        qk_read_cs<VEC>(cs, tok[u], half, chunk, c, s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = a[i] * r * ga[i], q = b[i] * r * gb[i];
-          a[i] = p * c[i] - q * s[i];
-          b[i] = q * c[i] + p * s[i];
-        }
-        PairIo<T, INTER, VEC>::store(static_cast<T*>(t.y) + qk_offset(g, t.flat, t.ys, (uint32_t)first + tok[u], head[u] - (which ? g.t[0].heads : 0)), chunk, half, a, b);
-      }
-    }
-  }
-}
-
-// blockIdx.y picks queries or keys, so that a lane's sums of the gain's gradient belong to one tensor; the sums of
-// all blocks are added in a fixed order by k_qk_gain_sum (no atomics: equal calls give equal gradients).
-template <typename T, bool INTER, bool VEC>
-__global__ void __launch_bounds__(QK_THREADS) k_qk_norm_rope_bwd(const __grid_constant__ QkArgs g) {
-  extern __shared__ __align__(16) float2 cs[];
-  __shared__ float warp_sum[QK_THREADS / 32][256];
-  const QkTensor& t = g.t[blockIdx.y];
-  const uint32_t total = (uint32_t)(qk_batch(g) * g.tokens);
-  const int half = g.head_dim / 2, lanes = g.lanes;
-  const int chunk = threadIdx.x & (lanes - 1);
-  const bool busy = chunk * 8 < half;
-  const uint32_t row = (uint32_t)t.heads * lanes;
+  const int tok = threadIdx.x / g.cols, col = blockIdx.y * g.cols + threadIdx.x % g.cols;
+  const int chunk = threadIdx.x & (lanes - 1);  // columns are whole groups of lanes
+  const int head_any = col / lanes, which = head_any >= g.t[0].heads;
+  const bool busy = tok < g.step && head_any < g.t[0].heads + g.t[1].heads && chunk * 8 < half;
+  const QkTensor& t = g.t[which];
+  const int head = busy ? head_any - (which ? g.t[0].heads : 0) : 0;
+  const T* x0 = static_cast<const T*>(t.x) + head * t.xs[2];
+  const T* d0 = BWD ? static_cast<const T*>(t.dy) + head * t.ds[2] : nullptr;
+  T* y0 = static_cast<T*>(t.y) + head * t.ys[2];
   const float inv_d = 1.f / (float)g.head_dim;
   float ga[8], gb[8], da[8], db[8];
   qk_gains<INTER>(t.gain, chunk, half, ga, gb);
 #pragma unroll
   for (int i = 0; i < 8; ++i) da[i] = db[i] = 0.f;
-  for (uint64_t first = (uint64_t)blockIdx.x * g.tile; first < total; first += (uint64_t)gridDim.x * g.tile) {
-    const uint32_t count = min((uint32_t)g.tile, total - (uint32_t)first);
-    const uint32_t items = count * row;
-    for (uint32_t base = 0; base < items; base += QK_THREADS * QK_ITEMS) {
-      PairIo<T, INTER, VEC> x[QK_ITEMS], dy[QK_ITEMS];
-      uint32_t tok[QK_ITEMS];
-      int head[QK_ITEMS];
+  const QkPairs pairs(half);
+  if (SHARED) {
+    qk_angles<sizeof(T) == 2>(g, pairs, 0, g.tokens, cs);
+    __syncthreads();
+  }
+  for (uint64_t first = (uint64_t)blockIdx.x * g.span; first < total; first += (uint64_t)gridDim.x * g.span) {
+    const uint32_t stop = (uint32_t)min((uint64_t)total, first + g.span);
+    Io x[U], dy[BWD ? U : 1];
+    int b[U], at[U];
+    uint32_t n = (uint32_t)first + tok;
+    b[0] = n / (uint32_t)g.tokens;
+    at[0] = n - b[0] * g.tokens;
 #pragma unroll
-      for (int u = 0; u < QK_ITEMS; ++u) {
-        const uint32_t i = base + u * QK_THREADS + threadIdx.x;
-        tok[u] = i / row;
-        head[u] = i < items && busy ? (int)((i - tok[u] * row) / lanes) : -1;
-        if (head[u] >= 0) {
-          x[u].load(static_cast<const T*>(t.x) + qk_offset(g, t.flat, t.xs, (uint32_t)first + tok[u], head[u]), chunk, half);
-          dy[u].load(static_cast<const T*>(t.dy) + qk_offset(g, t.flat, t.ds, (uint32_t)first + tok[u], head[u]), chunk, half);
-        } else {
+    for (int u = 0; u < U; ++u, n += g.step) {
+      if (u > 0) {
+        b[u] = b[u - 1] + g.step_b;
+        at[u] = at[u - 1] + g.step_t;
+        if (at[u] >= g.tokens) { at[u] -= g.tokens; ++b[u]; }
+      }
+      if (busy && n < stop) {
+        x[u].load(x0 + b[u] * t.xs[0] + at[u] * t.xs[1], chunk, half);
+        if (BWD) dy[u].load(d0 + b[u] * t.ds[0] + at[u] * t.ds[1], chunk, half);
+      } else {
+        x[u].clear();
+        if (BWD) dy[u].clear();
+      }
+    }
+    if (!SHARED) {
+      cs = angles + (odd ? g.span * half : 0);  // two buffers: a step's readers are past the barrier of the next one
+      odd ^= 1;
+      qk_angles<sizeof(T) == 2>(g, pairs, (uint32_t)first, stop - (uint32_t)first, cs);
+      __syncthreads();
+    }
+    n = (uint32_t)first + tok;
 #pragma unroll
-          for (int r = 0; r < PairIo<T, INTER, VEC>::R; ++r) x[u].raw[r] = dy[u].raw[r] = make_uint4(0u, 0u, 0u, 0u);
+    for (int u = 0; u < U; ++u, n += g.step) {
+      const bool live = busy && n < stop;
+      float a[8], bb[8], c[8], s[8], ss = 0.f;
+      x[u].get(a, bb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + bb[i] * bb[i];
+      ss = group_sum(ss, lanes);
+      const float r = rsqrtf(ss * inv_d + g.eps);
+      qk_read_cs<VEC>(cs + (live ? SHARED ? at[u] : u * g.step + tok : 0) * half, chunk, half, c, s);
+      if (!BWD) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = a[i] * r * ga[i], q = bb[i] * r * gb[i];
+          a[i] = p * c[i] - q * s[i];
+          bb[i] = q * c[i] + p * s[i];
         }
-      }
-      if (base == 0) {
-        __syncthreads();
-        qk_angles(g, (uint32_t)first, count, cs);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int u = 0; u < QK_ITEMS; ++u) {
-        float a[8], b[8], ua[8], ub[8], ss = 0.f, dot = 0.f;
-        x[u].get(a, b);
+      } else {
+        float ua[8], ub[8], dot = 0.f;
         dy[u].get(ua, ub);
-        if (head[u] >= 0) {
-          float c[8], s[8];
-          qk_read_cs<VEC>(cs, tok[u], half, chunk, c, s);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p = ua[i], q = ub[i];
-            ua[i] = p * c[i] + q * s[i];
-            ub[i] = q * c[i] - p * s[i];
-          }
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          ss += a[i] * a[i] + b[i] * b[i];
-          dot += ua[i] * ga[i] * a[i] + ub[i] * gb[i] * b[i];
+          const float p = ua[i], q = ub[i];
+          ua[i] = p * c[i] + q * s[i];
+          ub[i] = q * c[i] - p * s[i];
+          a[i] *= r;
+          bb[i] *= r;
+          da[i] += ua[i] * a[i];
+          db[i] += ub[i] * bb[i];
+          ua[i] *= ga[i];
+          ub[i] *= gb[i];
+          dot += ua[i] * a[i] + ub[i] * bb[i];
         }
-        ss = group_sum(ss, lanes);
-        dot = group_sum(dot, lanes);
-        if (head[u] < 0) continue;
-        const float r = rsqrtf(ss * inv_d + g.eps);
-        const float m = dot * r * inv_d;  // mean(w n)
+        const float m = group_sum(dot, lanes) * inv_d;  // mean(w n)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float na = a[i] * r, nb = b[i] * r;
-          da[i] += ua[i] * na;
-          db[i] += ub[i] * nb;
-          a[i] = r * (ua[i] * ga[i] - na * m);
-          b[i] = r * (ub[i] * gb[i] - nb * m);
+          a[i] = r * (ua[i] - a[i] * m);
+          bb[i] = r * (ub[i] - bb[i] * m);
         }
-        PairIo<T, INTER, VEC>::store(static_cast<T*>(t.y) + qk_offset(g, t.flat, t.ys, (uint32_t)first + tok[u], head[u]), chunk, half, a, b);
       }
+      if (live) Io::store(y0 + b[u] * t.ys[0] + at[u] * t.ys[1], chunk, half, a, bb);
     }
   }
-  // lanes with the same chunk, then the block's warps, then (next kernel) the blocks
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    for (int o = 16; o >= lanes; o >>= 1) {
-      da[i] += __shfl_xor_sync(0xffffffffu, da[i], o);
-      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
-    }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane < lanes) {
+  if (BWD) {
+    // the block's threads of one tensor and chunk in a fixed order, then (next kernel) the blocks: no atomics
+    float* part = reinterpret_cast<float*>(angles);  // [thread][16], padded
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = 8 * chunk + i;
-      if (c < half) {
-        warp_sum[warp][INTER ? 2 * c : c] = da[i];
-        warp_sum[warp][INTER ? 2 * c + 1 : half + c] = db[i];
-      }
+      part[threadIdx.x * 17 + (INTER ? 2 * i : i)] = da[i];
+      part[threadIdx.x * 17 + (INTER ? 2 * i + 1 : 8 + i)] = db[i];
     }
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < g.head_dim; d += QK_THREADS) {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < QK_THREADS / 32; ++w) s += warp_sum[w][d];
-    g.partial[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * g.head_dim + d] = s;
+    __syncthreads();
+    const int col0 = blockIdx.y * g.cols;
+    for (int e = threadIdx.x; e < 2 * g.head_dim; e += blockDim.x) {
+      const int w = e >= g.head_dim, d = e - w * g.head_dim;
+      const int pair = INTER ? d / 2 : d % half, slot = INTER ? d % 16 : (d / half) * 8 + pair % 8;
+      float sum = 0.f;
+      for (int h = w ? g.t[0].heads : 0; h < g.t[0].heads + (w ? g.t[1].heads : 0); ++h) {
+        const int c = h * lanes + pair / 8 - col0;
+        if (c < 0 || c >= g.cols) continue;
+        for (int k = 0; k < g.step; ++k) sum += part[(k * g.cols + c) * 17 + slot];
+      }
+      g.partial[((int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * 2 + w) * g.head_dim + d] = sum;
+    }
   }
 }
 
+// Block (w, c): 32 elements of the gain of queries (w = 0) or keys (1), summed over the rows of [blocks][2][head_dim].
 __global__ void __launch_bounds__(1024) k_qk_gain_sum(const float* __restrict__ partial, int blocks, int head_dim, float* dq_gain, float* dk_gain) {
-  __shared__ float part[1024];
-  const int rows = 1024 / head_dim;  // head_dim <= 256
-  const int d = threadIdx.x % head_dim, r = threadIdx.x / head_dim;
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, d = blockIdx.y * 32 + lane;
   float s = 0.f;
-  if (r < rows)
-    for (int b = r; b < blocks; b += rows) s += partial[((int64_t)blockIdx.x * blocks + b) * head_dim + d];
-  part[threadIdx.x] = s;
-  __syncthreads();
-  if (r == 0) {
-    for (int i = 1; i < rows; ++i) s += part[i * head_dim + d];
-    (blockIdx.x ? dk_gain : dq_gain)[d] = s;
+  if (d < head_dim) {
+#pragma unroll 4
+    for (int b = r; b < blocks; b += 32) s += partial[((int64_t)b * 2 + blockIdx.x) * head_dim + d];
   }
+  part[lane][r] = s;
+  __syncthreads();
+  s = part[r][lane];  // warp r: element r, its 32 partial sums
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0 && blockIdx.y * 32 + r < head_dim) (blockIdx.x ? dk_gain : dq_gain)[blockIdx.y * 32 + r] = s;
 }
 
 namespace {
@@ -376,7 +346,7 @@ int qk_prepare(const MgbsQkNormArgs* a, bool bwd, QkArgs* g, bool* vec, int* ele
     t.heads = i ? a->heads_k : a->heads_q;
     const int64_t *xs = i ? a->k_stride : a->q_stride, *ys = i ? a->k_out_stride : a->q_out_stride, *ds = i ? a->dk_out_stride : a->dq_out_stride;
     for (int j = 0; j < 3; ++j) { t.xs[j] = xs[j]; t.ys[j] = ys[j]; t.ds[j] = bwd ? ds[j] : 0; }
-    t.flat = t.xs[0] == a->tokens * t.xs[1] && t.ys[0] == a->tokens * t.ys[1] && (!bwd || t.ds[0] == a->tokens * t.ds[1]);
+    t.pad = 0;
     *vec = *vec && aligned16(t.x, t.xs, *elem) && aligned16(t.y, t.ys, *elem) && (!bwd || aligned16(t.dy, t.ds, *elem));
   }
   g->phase = a->phase;
@@ -396,29 +366,65 @@ int qk_prepare(const MgbsQkNormArgs* a, bool bwd, QkArgs* g, bool* vec, int* ele
   return 0;
 }
 
-// Tokens per block iteration: about one round of the block's items, and no more than shared memory holds.
-int qk_tile(int heads, int lanes) {
-  const int t = QK_THREADS * QK_ITEMS / (heads * lanes);
-  return t < 1 ? 1 : t;
+// How a block's threads lie over columns and tokens; returns the grid's second dimension.
+int qk_layout(QkArgs& g, int in_flight) {
+  const int row = (g.t[0].heads + g.t[1].heads) * g.lanes;
+  const int parts = (row + QK_THREADS - 1) / QK_THREADS;
+  g.cols = parts == 1 ? row : QK_THREADS;
+  g.step = QK_THREADS / g.cols;
+  g.step_b = g.step / g.tokens;
+  g.step_t = g.step % g.tokens;
+  // few tokens: one per thread, over more blocks
+  g.span = (int64_t)g.batch * g.tokens * parts > (int64_t)g.step * device_sms() * 2 ? g.step * in_flight : g.step;
+  while (g.span > g.step && 2 * g.span * (g.head_dim / 2) * (int64_t)sizeof(float2) > 32768) g.span -= g.step;  // two buffers of angles
+  return parts;
 }
 
-template <typename T, bool INTER, bool VEC> int qk_launch(QkArgs& g, bool bwd, int blocks, cudaStream_t st) {
-  const size_t smem = (size_t)g.tile * (g.head_dim / 2) * sizeof(float2);
-  if (bwd) k_qk_norm_rope_bwd<T, INTER, VEC><<<dim3(blocks, 2), QK_THREADS, smem, st>>>(g);
-  else k_qk_norm_rope<T, INTER, VEC><<<blocks, QK_THREADS, smem, st>>>(g);
+constexpr int QK_BWD_BLOCKS = 592;  // at most, also the number of partial sums of the gains' gradients
+
+// Blocks per SM of a kernel at this size; asked once per size class.
+template <typename K> int qk_resident(K kernel, int threads, size_t smem) {
+  static std::atomic<int> known[9][8];
+  std::atomic<int>& n = known[threads / 32][smem >> 13 > 7 ? 7 : smem >> 13];
+  int v = n.load(std::memory_order_relaxed);
+  if (!v) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, kernel, threads, smem) != cudaSuccess || v < 1) v = 1;
+    n.store(v, std::memory_order_relaxed);
+  }
+  return v;
+}
+
+template <typename T, bool INTER, bool VEC, int U, bool BWD, bool SHARED> int qk_start(QkArgs& g, int parts, int* blocks, cudaStream_t st) {
+  const auto kernel = k_qk_norm_rope<T, INTER, VEC, U, BWD, SHARED>;
+  const int threads = (g.cols * g.step + 31) / 32 * 32;
+  size_t smem = (size_t)(SHARED ? g.tokens : 2 * g.span) * (g.head_dim / 2) * sizeof(float2);
+  if (BWD && smem < QK_THREADS * 17 * sizeof(float)) smem = QK_THREADS * 17 * sizeof(float);
+  const int64_t turns = ((int64_t)g.batch * g.tokens + g.span - 1) / g.span;
+  int64_t most = (int64_t)device_sms() * qk_resident(kernel, threads, smem);  // one wave: every block has the same work
+  if (BWD && most > QK_BWD_BLOCKS) most = QK_BWD_BLOCKS;
+  most = most < parts ? 1 : most / parts;
+  if (BWD && parts > QK_BWD_BLOCKS) return MGBS_ERR_TOO_LARGE;
+  if (turns < most) most = turns;
+  kernel<<<dim3((unsigned)most, parts), threads, smem, st>>>(g);
+  *blocks = (int)most * parts;
   return (int)cudaGetLastError();
 }
-template <typename T> int qk_pick(QkArgs& g, bool inter, bool vec, bool bwd, int blocks, cudaStream_t st) {
-  if (inter) return vec ? qk_launch<T, true, true>(g, bwd, blocks, st) : qk_launch<T, true, false>(g, bwd, blocks, st);
-  return vec ? qk_launch<T, false, true>(g, bwd, blocks, st) : qk_launch<T, false, false>(g, bwd, blocks, st);
+template <typename T, bool INTER, bool VEC, bool BWD> int qk_launch(QkArgs& g, int* blocks, cudaStream_t st) {
+  constexpr int U = sizeof(T) == 4 ? (BWD ? 1 : 2) : (BWD ? 2 : 3);
+  const int parts = qk_layout(g, U);
+  if (VEC && g.pos_sb == 0 && g.batch > 1 && (int64_t)g.tokens * (g.head_dim / 2) * (int64_t)sizeof(float2) <= 16384)
+    return qk_start<T, INTER, VEC, U, BWD, VEC>(g, parts, blocks, st);
+  return qk_start<T, INTER, VEC, U, BWD, false>(g, parts, blocks, st);
 }
-int qk_dispatch(int dtype, QkArgs& g, bool inter, bool vec, bool bwd, int blocks, cudaStream_t st) {
-  if (dtype == MGBS_DT_BF16) return qk_pick<__nv_bfloat16>(g, inter, vec, bwd, blocks, st);
-  if (dtype == MGBS_DT_F16) return qk_pick<__half>(g, inter, vec, bwd, blocks, st);
-  return qk_pick<float>(g, inter, vec, bwd, blocks, st);
+template <typename T, bool BWD> int qk_pick(QkArgs& g, bool inter, bool vec, int* blocks, cudaStream_t st) {
+  if (inter) return vec ? qk_launch<T, true, true, BWD>(g, blocks, st) : qk_launch<T, true, false, BWD>(g, blocks, st);
+  return vec ? qk_launch<T, false, true, BWD>(g, blocks, st) : qk_launch<T, false, false, BWD>(g, blocks, st);
 }
-
-constexpr int QK_BWD_BLOCKS = 592;  // four per SM: also the number of partial sums of the gain's gradient
+template <bool BWD> int qk_dispatch(int dtype, QkArgs& g, bool inter, bool vec, int* blocks, cudaStream_t st) {
+  if (dtype == MGBS_DT_BF16) return qk_pick<__nv_bfloat16, BWD>(g, inter, vec, blocks, st);
+  if (dtype == MGBS_DT_F16) return qk_pick<__half, BWD>(g, inter, vec, blocks, st);
+  return qk_pick<float, BWD>(g, inter, vec, blocks, st);
+}
 
 }  // namespace
 
@@ -431,10 +437,8 @@ int qk_norm_rope_counted(const MgbsQkNormArgs* a, const uint32_t* count_dev, int
   if (g.batch == 0 || g.tokens == 0) return 0;
   g.count_dev = count_dev;
   g.count_offset = count_offset;
-  g.tile = qk_tile(a->heads_q + a->heads_k, g.lanes);
-  const int64_t tiles = ((int64_t)g.batch * g.tokens + g.tile - 1) / g.tile;
-  const int64_t most = (int64_t)device_sms() * 8;
-  return qk_dispatch(a->dtype, g, a->interleaved != 0, vec, false, (int)(tiles < most ? tiles : most), (cudaStream_t)stream);
+  int blocks;
+  return qk_dispatch<false>(a->dtype, g, a->interleaved != 0, vec, &blocks, (cudaStream_t)stream);
 }
 
 }  // namespace mgbs
@@ -461,13 +465,10 @@ int mgbs_qk_norm_rope_backward(const MgbsQkNormArgs* a, void* stream) {
   g.partial = a->workspace;
   int blocks = 0;
   if (g.batch > 0 && g.tokens > 0) {
-    g.tile = qk_tile(a->heads_q > a->heads_k ? a->heads_q : a->heads_k, g.lanes);
-    const int64_t tiles = ((int64_t)g.batch * g.tokens + g.tile - 1) / g.tile;
-    blocks = (int)(tiles < QK_BWD_BLOCKS ? tiles : QK_BWD_BLOCKS);
-    const int e = qk_dispatch(a->dtype, g, a->interleaved != 0, vec, true, blocks, st);
+    const int e = qk_dispatch<true>(a->dtype, g, a->interleaved != 0, vec, &blocks, st);
     if (e) return e;
   }
-  k_qk_gain_sum<<<2, 1024, 0, st>>>(a->workspace, blocks, a->head_dim, a->dq_gain, a->dk_gain);
+  k_qk_gain_sum<<<dim3(2, (a->head_dim + 31) / 32), 1024, 0, st>>>(a->workspace, blocks, a->head_dim, a->dq_gain, a->dk_gain);
   return (int)cudaGetLastError();
 }
 
