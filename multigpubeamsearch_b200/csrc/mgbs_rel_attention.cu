@@ -34,6 +34,9 @@ struct RelArgs {
 };
 
 constexpr int REL_THREADS = 128;
+#ifndef REL_FWD_BLOCKS
+#define REL_FWD_BLOCKS 4
+#endif
 constexpr float REL_BIG = 3.0e38f;
 // rows of the short form's matrices are padded by 16 bytes: eight rows then start in distinct banks
 template <int D> struct RelTile { static constexpr int PITCH = D + 8; };
@@ -70,6 +73,22 @@ template <typename T, int D> __device__ __forceinline__ void rows_product(float 
     ldsm4(b, m + kk * 32);
     mma16816<T>(s0, a[kk], b[0], b[1]);
     mma16816<T>(s1, a[kk], b[2], b[3]);
+  }
+}
+// The same from initial values c0, c1.
+template <typename T, int D>
+__device__ __forceinline__ void rows_product_from(float (&s0)[4], float (&s1)[4], const float (&c0)[4], const float (&c1)[4], const uint32_t (&a)[D / 16][4], uint32_t m) {
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    uint32_t b[4];
+    ldsm4(b, m + kk * 32);
+    if (kk == 0) {
+      mma16816_from<T>(s0, c0, a[kk], b[0], b[1]);
+      mma16816_from<T>(s1, c1, a[kk], b[2], b[3]);
+    } else {
+      mma16816<T>(s0, a[kk], b[0], b[1]);
+      mma16816<T>(s1, a[kk], b[2], b[3]);
+    }
   }
 }
 // o (16 x D) += a (16 x 16) times 16 rows of a row-major matrix
@@ -124,6 +143,7 @@ __device__ __forceinline__ float quad_sum(float v) {
 
 template <int STRIPS> __device__ __forceinline__ void group_sync(int group) {
   if (STRIPS == 1) __syncwarp();
+  else if (STRIPS == 4) __syncthreads();  // the group is the block
   else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(STRIPS * 32) : "memory");
 }
 
@@ -144,15 +164,26 @@ template <int STRIPS> struct Stream {
   }
 };
 
-// Copies the first `tokens` rows of one head into shared memory; rows from `len` on become zeros.
-template <typename T, int D, int STRIPS>
-__device__ __forceinline__ void stage_rows(uint32_t dst, const T* src, int64_t token_stride, int tokens, int len, int thread) {
-  constexpr int PITCH = RelTile<D>::PITCH, PARTS = D / 8;
-  for (int c = thread; c < tokens * PARTS; c += STRIPS * 32) {
-    const int t = c / PARTS, part = c % PARTS;
-    copy16(dst + (t * PITCH + part * 8) * 2, src + t * token_stride + part * 8, t < len ? 16u : 0u);
+// A thread's part in copying one head's rows into shared memory, sequence after sequence of a stream: 16 bytes of every
+// (STRIPS * 32 / parts)-th row.  Rows from `len` on become zeros; rows past `tokens` are not touched.
+template <typename T, int D, int STRIPS> struct RowCopy {
+  static constexpr int PITCH = RelTile<D>::PITCH, PARTS = D / 8, ROW_STEP = STRIPS * 32 / PARTS, TURNS = 16 * STRIPS / ROW_STEP;
+  const T* src;
+  int64_t next;  // elements to the stream's next sequence
+  __device__ __forceinline__ RowCopy(const void* base, const int64_t (&s)[3], int head, int first, int step, int thread) {
+    src = static_cast<const T*>(base) + first * s[0] + head * s[2] + (thread / PARTS) * s[1] + thread % PARTS * 8;
+    next = step * s[0];
   }
-}
+  static __device__ __forceinline__ uint32_t place(int thread) { return (uint32_t)((thread / PARTS * PITCH + thread % PARTS * 8) * 2); }
+  __device__ __forceinline__ void go(uint32_t dst, int64_t token_stride, int row, int tokens, int len) {
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      const int t = row + i * ROW_STEP;
+      if (t < tokens) copy16(dst + i * ROW_STEP * PITCH * 2, src + i * ROW_STEP * token_stride, t < len ? 16u : 0u);
+    }
+    src += next;
+  }
+};
 
 // Scores of a warp's 16 rows against 16 * STRIPS keys, as initial accumulators `bias` (bias / scale) + products, with
 // what the masks hide at -inf.  `steps`: blocks of 16 keys that hold any key.
@@ -163,9 +194,10 @@ __device__ __forceinline__ void short_scores(float (&s)[2 * STRIPS][4], const fl
   const int tig = threadIdx.x & 3;
 #pragma unroll
   for (int jj = 0; jj < STRIPS; ++jj) {
+    if (jj < steps) rows_product_from<T, D>(s[2 * jj], s[2 * jj + 1], bias[2 * jj], bias[2 * jj + 1], qa, k_addr + jj * 16 * PITCH * 2);
+    else
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { s[2 * jj][e] = bias[2 * jj][e]; s[2 * jj + 1][e] = bias[2 * jj + 1][e]; }
-    if (jj < steps) rows_product<T, D>(s[2 * jj], s[2 * jj + 1], qa, k_addr + jj * 16 * PITCH * 2);
+      for (int e = 0; e < 4; ++e) s[2 * jj][e] = s[2 * jj + 1][e] = -INFINITY;
   }
   if (masked) {
 #pragma unroll
@@ -191,8 +223,8 @@ template <typename T, int STRIPS> __device__ __forceinline__ void short_bias(con
     }
 }
 
-// In place: s -> 2^((s - max) sl2) (unnormalised); returns the sums of rows r and r + 8.
-template <int STRIPS> __device__ __forceinline__ void short_softmax(float (&s)[2 * STRIPS][4], float sl2, float& sum0, float& sum1) {
+// In place: s -> 2^((s - max) sl2) (unnormalised).
+template <int STRIPS> __device__ __forceinline__ void short_softmax(float (&s)[2 * STRIPS][4], float sl2) {
   float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
   for (int nb = 0; nb < 2 * STRIPS; ++nb) {
@@ -213,18 +245,13 @@ template <int STRIPS> __device__ __forceinline__ void short_softmax(float (&s)[2
       for (int e = 0; e < 2; ++e) { s[nb][e] -= m0; s[nb][2 + e] -= m1; }
     top0 = top1 = 0.f;
   }
-  sum0 = sum1 = 0.f;
 #pragma unroll
   for (int nb = 0; nb < 2 * STRIPS; ++nb)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       s[nb][e] = fast_exp2(fmaf(s[nb][e], sl2, -top0));
       s[nb][2 + e] = fast_exp2(fmaf(s[nb][2 + e], sl2, -top1));
-      sum0 += s[nb][e];
-      sum1 += s[nb][2 + e];
     }
-  sum0 = quad_sum(sum0);
-  sum1 = quad_sum(sum1);
 }
 
 template <typename T> __device__ __forceinline__ void pack_a(uint32_t (&a)[4], const float (&x)[4], const float (&y)[4]) {
@@ -237,7 +264,7 @@ template <typename T> __device__ __forceinline__ void pack_a(uint32_t (&a)[4], c
 template <typename T, int D, int STRIPS> constexpr int short_fwd_smem() { return (4 / STRIPS) * 2 * 3 * 16 * STRIPS * RelTile<D>::PITCH * 2; }
 
 template <typename T, int D, int STRIPS>
-__global__ void __launch_bounds__(REL_THREADS) k_rel_short(const __grid_constant__ RelArgs g) {
+__global__ void __launch_bounds__(REL_THREADS, REL_FWD_BLOCKS) k_rel_short(const __grid_constant__ RelArgs g) {
   constexpr int PITCH = RelTile<D>::PITCH, ROWS = 16 * STRIPS, MAT = ROWS * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
   const Stream<STRIPS> st(g);
@@ -248,12 +275,16 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_short(const __grid_constant
   const int thread = st.strip * 32 + st.lane, gid = st.lane >> 2;
   const int head_kv = st.head / (g.heads / g.heads_kv);
   const int row0 = st.strip * 16 + gid;
+  using Copy = RowCopy<T, D, STRIPS>;
+  Copy q(g.q, g.qs, st.head, st.first, st.step, thread), k(g.k, g.ks, head_kv, st.first, st.step, thread), v(g.v, g.vs, head_kv, st.first, st.step, thread);
+  const uint32_t place = base + Copy::place(thread);
+  const int copy_row = thread / Copy::PARTS;
   auto load = [&](int b, int stage) {
     const int len = rel_length(g, b);
-    const uint32_t to = base + stage * 3 * MAT * 2;
-    stage_rows<T, D, STRIPS>(to, static_cast<const T*>(g.q) + b * g.qs[0] + st.head * g.qs[2], g.qs[1], g.tokens, len, thread);
-    stage_rows<T, D, STRIPS>(to + MAT * 2, static_cast<const T*>(g.k) + b * g.ks[0] + head_kv * g.ks[2], g.ks[1], g.tokens, len, thread);
-    stage_rows<T, D, STRIPS>(to + 2 * MAT * 2, static_cast<const T*>(g.v) + b * g.vs[0] + head_kv * g.vs[2], g.vs[1], g.tokens, len, thread);
+    const uint32_t to = place + stage * 3 * MAT * 2;
+    q.go(to, g.qs[1], copy_row, g.tokens, len);
+    k.go(to + MAT * 2, g.ks[1], copy_row, g.tokens, len);
+    v.go(to + 2 * MAT * 2, g.vs[1], copy_row, g.tokens, len);
   };
   if (st.first < batch) load(st.first, 0);
   copy_commit();
@@ -264,39 +295,46 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_short(const __grid_constant
       *reinterpret_cast<uint4*>(mine + m * MAT + (g.tokens + c / (D / 8)) * PITCH + c % (D / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
   float bias[2 * STRIPS][4];
   short_bias<T, STRIPS>(g, st.head, row0, bias);
+  const int64_t row_size = (int64_t)g.heads * D;
+  T* p0 = static_cast<T*>(g.out) + ((int64_t)st.first * g.tokens + row0) * row_size + st.head * D;
+  const int64_t next = (int64_t)st.step * g.tokens * row_size;
+  const bool have0 = row0 < g.tokens, have1 = row0 + 8 < g.tokens;
+  const uint32_t ones = pack2<T>(1.f, 1.f);
   int stage = 0;
-  for (int b = st.first; b < batch; b += st.step, stage ^= 1) {
+  for (int b = st.first; b < batch; b += st.step, stage ^= 1, p0 += next) {
     copy_wait<0>();
     group_sync<STRIPS>(st.group);  // this stage has arrived, and every warp has left the other one
     if (b + st.step < batch) load(b + st.step, stage ^ 1);
     copy_commit();
     const int len = rel_length(g, b);
-    T* out = static_cast<T*>(g.out) + ((int64_t)b * g.tokens * g.heads + st.head) * D;
-    T* p0 = row0 < g.tokens ? out + (int64_t)row0 * g.heads * D : nullptr;
-    T* p1 = row0 + 8 < g.tokens ? out + (int64_t)(row0 + 8) * g.heads * D : nullptr;
-    if (st.strip * 16 >= len) store_zero_rows<T, D>(p0, p1);
-    else {
-      const uint32_t at = base + stage * 3 * MAT * 2;
-      uint32_t qa[D / 16][4];
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) ldsm4(qa[kk], at + (st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
-      const int steps = (len + 15) >> 4;
-      float s[2 * STRIPS][4], sum0, sum1;
-      short_scores<T, D, STRIPS>(s, bias, qa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, steps, g.causal || len < g.tokens, len, g.causal, row0);
-      short_softmax<STRIPS>(s, g.sl2, sum0, sum1);
-      float o[D / 8][4];
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-      for (int jj = 0; jj < STRIPS; ++jj)
-        if (jj < steps) {
-          uint32_t pa[4];
-          pack_a<T>(pa, s[2 * jj], s[2 * jj + 1]);
-          cols_product<T, D>(o, pa, at + (2 * MAT + jj * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
-        }
-      const bool in0 = row0 < len, in1 = row0 + 8 < len;
-      store_rows<T, D>(o, in0 && sum0 != 0.f ? 1.f / sum0 : 0.f, in1 && sum1 != 0.f ? 1.f / sum1 : 0.f, p0, p1);
+    T* to0 = have0 ? p0 : nullptr;
+    T* to1 = have1 ? p0 + 8 * row_size : nullptr;
+    if (st.strip * 16 >= len) {
+      store_zero_rows<T, D>(to0, to1);
+      continue;
     }
+    const uint32_t at = base + stage * 3 * MAT * 2;
+    uint32_t qa[D / 16][4];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) ldsm4(qa[kk], at + (st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
+    const int steps = (len + 15) >> 4;
+    float s[2 * STRIPS][4];
+    short_scores<T, D, STRIPS>(s, bias, qa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, steps, g.causal || len < g.tokens, len, g.causal, row0);
+    short_softmax<STRIPS>(s, g.sl2);
+    // The row sums come out of the product too, as one more column of ones: float32 sums of the same rounded terms that
+    // multiply v, so that a row's weights still sum to one.
+    float o[D / 8][4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+    for (int jj = 0; jj < STRIPS; ++jj)
+      if (jj < steps) {
+        uint32_t pa[4];
+        pack_a<T>(pa, s[2 * jj], s[2 * jj + 1]);
+        mma16816<T>(sum, pa, ones, ones);
+        cols_product<T, D>(o, pa, at + (2 * MAT + jj * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
+      }
+    store_rows<T, D>(o, row0 < len && sum[0] != 0.f ? 1.f / sum[0] : 0.f, row0 + 8 < len && sum[2] != 0.f ? 1.f / sum[2] : 0.f, to0, to1);
   }
 }
 
@@ -318,13 +356,18 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_short_bwd(const __grid_cons
   const uint32_t base = smem_addr(mine), ps_at = smem_addr(ps), dss_at = smem_addr(dss);
   const int thread = st.strip * 32 + st.lane, gid = st.lane >> 2, tig = st.lane & 3;
   const int row0 = st.strip * 16 + gid;
+  using Copy = RowCopy<T, D, STRIPS>;
+  Copy q(g.q, g.qs, st.head, st.first, st.step, thread), k(g.k, g.ks, st.head, st.first, st.step, thread);
+  Copy v(g.v, g.vs, st.head, st.first, st.step, thread), dout(g.dout, g.ds, st.head, st.first, st.step, thread);
+  const uint32_t place = base + Copy::place(thread);
+  const int copy_row = thread / Copy::PARTS;
   auto load = [&](int b, int stage) {
     const int len = rel_length(g, b);
-    const uint32_t to = base + stage * 4 * MAT * 2;
-    stage_rows<T, D, STRIPS>(to, static_cast<const T*>(g.q) + b * g.qs[0] + st.head * g.qs[2], g.qs[1], g.tokens, len, thread);
-    stage_rows<T, D, STRIPS>(to + MAT * 2, static_cast<const T*>(g.k) + b * g.ks[0] + st.head * g.ks[2], g.ks[1], g.tokens, len, thread);
-    stage_rows<T, D, STRIPS>(to + 2 * MAT * 2, static_cast<const T*>(g.v) + b * g.vs[0] + st.head * g.vs[2], g.vs[1], g.tokens, len, thread);
-    stage_rows<T, D, STRIPS>(to + 3 * MAT * 2, static_cast<const T*>(g.dout) + b * g.ds[0] + st.head * g.ds[2], g.ds[1], g.tokens, len, thread);
+    const uint32_t to = place + stage * 4 * MAT * 2;
+    q.go(to, g.qs[1], copy_row, g.tokens, len);
+    k.go(to + MAT * 2, g.ks[1], copy_row, g.tokens, len);
+    v.go(to + 2 * MAT * 2, g.vs[1], copy_row, g.tokens, len);
+    dout.go(to + 3 * MAT * 2, g.ds[1], copy_row, g.tokens, len);
   };
   if (st.first < g.batch) load(st.first, 0);
   copy_commit();
@@ -354,9 +397,13 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_short_bwd(const __grid_cons
       uint32_t fa[D / 16][4];
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) ldsm4(fa[kk], at + (st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
-      float s[2 * STRIPS][4], dp[2 * STRIPS][4], sum0, sum1;
+      float s[2 * STRIPS][4], dp[2 * STRIPS][4], sum0 = 0.f, sum1 = 0.f;
       short_scores<T, D, STRIPS>(s, bias, fa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, steps, g.causal || len < g.tokens, len, g.causal, row0);
-      short_softmax<STRIPS>(s, g.sl2, sum0, sum1);
+      short_softmax<STRIPS>(s, g.sl2);
+#pragma unroll
+      for (int n = 0; n < 2 * STRIPS; ++n) { sum0 += s[n][0] + s[n][1]; sum1 += s[n][2] + s[n][3]; }
+      sum0 = quad_sum(sum0);
+      sum1 = quad_sum(sum1);
       const float inv0 = sum0 != 0.f ? 1.f / sum0 : 0.f, inv1 = sum1 != 0.f ? 1.f / sum1 : 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) ldsm4(fa[kk], at + (3 * MAT + st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);

@@ -91,26 +91,39 @@ def _load():
     return _ready
 
 
+def _current_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same handle without a Stream object around it, where torch has the call: two microseconds of a small call's ten
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
+
+
 def _enqueue(fn, args, device: torch.device, what: str) -> None:
     """Run a C entry on the tensors' device and that device's current stream."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(C.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(C.byref(args), _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(C.byref(args), torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(C.byref(args), _raw_stream(index))
     if rc:
         _lib.check(rc, what)
 
 
-def _need(ok: bool, what: str, why: str) -> None:
-    if not ok:
-        raise RuntimeError(f"{what}: {why}")
+def _refuse(what: str, why: str):
+    raise RuntimeError(f"{what}: {why}")
 
 
-def _same_device(what: str, device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
+def _same_device(what: str, device: torch.device, *tensors) -> None:
+    for t in tensors:
         if t is not None and t.device != device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, the first tensor on {device}")
+            _refuse(what, f"tensors on {device} and {t.device}")
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised memory like t, contiguous."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -120,14 +133,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
     """Batch, token and head strides; a dimension of one entry has none."""
-    s, n = t.stride(), t.shape
-    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+    s0, s1, s2, _ = t.stride()
+    n0, n1, n2, _ = t.shape
+    return (s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """The tensor with 16-byte rows on 16-byte boundaries (a copy only where it has none)."""
+    """A 16-bit tensor with rows on 16-byte boundaries (a copy only where they are not)."""
     t = _rows(t)
-    if t.data_ptr() % 16 == 0 and not any(s * t.element_size() % 16 for s in _strides(t)):
+    s0, s1, s2 = _strides(t)
+    if not (t.data_ptr() % 16 or (s0 | s1 | s2) % 8):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -174,7 +189,7 @@ def _qk_args(q, k, q_gain, k_gain, rotary, positions, eps, interleaved) -> MgbsQ
 
 def _qk_forward(q, k, q_gain, k_gain, rotary, positions, eps, interleaved):
     a = _qk_args(q, k, q_gain, k_gain, rotary, positions, eps, interleaved)
-    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out, k_out = _dense(q), _dense(k)
     a.q_out_stride[:], a.k_out_stride[:] = _strides(q_out), _strides(k_out)
     a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
     _enqueue(_load().mgbs_qk_norm_rope, a, q.device, "qk_norm_rope")
@@ -195,15 +210,14 @@ class _QkNormRope(torch.autograd.Function):
         lib = _load()
         a = _qk_args(q, k, q_gain, k_gain, ctx.rotary, positions, ctx.eps, ctx.interleaved)
         dq_out, dk_out = _rows(dq_out), _rows(dk_out)
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dgains = torch.empty((2, q.shape[3]), dtype=torch.float32, device=q.device)
-        work = torch.empty((lib.mgbs_qk_norm_rope_backward_workspace(q.shape[3]) // 4,), dtype=torch.float32, device=q.device)
+        dq, dk, dq_gain, dk_gain = _dense(q), _dense(k), _dense(q_gain), _dense(k_gain)
+        work = q_gain.new_empty(lib.mgbs_qk_norm_rope_backward_workspace(q.shape[3]) // 4)
         a.q_out_stride[:], a.k_out_stride[:] = _strides(dq), _strides(dk)
         a.dq_out_stride[:], a.dk_out_stride[:] = _strides(dq_out), _strides(dk_out)
         a.q_out, a.k_out, a.dq_out, a.dk_out = dq.data_ptr(), dk.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr()
-        a.dq_gain, a.dk_gain, a.workspace = dgains.data_ptr(), dgains[1].data_ptr(), work.data_ptr()
+        a.dq_gain, a.dk_gain, a.workspace = dq_gain.data_ptr(), dk_gain.data_ptr(), work.data_ptr()
         _enqueue(lib.mgbs_qk_norm_rope_backward, a, q.device, "qk_norm_rope backward")
-        return dq, dk, dgains[0], dgains[1], None, None, None, None
+        return dq, dk, dq_gain, dk_gain, None, None, None, None
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: torch.Tensor, k_gain: torch.Tensor, rotary: RotaryFrequencies,
@@ -216,20 +230,28 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: torch.Tensor, k_gain:
     float32 [head_dim].  ``positions``: int32 or int64 [tokens] or [batch, tokens], negative ones included; by default a
     token's index.  Pairs are (i, i + head_dim / 2), or (2 i, 2 i + 1) with ``interleaved``.  Statistics and rotation are
     in float32, rounded once.  Differentiable in q, k and the gains."""
-    what = "qk_norm_rope"
-    _need(q.is_cuda and q.dim() == 4 and k.dim() == 4, what, "q and k must be [batch, tokens, heads, head_dim] CUDA tensors")
-    _need(q.dtype in DTYPES and k.dtype == q.dtype, what, "q and k must have one type: bfloat16, float16 or float32")
-    _need(q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3], what, "q and k must agree in batch, tokens and head_dim")
-    d = q.shape[3]
-    _need(2 <= d <= 256 and d % 2 == 0 and q.shape[2] >= 1 and k.shape[2] >= 1, what, "head_dim must be even, 2 to 256, with one head at least")
-    _need(d == rotary.head_dim, what, f"the frequencies are for head_dim {rotary.head_dim}")
-    for g in (q_gain, k_gain):
-        _need(g.dtype == torch.float32 and g.shape == (d,), what, "gains must be float32 [head_dim]")
-    _need(eps >= 0.0 and math.isfinite(eps), what, "eps must not be negative")
+    what, dtype, device = "qk_norm_rope", q.dtype, q.device
+    if not q.is_cuda or q.dim() != 4 or k.dim() != 4:
+        _refuse(what, "q and k must be [batch, tokens, heads, head_dim] CUDA tensors")
+    if dtype not in DTYPES or k.dtype != dtype:
+        _refuse(what, "q and k must have one type: bfloat16, float16 or float32")
+    (b, t, h, d), (kb, kt, kh, kd) = q.shape, k.shape
+    if (kb, kt, kd) != (b, t, d):
+        _refuse(what, "q and k must agree in batch, tokens and head_dim")
+    if not 2 <= d <= 256 or d % 2 or h < 1 or kh < 1:
+        _refuse(what, "head_dim must be even, 2 to 256, with one head at least")
+    if d != rotary.head_dim:
+        _refuse(what, f"the frequencies are for head_dim {rotary.head_dim}")
+    if q_gain.dtype != torch.float32 or k_gain.dtype != torch.float32 or q_gain.shape != (d,) or k_gain.shape != (d,):
+        _refuse(what, "gains must be float32 [head_dim]")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        _refuse(what, "eps must not be negative")
     if positions is not None:
-        _need(positions.dtype in (torch.int32, torch.int64), what, "positions must be int32 or int64")
-        _need(positions.shape in (q.shape[1:2], q.shape[:2]), what, "positions must be [tokens] or [batch, tokens]")
-    _same_device(what, q.device, k=k, q_gain=q_gain, k_gain=k_gain, positions=positions, rotary=rotary.phase)
+        if positions.dtype is not torch.int64 and positions.dtype is not torch.int32:
+            _refuse(what, "positions must be int32 or int64")
+        if positions.shape != (t,) and positions.shape != (b, t):
+            _refuse(what, "positions must be [tokens] or [batch, tokens]")
+    _same_device(what, device, k, q_gain, k_gain, positions, rotary.phase)
     q, k, q_gain, k_gain = _rows(q), _rows(k), q_gain.contiguous(), k_gain.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gain.requires_grad or k_gain.requires_grad):
         return _QkNormRope.apply(q, k, q_gain, k_gain, rotary, positions, float(eps), bool(interleaved))
@@ -302,7 +324,7 @@ def _rel_args(q, k, v, table, buckets, lengths, scale) -> MgbsRelAttentionArgs:
 
 def _rel_forward(q, k, v, table, buckets, lengths, scale, with_stats):
     a = _rel_args(q, k, v, table, buckets, lengths, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _dense(q)
     a.out = out.data_ptr()
     stats = None
     if with_stats:
@@ -328,8 +350,7 @@ class _RelativeAttention(torch.autograd.Function):
         lib = _load()
         a = _rel_args(q, k, v, table, ctx.buckets, lengths, ctx.scale)
         dout = _aligned(dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dtable = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+        dq, dk, dv, dtable = _dense(q), _dense(k), _dense(v), _dense(table)
         work = torch.empty((max(16, lib.mgbs_rel_attention_backward_workspace(C.byref(a))),), dtype=torch.uint8, device=q.device)
         a.dout_stride[:] = _strides(dout)
         a.out, a.dout = out.data_ptr(), dout.data_ptr()
@@ -349,22 +370,30 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     is made only where rows do not lie on 16-byte boundaries).  ``lengths`` (int32 [batch]): tokens of a sequence from
     its length on are padding: never read, their outputs and gradients are 0.  ``scale``: head_dim ** -0.5 by default.
     A row whose biases leave no key (all -inf) gives 0.  Differentiable in q, k, v and table."""
-    what = "relative_attention"
-    _need(q.is_cuda and q.dim() == 4 and k.dim() == 4 and v.dim() == 4, what, "q, k and v must be [batch, tokens, heads, head_dim] CUDA tensors")
-    _need(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype and table.dtype == q.dtype, what,
-          "q, k, v and table must have one type: bfloat16 or float16")
-    _need(k.shape == v.shape and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3], what, "q, k and v must agree in batch, tokens and head_dim")
-    _need(q.shape[3] in (32, 64), what, "head_dim must be 32 or 64")
-    _need(k.shape[2] >= 1 and q.shape[2] >= 1 and q.shape[2] % k.shape[2] == 0 and q.shape[2] <= 1024, what,
-          "query heads (at most 1024) must be a multiple of the key heads")
-    _need(q.shape[1] <= 1 << 20, what, "at most 2^20 tokens")
-    _need(table.shape == (buckets.num_buckets, q.shape[2]), what, "table must be [num_buckets, heads]")
+    what, dtype, device = "relative_attention", q.dtype, q.device
+    if not q.is_cuda or q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        _refuse(what, "q, k and v must be [batch, tokens, heads, head_dim] CUDA tensors")
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype != dtype or v.dtype != dtype or table.dtype != dtype:
+        _refuse(what, "q, k, v and table must have one type: bfloat16 or float16")
+    (b, t, h, d), (kb, kt, kh, kd) = q.shape, k.shape
+    if (kb, kt, kd) != (b, t, d) or v.shape != k.shape:
+        _refuse(what, "q, k and v must agree in batch, tokens and head_dim")
+    if d != 32 and d != 64:
+        _refuse(what, "head_dim must be 32 or 64")
+    if kh < 1 or not 1 <= h <= 1024 or h % kh:
+        _refuse(what, "query heads (at most 1024) must be a multiple of the key heads")
+    if t > 1 << 20:
+        _refuse(what, "at most 2^20 tokens")
+    if table.shape != (buckets.num_buckets, h):
+        _refuse(what, "table must be [num_buckets, heads]")
     if lengths is not None:
-        _need(lengths.shape == q.shape[:1] and lengths.dtype == torch.int32, what, "lengths must be int32 [batch]")
+        if lengths.shape != (b,) or lengths.dtype != torch.int32:
+            _refuse(what, "lengths must be int32 [batch]")
         lengths = lengths.contiguous()
-    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    _need(1e-30 <= scale <= 1e30, what, "scale must be positive and finite")
-    _same_device(what, q.device, k=k, v=v, table=table, buckets=buckets.map, lengths=lengths)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        _refuse(what, "scale must be positive and finite")
+    _same_device(what, device, k, v, table, buckets.map, lengths)
     q, k, v, table = _aligned(q), _aligned(k), _aligned(v), table.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
         return _RelativeAttention.apply(q, k, v, table, buckets, lengths, scale)
@@ -377,21 +406,32 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
 
 
 def _distill_check(what, logits, teacher, index, temperature):
-    _need(logits.is_cuda and logits.dim() == 2 and logits.dtype in DTYPES, what, "logits must be a [rows, width] CUDA tensor: bfloat16, float16 or float32")
-    _need(logits.shape[1] >= 1, what, "logits must have one column at least")
-    _need(teacher.dim() == 2 and teacher.shape == index.shape and teacher.shape[0] == logits.shape[0], what, "teacher and index must be [rows, entries]")
-    _need(1 <= teacher.shape[1] <= MAX_ENTRIES, what, f"1 to {MAX_ENTRIES} entries per row")
-    _need(teacher.dtype in DTYPES, what, "teacher must be bfloat16, float16 or float32")
-    _need(index.dtype in (torch.int32, torch.int64), what, "index must be int32 or int64")
-    _need(1e-30 <= temperature <= 1e30, what, "temperature must be positive and finite")
-    _same_device(what, logits.device, teacher=teacher, index=index)
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in DTYPES or logits.shape[1] < 1:
+        _refuse(what, "logits must be a [rows, width] CUDA tensor with one column at least: bfloat16, float16 or float32")
+    if teacher.dim() != 2 or teacher.shape != index.shape or teacher.shape[0] != logits.shape[0]:
+        _refuse(what, "teacher and index must be [rows, entries]")
+    if not 1 <= teacher.shape[1] <= MAX_ENTRIES:
+        _refuse(what, f"1 to {MAX_ENTRIES} entries per row")
+    if teacher.dtype not in DTYPES:
+        _refuse(what, "teacher must be bfloat16, float16 or float32")
+    if index.dtype is not torch.int64 and index.dtype is not torch.int32:
+        _refuse(what, "index must be int32 or int64")
+    if not 1e-30 <= temperature <= 1e30:
+        _refuse(what, "temperature must be positive and finite")
+    _same_device(what, logits.device, teacher, index)
+
+
+def _float(teacher: torch.Tensor) -> torch.Tensor:
+    teacher = teacher.detach()
+    return teacher if teacher.dtype is torch.float32 else teacher.float()
 
 
 def _distill_run(what, logits, teacher, index, temperature, weight, with_grad):
     a = MgbsDistillArgs()
-    loss = torch.empty((logits.shape[0],), dtype=torch.float32, device=logits.device)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if with_grad else None
-    a.dtype, a.entries, a.rows, a.width = DTYPES[logits.dtype], teacher.shape[1], logits.shape[0], logits.shape[1]
+    (rows, width), entries = logits.shape, teacher.shape[1]
+    loss = teacher.new_empty(rows)
+    grad = _dense(logits) if with_grad else None
+    a.dtype, a.entries, a.rows, a.width = DTYPES[logits.dtype], entries, rows, width
     a.index_bits, a.temperature = index.element_size() * 8, temperature
     a.row_stride, a.teacher_stride, a.index_stride = logits.stride(0), teacher.stride(0), index.stride(0)
     a.logits, a.teacher, a.index, a.loss = logits.data_ptr(), teacher.data_ptr(), index.data_ptr(), loss.data_ptr()
@@ -430,7 +470,7 @@ def distill_top_logits(logits: torch.Tensor, teacher_logits: torch.Tensor, teach
     distill_top_logits_step."""
     temperature = float(temperature)
     _distill_check("distill_top_logits", logits, teacher_logits, teacher_index, temperature)
-    logits, teacher, index = _rows(logits), _rows(teacher_logits.detach().float()), _rows(teacher_index)
+    logits, teacher, index = _rows(logits), _rows(_float(teacher_logits)), _rows(teacher_index)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillTopLogits.apply(logits, teacher, index, temperature)
     return _distill_run("distill_top_logits", logits, teacher, index, temperature, None, False)[0]
@@ -444,8 +484,8 @@ def distill_top_logits_step(logits: torch.Tensor, teacher_logits: torch.Tensor, 
     temperature = float(temperature)
     _distill_check(what, logits, teacher_logits, teacher_index, temperature)
     if row_weight is not None:
-        _need(row_weight.dtype == torch.float32 and row_weight.shape == logits.shape[:1], what, "row_weight must be float32 [rows]")
-        _same_device(what, logits.device, row_weight=row_weight)
+        if row_weight.dtype != torch.float32 or row_weight.shape != logits.shape[:1]:
+            _refuse(what, "row_weight must be float32 [rows]")
+        _same_device(what, logits.device, row_weight)
         row_weight = row_weight.detach().contiguous()
-    with torch.no_grad():
-        return _distill_run(what, _rows(logits.detach()), _rows(teacher_logits.detach().float()), _rows(teacher_index), temperature, row_weight, True)
+    return _distill_run(what, _rows(logits.detach()), _rows(_float(teacher_logits)), _rows(teacher_index), temperature, row_weight, True)
