@@ -37,6 +37,9 @@ constexpr int REL_THREADS = 128;
 #ifndef REL_FWD_BLOCKS
 #define REL_FWD_BLOCKS 4
 #endif
+#ifndef REL_BWD_BLOCKS
+#define REL_BWD_BLOCKS 3
+#endif
 constexpr float REL_BIG = 3.0e38f;
 // rows of the short form's matrices are padded by 16 bytes: eight rows then start in distinct banks
 template <int D> struct RelTile { static constexpr int PITCH = D + 8; };
@@ -128,6 +131,26 @@ template <typename T, int D> __device__ __forceinline__ void store_zero_rows(T* 
   }
 }
 
+// A warp's 16 x D accumulators, rows times f0 / f1, to `rows` rows of global memory (pitch row_size) through a strip of
+// shared memory of its own (16 rows of PITCH), so that every lane stores 16 bytes.
+template <typename T, int D> __device__ __forceinline__ void store_strip(const float (&o)[D / 8][4], float f0, float f1, T* strip, T* out, int64_t row_size, int rows) {
+  constexpr int PITCH = RelTile<D>::PITCH, PARTS = D / 8;
+  const int lane = threadIdx.x & 31;
+  __syncwarp();  // what the strip held has been read
+  const uint32_t at = smem_addr(strip) + frag_a<PITCH>(lane) * 2;
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n)
+    stsm4(at + n * 32, pack2<T>(o[2 * n][0] * f0, o[2 * n][1] * f0), pack2<T>(o[2 * n][2] * f1, o[2 * n][3] * f1),
+          pack2<T>(o[2 * n + 1][0] * f0, o[2 * n + 1][1] * f0), pack2<T>(o[2 * n + 1][2] * f1, o[2 * n + 1][3] * f1));
+  __syncwarp();
+  const int row = lane / PARTS, part = lane % PARTS * 8;
+#pragma unroll
+  for (int i = 0; i < PARTS / 2; ++i) {
+    const int r = row + i * (32 / PARTS);
+    if (r < rows) *reinterpret_cast<uint4*>(out + r * row_size + part) = *reinterpret_cast<const uint4*>(strip + r * PITCH + part);
+  }
+}
+
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -141,9 +164,12 @@ __device__ __forceinline__ float quad_sum(float v) {
 // Up to 64 tokens
 // ------------------------------------------------------------------------------------------------------------------
 
+// Groups of a block: four warps are cut into groups of one, two or four; a group of three is a block of three.
+template <int STRIPS> struct Groups { static constexpr int N = STRIPS == 1 ? 4 : STRIPS == 2 ? 2 : 1, THREADS = N * STRIPS * 32; };
+
 template <int STRIPS> __device__ __forceinline__ void group_sync(int group) {
   if (STRIPS == 1) __syncwarp();
-  else if (STRIPS == 4) __syncthreads();  // the group is the block
+  else if (STRIPS > 2) __syncthreads();  // the group is the block
   else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(STRIPS * 32) : "memory");
 }
 
@@ -156,8 +182,8 @@ template <int STRIPS> struct Stream {
     lane = threadIdx.x & 31;
     group = warp / STRIPS;
     strip = warp % STRIPS;
-    id = blockIdx.x * (4 / STRIPS) + group;
-    step = gridDim.x * (4 / STRIPS) / g.heads;
+    id = blockIdx.x * Groups<STRIPS>::N + group;
+    step = gridDim.x * Groups<STRIPS>::N / g.heads;
     live = id < step * g.heads;
     head = id % g.heads;
     first = id / g.heads;
@@ -186,18 +212,15 @@ template <typename T, int D, int STRIPS> struct RowCopy {
 };
 
 // Scores of a warp's 16 rows against 16 * STRIPS keys, as initial accumulators `bias` (bias / scale) + products, with
-// what the masks hide at -inf.  `steps`: blocks of 16 keys that hold any key.
+// what the masks hide at -inf.  All blocks of keys, also the empty ones: branches would keep the products from overlapping.
 template <typename T, int D, int STRIPS>
 __device__ __forceinline__ void short_scores(float (&s)[2 * STRIPS][4], const float (&bias)[2 * STRIPS][4], const uint32_t (&qa)[D / 16][4],
-                                             uint32_t k_addr, int steps, bool masked, int len, int causal, int row0) {
+                                             uint32_t k_addr, bool masked, int len, int causal, int row0) {
   constexpr int PITCH = RelTile<D>::PITCH;
   const int tig = threadIdx.x & 3;
 #pragma unroll
   for (int jj = 0; jj < STRIPS; ++jj) {
-    if (jj < steps) rows_product_from<T, D>(s[2 * jj], s[2 * jj + 1], bias[2 * jj], bias[2 * jj + 1], qa, k_addr + jj * 16 * PITCH * 2);
-    else
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[2 * jj][e] = s[2 * jj + 1][e] = -INFINITY;
+    rows_product_from<T, D>(s[2 * jj], s[2 * jj + 1], bias[2 * jj], bias[2 * jj + 1], qa, k_addr + jj * 16 * PITCH * 2);
   }
   if (masked) {
 #pragma unroll
@@ -205,7 +228,7 @@ __device__ __forceinline__ void short_scores(float (&s)[2 * STRIPS][4], const fl
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = nb * 8 + 2 * tig + (e & 1), i = row0 + (e >> 1) * 8;
-        if (j >= len || (causal && j > i)) s[nb][e] = -INFINITY;
+        if (j >= len || i >= len || (causal && j > i)) s[nb][e] = -INFINITY;
       }
   }
 }
@@ -261,10 +284,10 @@ template <typename T> __device__ __forceinline__ void pack_a(uint32_t (&a)[4], c
   a[3] = pack2<T>(y[2], y[3]);
 }
 
-template <typename T, int D, int STRIPS> constexpr int short_fwd_smem() { return (4 / STRIPS) * 2 * 3 * 16 * STRIPS * RelTile<D>::PITCH * 2; }
+template <typename T, int D, int STRIPS> constexpr int short_fwd_smem() { return Groups<STRIPS>::N * 2 * 3 * 16 * STRIPS * RelTile<D>::PITCH * 2; }
 
 template <typename T, int D, int STRIPS>
-__global__ void __launch_bounds__(REL_THREADS, REL_FWD_BLOCKS) k_rel_short(const __grid_constant__ RelArgs g) {
+__global__ void __launch_bounds__(Groups<STRIPS>::THREADS, REL_FWD_BLOCKS) k_rel_short(const __grid_constant__ RelArgs g) {
   constexpr int PITCH = RelTile<D>::PITCH, ROWS = 16 * STRIPS, MAT = ROWS * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
   const Stream<STRIPS> st(g);
@@ -296,30 +319,22 @@ __global__ void __launch_bounds__(REL_THREADS, REL_FWD_BLOCKS) k_rel_short(const
   float bias[2 * STRIPS][4];
   short_bias<T, STRIPS>(g, st.head, row0, bias);
   const int64_t row_size = (int64_t)g.heads * D;
-  T* p0 = static_cast<T*>(g.out) + ((int64_t)st.first * g.tokens + row0) * row_size + st.head * D;
+  T* out = static_cast<T*>(g.out) + ((int64_t)st.first * g.tokens + st.strip * 16) * row_size + st.head * D;
   const int64_t next = (int64_t)st.step * g.tokens * row_size;
-  const bool have0 = row0 < g.tokens, have1 = row0 + 8 < g.tokens;
   const uint32_t ones = pack2<T>(1.f, 1.f);
   int stage = 0;
-  for (int b = st.first; b < batch; b += st.step, stage ^= 1, p0 += next) {
+  for (int b = st.first; b < batch; b += st.step, stage ^= 1, out += next) {
     copy_wait<0>();
     group_sync<STRIPS>(st.group);  // this stage has arrived, and every warp has left the other one
     if (b + st.step < batch) load(b + st.step, stage ^ 1);
     copy_commit();
     const int len = rel_length(g, b);
-    T* to0 = have0 ? p0 : nullptr;
-    T* to1 = have1 ? p0 + 8 * row_size : nullptr;
-    if (st.strip * 16 >= len) {
-      store_zero_rows<T, D>(to0, to1);
-      continue;
-    }
     const uint32_t at = base + stage * 3 * MAT * 2;
     uint32_t qa[D / 16][4];
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) ldsm4(qa[kk], at + (st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
-    const int steps = (len + 15) >> 4;
     float s[2 * STRIPS][4];
-    short_scores<T, D, STRIPS>(s, bias, qa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, steps, g.causal || len < g.tokens, len, g.causal, row0);
+    short_scores<T, D, STRIPS>(s, bias, qa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, g.causal || len < g.tokens, len, g.causal, row0);
     short_softmax<STRIPS>(s, g.sl2);
     // The row sums come out of the product too, as one more column of ones: float32 sums of the same rounded terms that
     // multiply v, so that a row's weights still sum to one.
@@ -327,24 +342,25 @@ __global__ void __launch_bounds__(REL_THREADS, REL_FWD_BLOCKS) k_rel_short(const
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-    for (int jj = 0; jj < STRIPS; ++jj)
-      if (jj < steps) {
-        uint32_t pa[4];
-        pack_a<T>(pa, s[2 * jj], s[2 * jj + 1]);
-        mma16816<T>(sum, pa, ones, ones);
-        cols_product<T, D>(o, pa, at + (2 * MAT + jj * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
-      }
-    store_rows<T, D>(o, row0 < len && sum[0] != 0.f ? 1.f / sum[0] : 0.f, row0 + 8 < len && sum[2] != 0.f ? 1.f / sum[2] : 0.f, to0, to1);
+    for (int jj = 0; jj < STRIPS; ++jj) {
+      uint32_t pa[4];
+      pack_a<T>(pa, s[2 * jj], s[2 * jj + 1]);
+      mma16816<T>(sum, pa, ones, ones);
+      cols_product<T, D>(o, pa, at + (2 * MAT + jj * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
+    }
+    // rows from the length on have no term: their sums are 0, and so are they
+    store_strip<T, D>(o, sum[0] != 0.f ? 1.f / sum[0] : 0.f, sum[2] != 0.f ? 1.f / sum[2] : 0.f,
+                      mine + stage * 3 * MAT + st.strip * 16 * PITCH, out, row_size, g.tokens - st.strip * 16);
   }
 }
 
 template <typename T, int D, int STRIPS> __host__ __device__ constexpr int short_bwd_group() {  // bytes of one group
-  return (2 * 4 * 16 * STRIPS * RelTile<D>::PITCH + 2 * 16 * STRIPS * (16 * STRIPS + 8)) * 2;
+  return ((2 * 4 + 1) * 16 * STRIPS * RelTile<D>::PITCH + 2 * 16 * STRIPS * (16 * STRIPS + 8)) * 2;
 }
 
 // Softmax and delta are computed anew from q, k, v, dout: neither the output nor statistics are read.
 template <typename T, int D, int STRIPS>
-__global__ void __launch_bounds__(REL_THREADS) k_rel_short_bwd(const __grid_constant__ RelArgs g) {
+__global__ void __launch_bounds__(Groups<STRIPS>::THREADS, REL_BWD_BLOCKS) k_rel_short_bwd(const __grid_constant__ RelArgs g) {
   constexpr int PITCH = RelTile<D>::PITCH, ROWS = 16 * STRIPS, MAT = ROWS * PITCH, PP = ROWS + 8;
   extern __shared__ __align__(16) uint8_t rel_smem[];
   const Stream<STRIPS> st(g);
@@ -353,6 +369,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_short_bwd(const __grid_cons
   T* mine = reinterpret_cast<T*>(raw);
   T* ps = mine + 8 * MAT;      // P, then dS: [query][key]
   T* dss = ps + ROWS * PP;
+  T* out_strip = dss + ROWS * PP + st.strip * 16 * PITCH;  // of this warp alone
   const uint32_t base = smem_addr(mine), ps_at = smem_addr(ps), dss_at = smem_addr(dss);
   const int thread = st.strip * 32 + st.lane, gid = st.lane >> 2, tig = st.lane & 3;
   const int row0 = st.strip * 16 + gid;
@@ -379,108 +396,89 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_short_bwd(const __grid_cons
   short_bias<T, STRIPS>(g, st.head, row0, bias);
 #pragma unroll
   for (int nb = 0; nb < 2 * STRIPS; ++nb) dbias[nb][0] = dbias[nb][1] = dbias[nb][2] = dbias[nb][3] = 0.f;
+  const int64_t row_size = (int64_t)g.heads * D;
+  int64_t out_at = ((int64_t)st.first * g.tokens + st.strip * 16) * row_size + st.head * D;
+  const int64_t next = (int64_t)st.step * g.tokens * row_size;
+  const int rows = g.tokens - st.strip * 16;
+  const uint32_t strip_p = ps_at + (st.strip * 16 * PP + frag_a<PP>(st.lane)) * 2, strip_ds = dss_at + (st.strip * 16 * PP + frag_a<PP>(st.lane)) * 2;
+  const uint32_t turned = (uint32_t)(((st.lane & 7) + (st.lane >> 4) * 8) * PP + st.strip * 16 + ((st.lane >> 3) & 1) * 8) * 2;
   int stage = 0;
-  for (int b = st.first; b < g.batch; b += st.step, stage ^= 1) {
+  for (int b = st.first; b < g.batch; b += st.step, stage ^= 1, out_at += next) {
     copy_wait<0>();
     group_sync<STRIPS>(st.group);
     if (b + st.step < g.batch) load(b + st.step, stage ^ 1);
     copy_commit();
-    const int len = rel_length(g, b), steps = (len + 15) >> 4;
+    const int len = rel_length(g, b);
     const uint32_t at = base + stage * 4 * MAT * 2;
-    const int64_t row_at = ((int64_t)b * g.tokens * g.heads + st.head) * D;
-    const int64_t off0 = row_at + (int64_t)row0 * g.heads * D, off1 = off0 + (int64_t)8 * g.heads * D;
-    const bool have0 = row0 < g.tokens, have1 = row0 + 8 < g.tokens;
-    T* dq = static_cast<T*>(g.dq);
-    T* dk = static_cast<T*>(g.dk);
-    T* dv = static_cast<T*>(g.dv);
-    if (st.strip < steps) {
-      uint32_t fa[D / 16][4];
+    uint32_t fa[D / 16][4];
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) ldsm4(fa[kk], at + (st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
-      float s[2 * STRIPS][4], dp[2 * STRIPS][4], sum0 = 0.f, sum1 = 0.f;
-      short_scores<T, D, STRIPS>(s, bias, fa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, steps, g.causal || len < g.tokens, len, g.causal, row0);
-      short_softmax<STRIPS>(s, g.sl2);
+    for (int kk = 0; kk < D / 16; ++kk) ldsm4(fa[kk], at + (st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
+    float s[2 * STRIPS][4], dp[2 * STRIPS][4], sum0 = 0.f, sum1 = 0.f;
+    short_scores<T, D, STRIPS>(s, bias, fa, at + (MAT + frag_b<PITCH>(st.lane)) * 2, g.causal || len < g.tokens, len, g.causal, row0);
+    short_softmax<STRIPS>(s, g.sl2);
 #pragma unroll
-      for (int n = 0; n < 2 * STRIPS; ++n) { sum0 += s[n][0] + s[n][1]; sum1 += s[n][2] + s[n][3]; }
-      sum0 = quad_sum(sum0);
-      sum1 = quad_sum(sum1);
-      const float inv0 = sum0 != 0.f ? 1.f / sum0 : 0.f, inv1 = sum1 != 0.f ? 1.f / sum1 : 0.f;
+    for (int n = 0; n < 2 * STRIPS; ++n) { sum0 += s[n][0] + s[n][1]; sum1 += s[n][2] + s[n][3]; }
+    sum0 = quad_sum(sum0);
+    sum1 = quad_sum(sum1);
+    const float inv0 = sum0 != 0.f ? 1.f / sum0 : 0.f, inv1 = sum1 != 0.f ? 1.f / sum1 : 0.f;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) ldsm4(fa[kk], at + (3 * MAT + st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
-      float d0 = 0.f, d1 = 0.f;
+    for (int kk = 0; kk < D / 16; ++kk) ldsm4(fa[kk], at + (3 * MAT + st.strip * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2 + kk * 32);
+    float d0 = 0.f, d1 = 0.f;
 #pragma unroll
-      for (int jj = 0; jj < STRIPS; ++jj) {
+    for (int jj = 0; jj < STRIPS; ++jj) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dp[2 * jj][e] = dp[2 * jj + 1][e] = 0.f;
-        if (jj < steps) rows_product<T, D>(dp[2 * jj], dp[2 * jj + 1], fa, at + (2 * MAT + jj * 16 * PITCH + frag_b<PITCH>(st.lane)) * 2);
+      for (int e = 0; e < 4; ++e) dp[2 * jj][e] = dp[2 * jj + 1][e] = 0.f;
+      rows_product<T, D>(dp[2 * jj], dp[2 * jj + 1], fa, at + (2 * MAT + jj * 16 * PITCH + frag_b<PITCH>(st.lane)) * 2);
 #pragma unroll
-        for (int n = 2 * jj; n < 2 * jj + 2; ++n) {
-          s[n][0] *= inv0; s[n][1] *= inv0; s[n][2] *= inv1; s[n][3] *= inv1;
-          d0 += s[n][0] * dp[n][0] + s[n][1] * dp[n][1];
-          d1 += s[n][2] * dp[n][2] + s[n][3] * dp[n][3];
-        }
+      for (int n = 2 * jj; n < 2 * jj + 2; ++n) {
+        s[n][0] *= inv0; s[n][1] *= inv0; s[n][2] *= inv1; s[n][3] *= inv1;
+        d0 += s[n][0] * dp[n][0] + s[n][1] * dp[n][1];
+        d1 += s[n][2] * dp[n][2] + s[n][3] * dp[n][3];
       }
-      d0 = quad_sum(d0);
-      d1 = quad_sum(d1);
-      float o[D / 8][4];
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-      for (int jj = 0; jj < STRIPS; ++jj)
-        if (jj < steps) {
-#pragma unroll
-          for (int n = 2 * jj; n < 2 * jj + 2; ++n) {
-            T* to = ps + row0 * PP + n * 8 + 2 * tig;
-            *reinterpret_cast<uint32_t*>(to) = pack2<T>(s[n][0], s[n][1]);
-            *reinterpret_cast<uint32_t*>(to + 8 * PP) = pack2<T>(s[n][2], s[n][3]);
-            s[n][0] *= dp[n][0] - d0; s[n][1] *= dp[n][1] - d0;
-            s[n][2] *= dp[n][2] - d1; s[n][3] *= dp[n][3] - d1;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dbias[n][e] += s[n][e];
-          }
-          uint32_t da[4];
-          pack_a<T>(da, s[2 * jj], s[2 * jj + 1]);
-          T* to = dss + row0 * PP + jj * 16 + 2 * tig;
-          *reinterpret_cast<uint32_t*>(to) = da[0];
-          *reinterpret_cast<uint32_t*>(to + 8 * PP) = da[1];
-          *reinterpret_cast<uint32_t*>(to + 8) = da[2];
-          *reinterpret_cast<uint32_t*>(to + 8 * PP + 8) = da[3];
-          cols_product<T, D>(o, da, at + (MAT + jj * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
-        }
-      store_rows<T, D>(o, row0 < len ? g.scale : 0.f, row0 + 8 < len ? g.scale : 0.f, have0 ? dq + off0 : nullptr, have1 ? dq + off1 : nullptr);
-    } else {
-      store_zero_rows<T, D>(have0 ? dq + off0 : nullptr, have1 ? dq + off1 : nullptr);
     }
+    d0 = quad_sum(d0);
+    d1 = quad_sum(d1);
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+    for (int jj = 0; jj < STRIPS; ++jj) {
+      uint32_t a[4];
+      pack_a<T>(a, s[2 * jj], s[2 * jj + 1]);
+      stsm4(strip_p + jj * 32, a[0], a[1], a[2], a[3]);
+#pragma unroll
+      for (int n = 2 * jj; n < 2 * jj + 2; ++n) {
+        s[n][0] *= dp[n][0] - d0; s[n][1] *= dp[n][1] - d0;
+        s[n][2] *= dp[n][2] - d1; s[n][3] *= dp[n][3] - d1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dbias[n][e] += s[n][e];
+      }
+      pack_a<T>(a, s[2 * jj], s[2 * jj + 1]);
+      stsm4(strip_ds + jj * 32, a[0], a[1], a[2], a[3]);
+      cols_product<T, D>(o, a, at + (MAT + jj * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
+    }
+    // rows from the length on have P = dS = 0, as queries and as keys
+    store_strip<T, D>(o, g.scale, g.scale, out_strip, static_cast<T*>(g.dq) + out_at, row_size, rows);
     group_sync<STRIPS>(st.group);  // P and dS of all query strips are there
-    if (st.strip < steps) {
-      // this warp's 16 keys: dv = P^T dout, dk = dS^T q, over the query strips
-      const int turned = ((st.lane & 7) + (st.lane >> 4) * 8) * PP + st.strip * 16 + ((st.lane >> 3) & 1) * 8;
-      float o[D / 8][4];
+    // this warp's 16 keys: dv = P^T dout, dk = dS^T q, over the query strips
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-      for (int ii = 0; ii < STRIPS; ++ii)
-        if (ii < steps) {
-          uint32_t a[4];
-          ldsm4_t(a, ps_at + (ii * 16 * PP + turned) * 2);
-          cols_product<T, D>(o, a, at + (3 * MAT + ii * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
-        }
-      const float in0 = row0 < len ? 1.f : 0.f, in1 = row0 + 8 < len ? 1.f : 0.f;
-      store_rows<T, D>(o, in0, in1, have0 ? dv + off0 : nullptr, have1 ? dv + off1 : nullptr);
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-      for (int ii = 0; ii < STRIPS; ++ii)
-        if (ii < steps) {
-          uint32_t a[4];
-          ldsm4_t(a, dss_at + (ii * 16 * PP + turned) * 2);
-          cols_product<T, D>(o, a, at + (ii * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
-        }
-      store_rows<T, D>(o, in0 * g.scale, in1 * g.scale, have0 ? dk + off0 : nullptr, have1 ? dk + off1 : nullptr);
-    } else {
-      store_zero_rows<T, D>(have0 ? dv + off0 : nullptr, have1 ? dv + off1 : nullptr);
-      store_zero_rows<T, D>(have0 ? dk + off0 : nullptr, have1 ? dk + off1 : nullptr);
+    for (int ii = 0; ii < STRIPS; ++ii) {
+      uint32_t a[4];
+      ldsm4_t(a, ps_at + ii * 16 * PP * 2 + turned);
+      cols_product<T, D>(o, a, at + (3 * MAT + ii * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
     }
+    store_strip<T, D>(o, 1.f, 1.f, out_strip, static_cast<T*>(g.dv) + out_at, row_size, rows);
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+    for (int ii = 0; ii < STRIPS; ++ii) {
+      uint32_t a[4];
+      ldsm4_t(a, dss_at + ii * 16 * PP * 2 + turned);
+      cols_product<T, D>(o, a, at + (ii * 16 * PITCH + frag_a<PITCH>(st.lane)) * 2);
+    }
+    store_strip<T, D>(o, g.scale, g.scale, out_strip, static_cast<T*>(g.dk) + out_at, row_size, rows);
   }
   // dS summed over this stream's sequences -> diagonals -> buckets
   copy_wait<0>();
@@ -993,12 +991,11 @@ namespace {
 constexpr int REL_SHORT = 64;
 constexpr int REL_CHUNKS = 32;
 
-int short_strips(int tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4; }
+int short_strips(int tokens) { return (tokens + 15) / 16; }
 
 // Blocks of the short kernels: as many as the device holds at a time (`per_sm`), at least one stream per head, and
 // no more than sequences x heads need.
-int short_blocks(int64_t batch, int heads, int strips, int per_sm) {
-  const int groups = 4 / strips;
+int short_blocks(int64_t batch, int heads, int groups, int per_sm) {
   int64_t streams = (int64_t)device_sms() * per_sm * groups;
   if (streams < heads) streams = heads;
   if (streams > batch * heads) streams = batch * heads;
@@ -1007,9 +1004,9 @@ int short_blocks(int64_t batch, int heads, int strips, int per_sm) {
 
 bool short_backward(const MgbsRelAttentionArgs* a) { return a->tokens <= REL_SHORT && a->heads == a->heads_kv; }
 
-template <typename K> int resident(K kernel, int smem) {
+template <typename K> int resident(K kernel, int threads, int smem) {
   int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, REL_THREADS, smem) != cudaSuccess || n < 1) n = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
   return n;
 }
 
@@ -1020,8 +1017,8 @@ template <typename T, int D, int STRIPS> int run_short(const RelArgs& g, cudaStr
   const int rc = raise_smem(k_rel_short<T, D, STRIPS>, smem, raised);
   if (rc) return rc;
   int n = per_sm.load(std::memory_order_relaxed);
-  if (!n) per_sm.store(n = resident(k_rel_short<T, D, STRIPS>, smem), std::memory_order_relaxed);
-  k_rel_short<T, D, STRIPS><<<short_blocks(g.batch, g.heads, STRIPS, n), REL_THREADS, smem, st>>>(g);
+  if (!n) per_sm.store(n = resident(k_rel_short<T, D, STRIPS>, Groups<STRIPS>::THREADS, smem), std::memory_order_relaxed);
+  k_rel_short<T, D, STRIPS><<<short_blocks(g.batch, g.heads, Groups<STRIPS>::N, n), Groups<STRIPS>::THREADS, smem, st>>>(g);
   return (int)cudaGetLastError();
 }
 
@@ -1033,19 +1030,19 @@ template <typename T> int finish_table(const RelArgs& g, const float* in, int64_
 // Streams of the short backward: bounded independently of the device, because the workspace holds a row for each.
 constexpr int REL_BWD_STREAMS = 4096;
 template <typename T, int D, int STRIPS> int run_short_bwd(const RelArgs& g, void* dtable, cudaStream_t st) {
-  constexpr int smem = (4 / STRIPS) * short_bwd_group<T, D, STRIPS>();
+  constexpr int smem = Groups<STRIPS>::N * short_bwd_group<T, D, STRIPS>();
   static std::atomic<uint64_t> raised{0};
   static std::atomic<int> per_sm{0};
   const int rc = raise_smem(k_rel_short_bwd<T, D, STRIPS>, smem, raised);
   if (rc) return rc;
   int n = per_sm.load(std::memory_order_relaxed);
-  if (!n) per_sm.store(n = resident(k_rel_short_bwd<T, D, STRIPS>, smem), std::memory_order_relaxed);
-  int blocks = short_blocks(g.batch, g.heads, STRIPS, n);
-  const int most = REL_BWD_STREAMS / (4 / STRIPS);
+  if (!n) per_sm.store(n = resident(k_rel_short_bwd<T, D, STRIPS>, Groups<STRIPS>::THREADS, smem), std::memory_order_relaxed);
+  int blocks = short_blocks(g.batch, g.heads, Groups<STRIPS>::N, n);
+  const int most = REL_BWD_STREAMS / Groups<STRIPS>::N;
   if (blocks > most) blocks = most;
-  const int step = blocks * (4 / STRIPS) / g.heads;
+  const int step = blocks * Groups<STRIPS>::N / g.heads;
   if (step < 1) return MGBS_ERR_TOO_LARGE;
-  k_rel_short_bwd<T, D, STRIPS><<<blocks, REL_THREADS, smem, st>>>(g);
+  k_rel_short_bwd<T, D, STRIPS><<<blocks, Groups<STRIPS>::THREADS, smem, st>>>(g);
   const int e = (int)cudaGetLastError();
   return e ? e : finish_table<T>(g, g.partial, step, 1, g.heads, dtable, st);
 }
@@ -1088,12 +1085,13 @@ template <typename T, int D> int forward_as(const RelArgs& g, cudaStream_t st) {
   // with statistics asked for, the form whose backward reads them
   if (g.tokens > REL_SHORT || (g.stats && g.heads != g.heads_kv)) return run_tiles<T, D>(g, st);
   const int strips = short_strips(g.tokens);
-  return strips == 1 ? run_short<T, D, 1>(g, st) : strips == 2 ? run_short<T, D, 2>(g, st) : run_short<T, D, 4>(g, st);
+  return strips == 1 ? run_short<T, D, 1>(g, st) : strips == 2 ? run_short<T, D, 2>(g, st) : strips == 3 ? run_short<T, D, 3>(g, st) : run_short<T, D, 4>(g, st);
 }
 template <typename T, int D> int backward_as(const RelArgs& g, bool is_short, void* dtable, float* sums, cudaStream_t st) {
   if (!is_short) return run_tiles_bwd<T, D>(g, dtable, sums, st);
   const int strips = short_strips(g.tokens);
-  return strips == 1 ? run_short_bwd<T, D, 1>(g, dtable, st) : strips == 2 ? run_short_bwd<T, D, 2>(g, dtable, st) : run_short_bwd<T, D, 4>(g, dtable, st);
+  return strips == 1 ? run_short_bwd<T, D, 1>(g, dtable, st) : strips == 2 ? run_short_bwd<T, D, 2>(g, dtable, st)
+         : strips == 3 ? run_short_bwd<T, D, 3>(g, dtable, st) : run_short_bwd<T, D, 4>(g, dtable, st);
 }
 
 bool fits16(const void* p, const int64_t (&s)[3]) {
