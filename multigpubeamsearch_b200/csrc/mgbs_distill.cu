@@ -10,14 +10,11 @@
 // maximum and sum and the pass that writes the gradient, so that z is read once.  Rows that not even a cluster holds
 // (over 512 KB) are read twice.  Sums are in float32 and in a fixed order; no atomics.
 
-#include <cooperative_groups.h>
 #include <math.h>
 
 #include "mgbs_operators.cuh"
 
 namespace mgbs {
-
-namespace cg = cooperative_groups;
 
 struct DistillArgs {
   const void* logits;
@@ -36,6 +33,23 @@ __device__ __forceinline__ int distill_index(const DistillArgs& g, int64_t row, 
   const int64_t i = g.index64 ? static_cast<const int64_t*>(g.index)[at] : (int64_t) static_cast<const int32_t*>(g.index)[at];
   return i >= 0 && i < g.width ? (int)i : -1;
 }
+
+// 2^(x c) relative to the row's maximum m.  Where |m c| is out of all proportion (rows at the type's lowest value, where
+// x c would overflow) differences come first, so that equal logits still get equal weights.
+struct Scale {
+  float c, m, k;
+  bool huge;
+  __device__ __forceinline__ Scale(float m_, float c_) : c(c_), m(m_) {
+    k = rintf(m_ * c_);
+    huge = !(fabsf(k) <= 0x1p20f);
+  }
+  __device__ __forceinline__ float arg(float x) const { return huge ? (x - m) * c : fmaf(x, c, -k); }
+  // what a sum taken relative to maximum `other` is multiplied with
+  __device__ __forceinline__ float from(float other) const {
+    const Scale o(other, c);
+    return fast_exp2(huge || o.huge ? (other - m) * c : o.k - k);
+  }
+};
 
 constexpr int DISTILL_THREADS = 256;
 
@@ -64,11 +78,11 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
     tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
     any |= __shfl_xor_sync(0xffffffffu, any, o);
   }
-  // differences first: entries at the type's lowest value stay finite, and equal ones stay equal
+  const Scale sc(m, g.c);
   float s = 0.f, ts = 0.f;
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
-    v[i] = lane + i * lanes < g.width ? fast_exp2((v[i] - m) * g.c) : 0.f;
+    v[i] = lane + i * lanes < g.width ? fast_exp2(sc.arg(v[i])) : 0.f;
     s += v[i];
   }
   for (int k = lane; k < g.entries; k += lanes)
@@ -85,7 +99,7 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
       if (i < 0) continue;
       const float t = (g.teacher[row * g.teacher_stride + k] - tm) * g.c;
       const float p = fast_exp2(t) * inv_ts;
-      if (p != 0.f) loss += p * (t - (Elem<T>::up(z[i]) - m) * g.c + log_ratio);
+      if (p != 0.f) loss += p * (t - sc.arg(Elem<T>::up(z[i])) + log_ratio);
     }
   for (int o = lanes >> 1; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
   if (live && lane == 0) g.loss[row] = loss * kLn2;
@@ -113,103 +127,130 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
             first = first && n >= k;
             p += fast_exp2((g.teacher[row * g.teacher_stride + n] - tm) * g.c);
           }
-        if (first) out[i] = Elem<T>::down(fast_exp2((Elem<T>::up(z[i]) - m) * g.c) * scale - p * inv_ts * w);
+        if (first) out[i] = Elem<T>::down(fast_exp2(sc.arg(Elem<T>::up(z[i]))) * scale - p * inv_ts * w);
       }
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 
-constexpr int DISTILL_WIDE = 512;  // threads of a block
+constexpr int DISTILL_WIDE = 512;  // threads of a block at most
+#ifndef DW_T
+#define DW_T 256
+#endif
 
-struct MaxSum { float m, s; };  // maximum and sum of 2^((x - m) c)
+// Maximum m of some logits and the sum of 2^(x c - k), k = m c rounded to a whole number: sums of different m differ by
+// exact powers of two, and a term costs one fused step without an error of its own in k.
+struct MaxSum { float m, s; };
 
 __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
   const float m = fmaxf(a.m, b.m);
-  const float base = m == -INFINITY ? 0.f : m;  // nothing yet on either side: both sums are 0
-  return {m, a.s * fast_exp2((a.m - base) * c) + b.s * fast_exp2((b.m - base) * c)};
+  const Scale to(m == -INFINITY ? 0.f : m, c);  // nothing yet on either side: both sums are 0
+  return {m, a.s * to.from(a.m) + b.s * to.from(b.m)};
 }
 
-// One row per cluster of gridDim-given size; piece p of the row holds 16 bytes.  A row that does not start on a
-// 16-byte boundary is read from the boundary before it, its first and last piece element by element.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void put_remote(float2* local, int rank, float2 v) {  // the same address in block `rank`
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
+}
+
+// 16 bytes of -inf: what a thread holds where the row has ended
+template <typename T> __device__ __forceinline__ uint4 nothing16();
+template <> __device__ __forceinline__ uint4 nothing16<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+template <> __device__ __forceinline__ uint4 nothing16<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+template <> __device__ __forceinline__ uint4 nothing16<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
+// One row per cluster, in pieces of 16 bytes on 16-byte boundaries; the elements before the first and after the last
+// boundary belong to single threads of the first and the last block.  The unrolled loops hold the ordinary case alone
+// (out-of-proportion maxima and outputs on other boundaries go through rolled ones): instruction fetch counts here.  Blocks send one another their maximum and sum
+// and meet once; everything about the teacher's entries is fetched while the row is on its way.
 template <typename T, int NV, bool GRAD>
-__global__ void __launch_bounds__(DISTILL_WIDE) k_distill_wide(const __grid_constant__ DistillArgs g, int pieces_per_block) {
+__global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_constant__ DistillArgs g, int ranks, int pieces_per_block) {
   constexpr int E = Vec16<T>::N;
   __shared__ MaxSum warp_part[DISTILL_WIDE / 32];
-  __shared__ MaxSum block_part;
-  __shared__ float s_t[MGBS_DISTILL_MAX_ENTRIES];
-  __shared__ int s_i[MGBS_DISTILL_MAX_ENTRIES];
+  __shared__ float2 parts[8];                       // maximum and sum of every block of the cluster
+  __shared__ float s_t[MGBS_DISTILL_MAX_ENTRIES];   // teacher logits
+  __shared__ float s_z[MGBS_DISTILL_MAX_ENTRIES];   // the student's at the same columns
+  __shared__ __align__(16) int s_i[MGBS_DISTILL_MAX_ENTRIES];
   __shared__ float s_tm, s_ts;
   __shared__ int s_any;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
   const int64_t row = blockIdx.x / ranks;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
+  if (ranks > 1) cluster_arrive();  // "this block runs": waited for before anything is sent to it
   const T* z = static_cast<const T*>(g.logits) + row * g.row_stride;
-  const int skew = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-  for (int k = tid; k < g.entries; k += DISTILL_WIDE) {
-    s_i[k] = distill_index(g, row, k);
-    s_t[k] = g.teacher[row * g.teacher_stride + k];
-  }
-  const int pieces = (g.width + skew + E - 1) / E;
-  const int p0 = rank * pieces_per_block, p1 = min(pieces, p0 + pieces_per_block);
+  const int head = (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T));  // elements before the first boundary
+  const int pieces = (g.width - head) / E, tail = g.width - head - pieces * E;
+  const uint4* body = reinterpret_cast<const uint4*>(z + head);
+  const int p0 = min(pieces, rank * pieces_per_block), p1 = min(pieces, p0 + pieces_per_block);
+  const bool last = rank == ranks - 1;
+  const int edge = rank == 0 && tid < head ? tid : last && tid >= 32 && tid < 32 + tail ? g.width - tail + tid - 32 : -1;
+  const float edge_z = edge >= 0 ? Elem<T>::up(z[edge]) : -INFINITY;
   uint4 raw[NV];
   auto fetch = [&](int base) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int p = base + i * DISTILL_WIDE + tid;
-      const int e = p * E - skew;
-      raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (p < p1) {
-        if (e >= 0 && e + E <= g.width) raw[i] = __ldg(reinterpret_cast<const uint4*>(z + e));
-        else {
-          T* part = reinterpret_cast<T*>(&raw[i]);
-#pragma unroll
-          for (int j = 0; j < E; ++j) part[j] = e + j >= 0 && e + j < g.width ? z[e + j] : Elem<T>::down(-INFINITY);
-        }
-      }
+      const int p = base + i * threads + tid;
+      raw[i] = p < p1 ? __ldg(body + p) : nothing16<T>();
     }
   };
+  fetch(p0);
+  const int entries4 = (g.entries + 3) / 4;
+  for (int k = tid; k < 4 * entries4; k += threads) {
+    const int i = k < g.entries ? distill_index(g, row, k) : -1;
+    s_i[k] = i;
+    s_t[k] = k < g.entries ? g.teacher[row * g.teacher_stride + k] : -INFINITY;
+    s_z[k] = i >= 0 ? Elem<T>::up(z[i]) : 0.f;
+  }
   MaxSum mine{-INFINITY, 0.f};
-  for (int base = p0; base < p1; base += NV * DISTILL_WIDE) {
-    fetch(base);
-    float top = mine.m;
+  for (int base = p0; base == p0 || base < p1; base += NV * threads) {
+    if (base != p0) fetch(base);
+    float top = base == p0 ? edge_z : mine.m;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (base + i * DISTILL_WIDE + tid < p1) {
-        float v[E];
-        Vec16<T>::up(raw[i], v);
+    for (int i = 0; i < NV; ++i) top = fmaxf(top, Vec16<T>::top(raw[i]));
 #pragma unroll
-        for (int j = 0; j < E; ++j) top = fmaxf(top, v[j]);
-      }
-    const float seen = top == -INFINITY ? 0.f : top;
-    mine.s *= fast_exp2((mine.m - seen) * g.c);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const Scale sc(top == -INFINITY ? 0.f : top, g.c);  // one for the warp
+    mine.s = base == p0 ? fast_exp2(sc.arg(edge_z)) : mine.s * sc.from(mine.m);
     mine.m = top;
+    if (!sc.huge) {
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (base + i * DISTILL_WIDE + tid < p1) {
+      for (int i = 0; i < NV; ++i) {
         float v[E];
         Vec16<T>::up(raw[i], v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) mine.s += fast_exp2((v[j] - seen) * g.c);
+        for (int j = 0; j < E; ++j) part[j & 3] += fast_exp2(fmaf(v[j], g.c, -sc.k));
       }
+      mine.s += (part[0] + part[1]) + (part[2] + part[3]);
+    } else {
+#pragma unroll 1
+      for (int p = base + tid; p < min(p1, base + NV * threads); p += threads) {
+        float v[E];
+        Vec16<T>::up(__ldg(body + p), v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) mine.s += fast_exp2(sc.arg(v[j]));
+      }
+    }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const MaxSum other{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o)};
-    mine = merge(mine, other, g.c);
-  }
-  const int warp = tid >> 5, lane = tid & 31;
+  for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
   if (lane == 0) warp_part[warp] = mine;
   __syncthreads();
+  if (ranks > 1) cluster_wait();
   if (warp == 0) {
-    mine = lane < DISTILL_WIDE / 32 ? warp_part[lane] : MaxSum{-INFINITY, 0.f};
+    mine = lane < threads / 32 ? warp_part[lane] : MaxSum{-INFINITY, 0.f};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = DISTILL_WIDE / 64; o > 0; o >>= 1) {
       const MaxSum other{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o)};
       mine = merge(mine, other, g.c);
     }
-    if (lane == 0) block_part = mine;
+    const MaxSum whole{__shfl_sync(0xffffffffu, mine.m, 0), __shfl_sync(0xffffffffu, mine.s, 0)};
+    if (ranks == 1) { if (lane == 0) parts[0] = make_float2(whole.m, whole.s); }
+    else if (lane < ranks) put_remote(&parts[rank], lane, make_float2(whole.m, whole.s));
   } else if (warp == 1) {  // the teacher's softmax
     float tm = -INFINITY, ts = 0.f;
     int any = 0;
@@ -226,14 +267,12 @@ __global__ void __launch_bounds__(DISTILL_WIDE) k_distill_wide(const __grid_cons
     for (int o = 16; o > 0; o >>= 1) ts += __shfl_xor_sync(0xffffffffu, ts, o);
     if (lane == 0) { s_tm = tm; s_ts = ts; s_any = any; }
   }
-  if (ranks > 1) cluster.sync();
+  if (ranks > 1) { cluster_arrive(); cluster_wait(); }
   else __syncthreads();
-  MaxSum all = block_part;
-  if (ranks > 1) {
-    all = *cluster.map_shared_rank(&block_part, 0);
-    for (int r = 1; r < ranks; ++r) all = merge(all, *cluster.map_shared_rank(&block_part, r), g.c);
-  }
-  const float m = all.m, tm = s_tm, inv_ts = 1.f / s_ts;
+  MaxSum all{parts[0].x, parts[0].y};
+  for (int r = 1; r < ranks; ++r) all = merge(all, MaxSum{parts[r].x, parts[r].y}, g.c);
+  const Scale sc(all.m, g.c);
+  const float tm = s_tm, inv_ts = 1.f / s_ts;
   const bool any = s_any != 0;
   if (rank == 0 && warp == 0) {
     const float log_ratio = log2f(all.s) - log2f(s_ts);
@@ -242,7 +281,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE) k_distill_wide(const __grid_cons
       for (int k = lane; k < g.entries; k += 32) {
         if (s_i[k] < 0) continue;
         const float t = (s_t[k] - tm) * g.c, p = fast_exp2(t) * inv_ts;
-        if (p != 0.f) loss += p * (t - (Elem<T>::up(z[s_i[k]]) - m) * g.c + log_ratio);
+        if (p != 0.f) loss += p * (t - sc.arg(s_z[k]) + log_ratio);
       }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
@@ -253,43 +292,54 @@ __global__ void __launch_bounds__(DISTILL_WIDE) k_distill_wide(const __grid_cons
     const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
     const float w = (g.weight ? g.weight[row] : 1.f) * g.inv_t;
     const float scale = any ? w / all.s : 0.f;
-    for (int base = p0; base < p1; base += NV * DISTILL_WIDE) {
-      if (p1 - p0 > NV * DISTILL_WIDE) fetch(base);  // the row does not stay in registers
+    if (edge >= 0) out[edge] = Elem<T>::down(any ? fast_exp2(sc.arg(edge_z)) * scale : 0.f);
+    T* out_body = out + head;
+    if (same && any && !sc.huge) {
+      for (int base = p0; base < p1; base += NV * threads) {
+        if (p1 - p0 > NV * threads) fetch(base);  // the row does not stay in registers
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int p = base + i * DISTILL_WIDE + tid;
-        if (p >= p1) continue;
-        const int e = p * E - skew;
-        float v[E];
-        Vec16<T>::up(raw[i], v);
+        for (int i = 0; i < NV; ++i) {
+          const int p = base + i * threads + tid;
+          float v[E];
+          Vec16<T>::up(raw[i], v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = any ? fast_exp2((v[j] - m) * g.c) * scale : 0.f;
-        if (same && e >= 0 && e + E <= g.width) *reinterpret_cast<uint4*>(out + e) = Vec16<T>::down(v);
-        else {
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (e + j >= 0 && e + j < g.width) out[e + j] = Elem<T>::down(v[j]);
+          for (int j = 0; j < E; ++j) v[j] = fast_exp2(fmaf(v[j], g.c, -sc.k)) * scale;
+          if (p < p1) reinterpret_cast<uint4*>(out_body)[p] = Vec16<T>::down(v);
         }
+      }
+    } else {
+#pragma unroll 1
+      for (int p = p0 + tid; p < p1; p += threads) {
+        float v[E];
+        Vec16<T>::up(__ldg(body + p), v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) out_body[p * E + j] = Elem<T>::down(any ? fast_exp2(sc.arg(v[j])) * scale : 0.f);
       }
     }
     __syncthreads();
+    // the entries' columns once more, from float32: the first of equal indices writes, for all of them
     if (any)
-      for (int k = tid; k < g.entries; k += DISTILL_WIDE) {
+      for (int k = tid; k < g.entries; k += threads) {
         const int i = s_i[k];
         if (i < 0) continue;
-        const int piece = (i + skew) / E;
-        if (piece < p0 || piece >= p1) continue;  // another block's column
+        const int piece = i < head ? -1 : (i - head) / E;  // -1 and `pieces`: the edges
+        if (piece < 0 ? rank != 0 : piece >= pieces ? !last : piece < p0 || piece >= p1) continue;  // another block's column
         float p = 0.f;
         bool first = true;
-        for (int n = 0; n < g.entries; ++n)
-          if (s_i[n] == i) {
-            first = first && n >= k;
-            p += fast_exp2((s_t[n] - tm) * g.c);
-          }
-        if (first) out[i] = Elem<T>::down(fast_exp2((Elem<T>::up(z[i]) - m) * g.c) * scale - p * inv_ts * w);
+        for (int n = 0; n < entries4; ++n) {
+          const int4 four = reinterpret_cast<const int4*>(s_i)[n];
+          if (four.x != i && four.y != i && four.z != i && four.w != i) continue;
+          const int f[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (f[j] == i) {
+              first = first && 4 * n + j >= k;
+              p += fast_exp2((s_t[4 * n + j] - tm) * g.c);
+            }
+        }
+        if (first) out[i] = Elem<T>::down(fast_exp2(sc.arg(s_z[k])) * scale - p * inv_ts * w);
       }
   }
-  if (ranks > 1) cluster.sync();  // a block's sums stay until all have read them
 }
 
 namespace {
@@ -305,10 +355,10 @@ template <typename T, bool GRAD> int distill_rows(const DistillArgs& g, cudaStre
   return (int)cudaGetLastError();
 }
 
-template <typename T, int NV, bool GRAD> int distill_wide_as(const DistillArgs& g, int ranks, int per_block, cudaStream_t st) {
+template <typename T, int NV, bool GRAD> int distill_wide_as(const DistillArgs& g, int ranks, int per_block, int threads, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(g.rows * ranks));
-  cfg.blockDim = dim3(DISTILL_WIDE);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -316,21 +366,23 @@ template <typename T, int NV, bool GRAD> int distill_wide_as(const DistillArgs& 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, k_distill_wide<T, NV, GRAD>, g, per_block);
+  return (int)cudaLaunchKernelEx(&cfg, k_distill_wide<T, NV, GRAD>, g, ranks, per_block);
 }
 
 template <typename T, bool GRAD> int distill_wide(const DistillArgs& g, int sms, cudaStream_t st) {
-  const int64_t pieces = ((int64_t)g.width + 2 * Vec16<T>::N - 2) / Vec16<T>::N;  // whatever the row's first byte
-  // the fewest blocks that hold the row in eight pieces per thread; more of them while that leaves SMs without work
-  int ranks = 1;
-  while (ranks < 8 && pieces > (int64_t)ranks * 8 * DISTILL_WIDE) ranks *= 2;
-  while (ranks < 8 && g.rows * ranks < sms && pieces > (int64_t)ranks * DISTILL_WIDE) ranks *= 2;
+  const int64_t pieces = g.width / Vec16<T>::N;  // at most, whatever the row's first byte
+  // the fewest blocks that hold the row in eight pieces per thread; more of them while that leaves SMs without work.
+  // Blocks of 256 threads, four to an SM, cover one another's waits better than two of 512; those serve the widest rows.
+  int ranks = 1, threads = DW_T;
+  if (pieces > (int64_t)8 * 8 * threads) threads = DISTILL_WIDE;
+  while (ranks < 8 && pieces > (int64_t)ranks * 8 * threads) ranks *= 2;
+  while (ranks < 8 && g.rows * ranks < sms && pieces > (int64_t)ranks * threads) ranks *= 2;
   if (g.rows * ranks > 0x7fffffffll) return MGBS_ERR_TOO_LARGE;
   const int per_block = (int)((pieces + ranks - 1) / ranks);
-  if (per_block <= DISTILL_WIDE) return distill_wide_as<T, 1, GRAD>(g, ranks, per_block, st);
-  if (per_block <= 2 * DISTILL_WIDE) return distill_wide_as<T, 2, GRAD>(g, ranks, per_block, st);
-  if (per_block <= 4 * DISTILL_WIDE) return distill_wide_as<T, 4, GRAD>(g, ranks, per_block, st);
-  return distill_wide_as<T, 8, GRAD>(g, ranks, per_block, st);
+  if (per_block <= threads) return distill_wide_as<T, 1, GRAD>(g, ranks, per_block, threads, st);
+  if (per_block <= 2 * threads) return distill_wide_as<T, 2, GRAD>(g, ranks, per_block, threads, st);
+  if (per_block <= 4 * threads) return distill_wide_as<T, 4, GRAD>(g, ranks, per_block, threads, st);
+  return distill_wide_as<T, 8, GRAD>(g, ranks, per_block, threads, st);
 }
 
 template <typename T> int distill_typed(const DistillArgs& g, cudaStream_t st) {

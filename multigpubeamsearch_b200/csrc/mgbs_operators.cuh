@@ -45,9 +45,24 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
 }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
+// Largest of two packed pairs, and of a pair (a NaN counts as nothing, as with fmaxf).
+template <typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t max2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <> __device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b) {
+  const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+
 // 16 bytes of elements <-> float32
 template <typename T> struct Vec16 {
   static constexpr int N = 16 / (int)sizeof(T);
+  static __device__ __forceinline__ float top(const uint4& r) {
+    const float2 f = unpack2<T>(max2<T>(max2<T>(r.x, r.y), max2<T>(r.z, r.w)));
+    return fmaxf(f.x, f.y);
+  }
   static __device__ __forceinline__ void up(const uint4& r, float* v) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -59,6 +74,9 @@ template <typename T> struct Vec16 {
 };
 template <> struct Vec16<float> {
   static constexpr int N = 4;
+  static __device__ __forceinline__ float top(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
   static __device__ __forceinline__ void up(const uint4& r, float* v) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
   }
