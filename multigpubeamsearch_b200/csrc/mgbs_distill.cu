@@ -5,10 +5,9 @@
 // A row without entries has loss 0 and gradient 0; an index given twice counts with both probabilities.
 //
 // What bounds it: bytes, one read of z and (with the gradient) one write.  Two forms, by the width of a row:
-// up to 1024 entries a group of 4 to 32 lanes holds the row in registers; wider rows are split over a block, or over a
-// cluster of up to eight, each thread holding up to eight 16-byte pieces in registers between the pass that takes
-// maximum and sum and the pass that writes the gradient, so that z is read once.  Rows that not even a cluster holds
-// (over 512 KB) are read twice.  Sums are in float32 and in a fixed order; no atomics.
+// up to 1024 entries a group of 4 to 32 lanes holds the row in registers; a wider row is held in the shared memory of a
+// block, or of a cluster of up to eight, between the pass that takes maximum and sum and the pass that writes the
+// gradient, so that z is read once.  Rows that not even a cluster holds (over 864 KB) are read twice.  Sums are in float32 and in a fixed order; no atomics.
 
 #include <math.h>
 
@@ -135,9 +134,6 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
 // ---------------------------------------------------------------------------------------------------------------
 
 constexpr int DISTILL_WIDE = 512;  // threads of a block at most
-#ifndef DW_T
-#define DW_T 256
-#endif
 
 // Maximum m of some logits and the sum of 2^(x c - k), k = m c rounded to a whole number: sums of different m differ by
 // exact powers of two, and a term costs one fused step without an error of its own in k.
@@ -149,38 +145,52 @@ __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
   return {m, a.s * to.from(a.m) + b.s * to.from(b.m)};
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ void put_remote(float2* local, int rank, float2 v) {  // the same address in block `rank`
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
+// n of them in shared memory, in order.
+__device__ __forceinline__ MaxSum gather(const MaxSum* v, int n, float c) {
+  float m = v[0].m;
+  for (int i = 1; i < n; ++i) m = fmaxf(m, v[i].m);
+  const float k = rintf(m * c);
+  if (fabsf(k) <= 0x1p20f) {
+    float s = 0.f;
+    for (int i = 0; i < n; ++i) s += v[i].m == -INFINITY ? 0.f : v[i].s * fast_exp2(fmaxf(rintf(v[i].m * c), -0x1p30f) - k);
+    return {m, s};
+  }
+  MaxSum all = v[0];
+  for (int i = 1; i < n; ++i) all = merge(all, v[i], c);
+  return all;
 }
 
-// 16 bytes of -inf: what a thread holds where the row has ended
-template <typename T> __device__ __forceinline__ uint4 nothing16();
-template <> __device__ __forceinline__ uint4 nothing16<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
-template <> __device__ __forceinline__ uint4 nothing16<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
-template <> __device__ __forceinline__ uint4 nothing16<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void put_remote(MaxSum* local, int rank, MaxSum v) {  // the same address in block `rank`
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.m), "f"(v.s) : "memory");
+}
 
-// One row per cluster, in pieces of 16 bytes on 16-byte boundaries; the elements before the first and after the last
-// boundary belong to single threads of the first and the last block.  The unrolled loops hold the ordinary case alone
-// (out-of-proportion maxima and outputs on other boundaries go through rolled ones): instruction fetch counts here.  Blocks send one another their maximum and sum
-// and meet once; everything about the teacher's entries is fetched while the row is on its way.
-template <typename T, int NV, bool GRAD>
-__global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_constant__ DistillArgs g, int ranks, int pieces_per_block) {
+// One row per cluster of `ranks` blocks, in pieces of 16 bytes on 16-byte boundaries; the elements before the first and
+// after the last boundary belong to single threads of the first and the last block.  Shared memory stands in for
+// registers: a thread copies its own pieces there asynchronously, in four groups, and reads only those, first for maximum
+// and sum as the groups arrive, then for the gradient.  Two blocks of an SM cover one another's waits.  Blocks of a
+// cluster send one another their maximum and sum and meet once; everything about the teacher's entries is fetched while
+// the row is on its way.
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_constant__ DistillArgs g, int ranks, int pieces_per_block, int capacity) {
   constexpr int E = Vec16<T>::N;
+  extern __shared__ __align__(16) uint8_t held[];  // [capacity] pieces, then the entries
   __shared__ MaxSum warp_part[DISTILL_WIDE / 32];
-  __shared__ float2 parts[8];                       // maximum and sum of every block of the cluster
-  __shared__ float s_t[MGBS_DISTILL_MAX_ENTRIES];   // teacher logits
-  __shared__ float s_z[MGBS_DISTILL_MAX_ENTRIES];   // the student's at the same columns
-  __shared__ __align__(16) int s_i[MGBS_DISTILL_MAX_ENTRIES];
+  __shared__ MaxSum parts[8];                       // maximum and sum of every block of the cluster
   __shared__ float s_tm, s_ts;
   __shared__ int s_any;
+  const int entries4 = (g.entries + 3) / 4;
+  int* s_i = reinterpret_cast<int*>(held + (size_t)capacity * 16);
+  float* s_t = reinterpret_cast<float*>(s_i + 4 * entries4);  // teacher logits
+  float* s_z = s_t + 4 * entries4;                            // the student's at the same columns
   const int rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
   const int64_t row = blockIdx.x / ranks;
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
-  if (ranks > 1) cluster_arrive();  // "this block runs": waited for before anything is sent to it
+  if (ranks > 1) cluster_arrive_relaxed();  // "this block runs": waited for before anything is sent to it
   const T* z = static_cast<const T*>(g.logits) + row * g.row_stride;
   const int head = (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T));  // elements before the first boundary
   const int pieces = (g.width - head) / E, tail = g.width - head - pieces * E;
@@ -189,52 +199,75 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   const bool last = rank == ranks - 1;
   const int edge = rank == 0 && tid < head ? tid : last && tid >= 32 && tid < 32 + tail ? g.width - tail + tid - 32 : -1;
   const float edge_z = edge >= 0 ? Elem<T>::up(z[edge]) : -INFINITY;
-  uint4 raw[NV];
+  const uint4* mine16 = reinterpret_cast<const uint4*>(held) + tid;
+  const uint32_t mine_at = smem_addr(mine16);
+  const int turns = (min(capacity, p1 - p0) + threads - 1) / threads, group = (turns + 3) / 4;  // pieces per thread, and of them per group
   auto fetch = [&](int base) {
+    const int end = min(p1, base + capacity);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int p = base + i * threads + tid;
-      raw[i] = p < p1 ? __ldg(body + p) : nothing16<T>();
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll 2
+      for (int i = q * group; i < (q + 1) * group; ++i) {
+        const int p = base + i * threads + tid;
+        if (p < end) copy16(mine_at + i * threads * 16, body + p, 16);
+      }
+      copy_commit();
     }
   };
   fetch(p0);
-  const int entries4 = (g.entries + 3) / 4;
   for (int k = tid; k < 4 * entries4; k += threads) {
     const int i = k < g.entries ? distill_index(g, row, k) : -1;
     s_i[k] = i;
     s_t[k] = k < g.entries ? g.teacher[row * g.teacher_stride + k] : -INFINITY;
     s_z[k] = i >= 0 ? Elem<T>::up(z[i]) : 0.f;
   }
+  const float w = GRAD ? (g.weight ? g.weight[row] : 1.f) * g.inv_t : 0.f;
   MaxSum mine{-INFINITY, 0.f};
-  for (int base = p0; base == p0 || base < p1; base += NV * threads) {
-    if (base != p0) fetch(base);
-    float top = base == p0 ? edge_z : mine.m;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) top = fmaxf(top, Vec16<T>::top(raw[i]));
+  auto take = [&](int base, int q, float extra) {  // group q of the pieces held from `base` on
+    const int end = min(p1, base + capacity);
+    float top = fmaxf(mine.m, extra);
+#pragma unroll 2
+    for (int i = q * group; i < (q + 1) * group; ++i)
+      if (base + i * threads + tid < end) top = fmaxf(top, Vec16<T>::top(mine16[i * threads]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const Scale sc(top == -INFINITY ? 0.f : top, g.c);  // one for the warp
-    mine.s = base == p0 ? fast_exp2(sc.arg(edge_z)) : mine.s * sc.from(mine.m);
+    mine.s = mine.s * sc.from(mine.m) + fast_exp2(sc.arg(extra));
     mine.m = top;
     if (!sc.huge) {
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const Pair c2 = pair(g.c, g.c), k2 = pair(-sc.k, -sc.k);
+      Pair part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll 2
+      for (int i = q * group; i < (q + 1) * group; ++i)
+        if (base + i * threads + tid < end) {
+          float v[E];
+          Vec16<T>::up(mine16[i * threads], v);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float v[E];
-        Vec16<T>::up(raw[i], v);
-#pragma unroll
-        for (int j = 0; j < E; ++j) part[j & 3] += fast_exp2(fmaf(v[j], g.c, -sc.k));
-      }
-      mine.s += (part[0] + part[1]) + (part[2] + part[3]);
+          for (int j = 0; j < E; j += 2) part[j / 2 & 1] = add2(part[j / 2 & 1], exp2_2(fma2(pair(v[j], v[j + 1]), c2, k2)));
+        }
+      const float2 sum = both(add2(part[0], part[1]));
+      mine.s += sum.x + sum.y;
     } else {
 #pragma unroll 1
-      for (int p = base + tid; p < min(p1, base + NV * threads); p += threads) {
-        float v[E];
-        Vec16<T>::up(__ldg(body + p), v);
+      for (int i = q * group; i < (q + 1) * group; ++i)
+        if (base + i * threads + tid < end) {
+          float v[E];
+          Vec16<T>::up(mine16[i * threads], v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) mine.s += fast_exp2(sc.arg(v[j]));
-      }
+          for (int j = 0; j < E; ++j) mine.s += fast_exp2(sc.arg(v[j]));
+        }
     }
+  };
+  for (int base = p0; base == p0 || base < p1; base += capacity) {
+    if (base != p0) fetch(base);
+    copy_wait<3>();
+    take(base, 0, base == p0 ? edge_z : -INFINITY);
+    copy_wait<2>();
+    take(base, 1, -INFINITY);
+    copy_wait<1>();
+    take(base, 2, -INFINITY);
+    copy_wait<0>();
+    take(base, 3, -INFINITY);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
@@ -242,15 +275,9 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   __syncthreads();
   if (ranks > 1) cluster_wait();
   if (warp == 0) {
-    mine = lane < threads / 32 ? warp_part[lane] : MaxSum{-INFINITY, 0.f};
-#pragma unroll
-    for (int o = DISTILL_WIDE / 64; o > 0; o >>= 1) {
-      const MaxSum other{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o)};
-      mine = merge(mine, other, g.c);
-    }
-    const MaxSum whole{__shfl_sync(0xffffffffu, mine.m, 0), __shfl_sync(0xffffffffu, mine.s, 0)};
-    if (ranks == 1) { if (lane == 0) parts[0] = make_float2(whole.m, whole.s); }
-    else if (lane < ranks) put_remote(&parts[rank], lane, make_float2(whole.m, whole.s));
+    const MaxSum whole = gather(warp_part, threads / 32, g.c);
+    if (ranks == 1) { if (lane == 0) parts[0] = whole; }
+    else if (lane < ranks) put_remote(&parts[rank], lane, whole);
   } else if (warp == 1) {  // the teacher's softmax
     float tm = -INFINITY, ts = 0.f;
     int any = 0;
@@ -269,8 +296,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   }
   if (ranks > 1) { cluster_arrive(); cluster_wait(); }
   else __syncthreads();
-  MaxSum all{parts[0].x, parts[0].y};
-  for (int r = 1; r < ranks; ++r) all = merge(all, MaxSum{parts[r].x, parts[r].y}, g.c);
+  const MaxSum all = gather(parts, ranks, g.c);
   const Scale sc(all.m, g.c);
   const float tm = s_tm, inv_ts = 1.f / s_ts;
   const bool any = s_any != 0;
@@ -290,30 +316,36 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   if (GRAD) {
     T* out = static_cast<T*>(g.grad) + row * g.grad_stride;
     const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
-    const float w = (g.weight ? g.weight[row] : 1.f) * g.inv_t;
     const float scale = any ? w / all.s : 0.f;
     if (edge >= 0) out[edge] = Elem<T>::down(any ? fast_exp2(sc.arg(edge_z)) * scale : 0.f);
     T* out_body = out + head;
-    if (same && any && !sc.huge) {
-      for (int base = p0; base < p1; base += NV * threads) {
-        if (p1 - p0 > NV * threads) fetch(base);  // the row does not stay in registers
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int p = base + i * threads + tid;
-          float v[E];
-          Vec16<T>::up(raw[i], v);
-#pragma unroll
-          for (int j = 0; j < E; ++j) v[j] = fast_exp2(fmaf(v[j], g.c, -sc.k)) * scale;
-          if (p < p1) reinterpret_cast<uint4*>(out_body)[p] = Vec16<T>::down(v);
-        }
+    const Pair c2 = pair(g.c, g.c), k2 = pair(-sc.k, -sc.k), w2 = pair(scale, scale);
+    for (int base = p0; base < p1; base += capacity) {
+      const int end = min(p1, base + capacity);
+      if (p1 - p0 > capacity) {  // the row is not all held
+        fetch(base);
+        copy_wait<0>();
       }
-    } else {
-#pragma unroll 1
-      for (int p = p0 + tid; p < p1; p += threads) {
-        float v[E];
-        Vec16<T>::up(__ldg(body + p), v);
+      if (same && any && !sc.huge) {
+#pragma unroll 2
+        for (int p = base + tid, i = 0; p < end; p += threads, i += threads) {
+          float v[E];
+          Vec16<T>::up(mine16[i], v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) out_body[p * E + j] = Elem<T>::down(any ? fast_exp2(sc.arg(v[j])) * scale : 0.f);
+          for (int j = 0; j < E; j += 2) {
+            const float2 q = both(mul2(exp2_2(fma2(pair(v[j], v[j + 1]), c2, k2)), w2));
+            v[j] = q.x; v[j + 1] = q.y;
+          }
+          reinterpret_cast<uint4*>(out_body)[p] = Vec16<T>::down(v);
+        }
+      } else {
+#pragma unroll 1
+        for (int p = base + tid, i = 0; p < end; p += threads, i += threads) {
+          float v[E];
+          Vec16<T>::up(mine16[i], v);
+#pragma unroll
+          for (int j = 0; j < E; ++j) out_body[p * E + j] = Elem<T>::down(any ? fast_exp2(sc.arg(v[j])) * scale : 0.f);
+        }
       }
     }
     __syncthreads();
@@ -355,10 +387,25 @@ template <typename T, bool GRAD> int distill_rows(const DistillArgs& g, cudaStre
   return (int)cudaGetLastError();
 }
 
-template <typename T, int NV, bool GRAD> int distill_wide_as(const DistillArgs& g, int ranks, int per_block, int threads, cudaStream_t st) {
+constexpr int DISTILL_HELD = 108 * 1024;  // bytes of a row per block: two blocks and their entries fit an SM
+template <typename T, bool GRAD> int distill_wide(const DistillArgs& g, int sms, cudaStream_t st) {
+  static std::atomic<uint64_t> raised{0};
+  const int rc = raise_smem(k_distill_wide<T, GRAD>, DISTILL_HELD + 12 * MGBS_DISTILL_MAX_ENTRIES, raised);
+  if (rc) return rc;
+  const int64_t pieces = g.width / Vec16<T>::N;  // at most, whatever the row's first byte
+  // the fewest blocks that hold the row; more of them while that leaves SMs without work
+  int64_t ranks = (pieces * 16 + DISTILL_HELD - 1) / DISTILL_HELD;
+  if (ranks > 8) ranks = 8;
+  while (ranks < 8 && g.rows * ranks < sms && pieces > ranks * 1024) ++ranks;
+  if (g.rows * ranks > 0x7fffffffll) return MGBS_ERR_TOO_LARGE;
+  const int per_block = (int)((pieces + ranks - 1) / ranks);
+  const int capacity = per_block * 16 <= DISTILL_HELD ? per_block : DISTILL_HELD / 16;
+  int threads = 128;  // some four pieces per thread and more
+  while (threads < DISTILL_WIDE && threads * 8 <= per_block) threads *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(g.rows * ranks));
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (size_t)capacity * 16 + (size_t)(g.entries + 3) / 4 * 4 * 12;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -366,23 +413,7 @@ template <typename T, int NV, bool GRAD> int distill_wide_as(const DistillArgs& 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, k_distill_wide<T, NV, GRAD>, g, ranks, per_block);
-}
-
-template <typename T, bool GRAD> int distill_wide(const DistillArgs& g, int sms, cudaStream_t st) {
-  const int64_t pieces = g.width / Vec16<T>::N;  // at most, whatever the row's first byte
-  // the fewest blocks that hold the row in eight pieces per thread; more of them while that leaves SMs without work.
-  // Blocks of 256 threads, four to an SM, cover one another's waits better than two of 512; those serve the widest rows.
-  int ranks = 1, threads = DW_T;
-  if (pieces > (int64_t)8 * 8 * threads) threads = DISTILL_WIDE;
-  while (ranks < 8 && pieces > (int64_t)ranks * 8 * threads) ranks *= 2;
-  while (ranks < 8 && g.rows * ranks < sms && pieces > (int64_t)ranks * threads) ranks *= 2;
-  if (g.rows * ranks > 0x7fffffffll) return MGBS_ERR_TOO_LARGE;
-  const int per_block = (int)((pieces + ranks - 1) / ranks);
-  if (per_block <= threads) return distill_wide_as<T, 1, GRAD>(g, ranks, per_block, threads, st);
-  if (per_block <= 2 * threads) return distill_wide_as<T, 2, GRAD>(g, ranks, per_block, threads, st);
-  if (per_block <= 4 * threads) return distill_wide_as<T, 4, GRAD>(g, ranks, per_block, threads, st);
-  return distill_wide_as<T, 8, GRAD>(g, ranks, per_block, threads, st);
+  return (int)cudaLaunchKernelEx(&cfg, k_distill_wide<T, GRAD>, g, (int)ranks, per_block, capacity);
 }
 
 template <typename T> int distill_typed(const DistillArgs& g, cudaStream_t st) {
