@@ -43,11 +43,6 @@ struct Scale {
     huge = !(fabsf(k) <= 0x1p20f);
   }
   __device__ __forceinline__ float arg(float x) const { return huge ? (x - m) * c : fmaf(x, c, -k); }
-  // what a sum taken relative to maximum `other` is multiplied with
-  __device__ __forceinline__ float from(float other) const {
-    const Scale o(other, c);
-    return fast_exp2(huge || o.huge ? (other - m) * c : o.k - k);
-  }
 };
 
 constexpr int DISTILL_THREADS = 256;
@@ -135,58 +130,57 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
 
 constexpr int DISTILL_WIDE = 512;  // threads of a block at most
 
-// Maximum m of some logits and the sum of 2^(x c - k), k = m c rounded to a whole number: sums of different m differ by
-// exact powers of two, and a term costs one fused step without an error of its own in k.
-struct MaxSum { float m, s; };
+// Sum of 2^(x c - k) over some logits, k whole: sums of different k differ by exact powers of two, and a term costs one
+// fused step without an error of its own in k.
+struct Sum { int k; float s; };
+constexpr int DISTILL_FAR = 1 << 24;  // |k| of logits out of all proportion: the row takes the slow way
 
-__device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  const Scale to(m == -INFINITY ? 0.f : m, c);  // nothing yet on either side: both sums are 0
-  return {m, a.s * to.from(a.m) + b.s * to.from(b.m)};
-}
-
-// n of them in shared memory, in order.
-__device__ __forceinline__ MaxSum gather(const MaxSum* v, int n, float c) {
-  float m = v[0].m;
-  for (int i = 1; i < n; ++i) m = fmaxf(m, v[i].m);
-  const float k = rintf(m * c);
-  if (fabsf(k) <= 0x1p20f) {
-    float s = 0.f;
-    for (int i = 0; i < n; ++i) s += v[i].m == -INFINITY ? 0.f : v[i].s * fast_exp2(fmaxf(rintf(v[i].m * c), -0x1p30f) - k);
-    return {m, s};
-  }
-  MaxSum all = v[0];
-  for (int i = 1; i < n; ++i) all = merge(all, v[i], c);
-  return all;
+// n <= 32 of them in shared memory, in a fixed order; the whole warp calls.
+__device__ __forceinline__ Sum gather(const Sum* v, int n) {
+  const int lane = threadIdx.x & 31;
+  const Sum own = lane < n ? v[lane] : Sum{-2 * DISTILL_FAR, 0.f};
+  const int k = __reduce_max_sync(0xffffffffu, own.k);
+  float s = own.s * fast_exp2((float)(own.k - k));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return {k, s};
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ void put_remote(MaxSum* local, int rank, MaxSum v) {  // the same address in block `rank`
+__device__ __forceinline__ void put_remote(Sum* local, int rank, Sum v) {  // the same address in block `rank`
   uint32_t at;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.m), "f"(v.s) : "memory");
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(v.k), "r"(__float_as_int(v.s)) : "memory");
 }
+
+// 16 bytes of -inf: what a thread holds where the row has ended
+template <typename T> __device__ __forceinline__ uint4 nothing16();
+template <> __device__ __forceinline__ uint4 nothing16<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+template <> __device__ __forceinline__ uint4 nothing16<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+template <> __device__ __forceinline__ uint4 nothing16<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
 
 // One row per cluster of `ranks` blocks, in pieces of 16 bytes on 16-byte boundaries; the elements before the first and
 // after the last boundary belong to single threads of the first and the last block.  Shared memory stands in for
-// registers: a thread copies its own pieces there asynchronously, in four groups, and reads only those, first for maximum
-// and sum as the groups arrive, then for the gradient.  Two blocks of an SM cover one another's waits.  Blocks of a
-// cluster send one another their maximum and sum and meet once; everything about the teacher's entries is fetched while
-// the row is on its way.
+// registers: a thread copies its own pieces there asynchronously and reads only those, first for the sum as they arrive,
+// then for the gradient.  Two blocks of an SM cover one another's waits.  The sum's scale is a warp's maximum over its
+// first pieces alone: float32 has room for 2^100 above it, so no further maximum is taken; a warp whose sum leaves that
+// room (logits far above its first ones, or nothing but masks among those) makes it anew with its true maximum.  Blocks
+// of a cluster send one another their sums and meet once; one warp sees to the teacher's entries while the row is on
+// its way.
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_constant__ DistillArgs g, int ranks, int pieces_per_block, int capacity) {
   constexpr int E = Vec16<T>::N;
   extern __shared__ __align__(16) uint8_t held[];  // [capacity] pieces, then the entries
-  __shared__ MaxSum warp_part[DISTILL_WIDE / 32];
-  __shared__ MaxSum parts[8];                       // maximum and sum of every block of the cluster
-  __shared__ float s_tm, s_ts;
+  __shared__ Sum warp_part[DISTILL_WIDE / 32];
+  __shared__ Sum parts[8];  // of every block of the cluster
+  __shared__ float s_ts;
   __shared__ int s_any;
   const int entries4 = (g.entries + 3) / 4;
   int* s_i = reinterpret_cast<int*>(held + (size_t)capacity * 16);
-  float* s_t = reinterpret_cast<float*>(s_i + 4 * entries4);  // teacher logits
-  float* s_z = s_t + 4 * entries4;                            // the student's at the same columns
+  float* s_p = reinterpret_cast<float*>(s_i + 4 * entries4);  // the entry's probability times s_ts
+  float* s_z = s_p + 4 * entries4;                            // the student's logit there
   const int rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
   const int64_t row = blockIdx.x / ranks;
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
@@ -201,117 +195,179 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   const float edge_z = edge >= 0 ? Elem<T>::up(z[edge]) : -INFINITY;
   const uint4* mine16 = reinterpret_cast<const uint4*>(held) + tid;
   const uint32_t mine_at = smem_addr(mine16);
-  const int turns = (min(capacity, p1 - p0) + threads - 1) / threads, group = (turns + 3) / 4;  // pieces per thread, and of them per group
+  constexpr int TURN = 4;  // pieces per thread and turn: one group of copies
+  const int turns = (min(capacity, p1 - p0) + TURN * threads - 1) / (TURN * threads);
   auto fetch = [&](int base) {
     const int end = min(p1, base + capacity);
+    for (int t = 0; t < turns; ++t) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-#pragma unroll 2
-      for (int i = q * group; i < (q + 1) * group; ++i) {
-        const int p = base + i * threads + tid;
-        if (p < end) copy16(mine_at + i * threads * 16, body + p, 16);
+      for (int i = 0; i < TURN; ++i) {
+        const int at = (t * TURN + i) * threads;
+        if (base + at + tid < end) copy16(mine_at + at * 16, body + base + at + tid, 16);
       }
       copy_commit();
     }
   };
   fetch(p0);
-  for (int k = tid; k < 4 * entries4; k += threads) {
-    const int i = k < g.entries ? distill_index(g, row, k) : -1;
-    s_i[k] = i;
-    s_t[k] = k < g.entries ? g.teacher[row * g.teacher_stride + k] : -INFINITY;
-    s_z[k] = i >= 0 ? Elem<T>::up(z[i]) : 0.f;
-  }
   const float w = GRAD ? (g.weight ? g.weight[row] : 1.f) * g.inv_t : 0.f;
-  MaxSum mine{-INFINITY, 0.f};
-  auto take = [&](int base, int q, float extra) {  // group q of the pieces held from `base` on
-    const int end = min(p1, base + capacity);
-    float top = fmaxf(mine.m, extra);
-#pragma unroll 2
-    for (int i = q * group; i < (q + 1) * group; ++i)
-      if (base + i * threads + tid < end) top = fmaxf(top, Vec16<T>::top(mine16[i * threads]));
+  float entropy = 0.f;  // warp 1: sum p log2 p, later the loss
+  if (warp == 1) {
+    float tm = -INFINITY, ts = 0.f;
+    int any = 0;
+    for (int k = lane; k < 4 * entries4; k += 32) {
+      const int i = k < g.entries ? distill_index(g, row, k) : -1;
+      const float t = i >= 0 ? g.teacher[row * g.teacher_stride + k] : -INFINITY;
+      s_i[k] = i;
+      s_p[k] = t;
+      s_z[k] = i >= 0 ? Elem<T>::up(z[i]) : 0.f;
+      any |= t != -INFINITY;
+      tm = fmaxf(tm, t);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const Scale sc(top == -INFINITY ? 0.f : top, g.c);  // one for the warp
-    mine.s = mine.s * sc.from(mine.m) + fast_exp2(sc.arg(extra));
-    mine.m = top;
-    if (!sc.huge) {
-      const Pair c2 = pair(g.c, g.c), k2 = pair(-sc.k, -sc.k);
-      Pair part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-#pragma unroll 2
-      for (int i = q * group; i < (q + 1) * group; ++i)
-        if (base + i * threads + tid < end) {
+    for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+    any = __any_sync(0xffffffffu, any);
+    for (int k = lane; k < 4 * entries4; k += 32) {
+      const float t = any ? (s_p[k] - tm) * g.c : -INFINITY, p = fast_exp2(t);
+      ts += p;
+      if (p != 0.f) entropy += p * t;
+      s_p[k] = p;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ts += __shfl_xor_sync(0xffffffffu, ts, o);
+      entropy += __shfl_xor_sync(0xffffffffu, entropy, o);
+    }
+    if (lane == 0) { s_ts = ts; s_any = any; }
+    __syncwarp();
+  }
+  Sum mine{0, 0.f};
+  {
+    const Pair c2 = pair(g.c, g.c);
+    Pair k2 = pair(0.f, 0.f), part[2] = {k2, k2};
+    for (int base = p0; base == p0 || base < p1; base += capacity) {
+      if (base != p0) fetch(base);
+      const int end = min(p1, base + capacity);
+      for (int t = 0; t < turns || (t == 0 && base == p0); ++t) {
+        const int left = turns - 1 - t;  // groups still on their way
+        if (left >= 3) copy_wait<3>();
+        else if (left == 2) copy_wait<2>();
+        else if (left == 1) copy_wait<1>();
+        else copy_wait<0>();
+        uint4 raw[TURN];
+#pragma unroll
+        for (int i = 0; i < TURN; ++i) {
+          const int at = (t * TURN + i) * threads;
+          raw[i] = base + at + tid < end ? mine16[at] : nothing16<T>();
+        }
+        if (t == 0 && base == p0) {
+          float top = edge_z;
+#pragma unroll
+          for (int i = 0; i < TURN; ++i) top = fmaxf(top, Vec16<T>::top(raw[i]));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float k = rintf(top * g.c);
+          mine.k = fabsf(k) <= 0x1p20f ? (int)k : 0;
+          k2 = pair(-(float)mine.k, -(float)mine.k);
+          part[0] = pair(fast_exp2(fmaf(edge_z, g.c, -(float)mine.k)), 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < TURN; ++i) {
           float v[E];
-          Vec16<T>::up(mine16[i * threads], v);
+          Vec16<T>::up(raw[i], v);
 #pragma unroll
           for (int j = 0; j < E; j += 2) part[j / 2 & 1] = add2(part[j / 2 & 1], exp2_2(fma2(pair(v[j], v[j + 1]), c2, k2)));
         }
-      const float2 sum = both(add2(part[0], part[1]));
-      mine.s += sum.x + sum.y;
-    } else {
-#pragma unroll 1
-      for (int i = q * group; i < (q + 1) * group; ++i)
-        if (base + i * threads + tid < end) {
-          float v[E];
-          Vec16<T>::up(mine16[i * threads], v);
-#pragma unroll
-          for (int j = 0; j < E; ++j) mine.s += fast_exp2(sc.arg(v[j]));
-        }
+      }
     }
-  };
-  for (int base = p0; base == p0 || base < p1; base += capacity) {
-    if (base != p0) fetch(base);
-    copy_wait<3>();
-    take(base, 0, base == p0 ? edge_z : -INFINITY);
-    copy_wait<2>();
-    take(base, 1, -INFINITY);
-    copy_wait<1>();
-    take(base, 2, -INFINITY);
-    copy_wait<0>();
-    take(base, 3, -INFINITY);
+    const float2 sum = both(add2(part[0], part[1]));
+    mine.s = sum.x + sum.y;
   }
+  // The slow way, from global memory: this thread's maximum, and its sum relative to a given one.
+  auto maximum = [&]() {
+    float top = edge_z;
+#pragma unroll 1
+    for (int p = p0 + tid; p < p1; p += threads) top = fmaxf(top, Vec16<T>::top(__ldg(body + p)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+  };
+  auto sum_to = [&](const Scale& sc) {
+    float sum = edge >= 0 ? fast_exp2(sc.arg(edge_z)) : 0.f;
+#pragma unroll 1
+    for (int p = p0 + tid; p < p1; p += threads) {
+      float v[E];
+      Vec16<T>::up(__ldg(body + p), v);
+#pragma unroll
+      for (int j = 0; j < E; ++j) sum += fast_exp2(sc.arg(v[j]));
+    }
+    return sum;
+  };
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
-  if (lane == 0) warp_part[warp] = mine;
-  __syncthreads();
-  if (ranks > 1) cluster_wait();
-  if (warp == 0) {
-    const MaxSum whole = gather(warp_part, threads / 32, g.c);
-    if (ranks == 1) { if (lane == 0) parts[0] = whole; }
-    else if (lane < ranks) put_remote(&parts[rank], lane, whole);
-  } else if (warp == 1) {  // the teacher's softmax
-    float tm = -INFINITY, ts = 0.f;
-    int any = 0;
-    for (int k = lane; k < g.entries; k += 32)
-      if (s_i[k] >= 0 && s_t[k] != -INFINITY) { any = 1; tm = fmaxf(tm, s_t[k]); }
+  if (!(mine.s >= 0x1p-40f && mine.s <= 0x1p100f)) {  // the whole warp
+    const Scale sc(maximum(), g.c);
+    mine.k = sc.huge ? (sc.m > 0.f ? DISTILL_FAR : -DISTILL_FAR) : (int)sc.k;
+    mine.s = sc.huge ? 0.f : sum_to(sc);
+    if (!sc.huge) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-      any |= __shfl_xor_sync(0xffffffffu, any, o);
+      for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
     }
-    for (int k = lane; k < g.entries; k += 32)
-      if (s_i[k] >= 0) ts += fast_exp2((s_t[k] - tm) * g.c);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ts += __shfl_xor_sync(0xffffffffu, ts, o);
-    if (lane == 0) { s_tm = tm; s_ts = ts; s_any = any; }
   }
-  if (ranks > 1) { cluster_arrive(); cluster_wait(); }
-  else __syncthreads();
-  const MaxSum all = gather(parts, ranks, g.c);
-  const Scale sc(all.m, g.c);
-  const float tm = s_tm, inv_ts = 1.f / s_ts;
-  const bool any = s_any != 0;
-  if (rank == 0 && warp == 0) {
-    const float log_ratio = log2f(all.s) - log2f(s_ts);
-    float loss = 0.f;
-    if (any)
-      for (int k = lane; k < g.entries; k += 32) {
-        if (s_i[k] < 0) continue;
-        const float t = (s_t[k] - tm) * g.c, p = fast_exp2(t) * inv_ts;
-        if (p != 0.f) loss += p * (t - sc.arg(s_z[k]) + log_ratio);
-      }
+  // sums of the block, and of the cluster: every warp ends with the same
+  bool first = true;
+  auto collect = [&](Sum v) {
+    __syncthreads();
+    if (lane == 0) warp_part[warp] = v;
+    __syncthreads();
+    if (ranks == 1) return gather(warp_part, threads / 32);
+    if (first) cluster_wait();  // all blocks run
+    first = false;
+    if (warp == 0) {
+      const Sum whole = gather(warp_part, threads / 32);
+      if (lane < ranks) put_remote(&parts[rank], lane, whole);
+    }
+    cluster_arrive();
+    cluster_wait();
+    const Sum all = gather(parts, ranks);
+    return all;
+  };
+  Sum all = collect(mine);
+  Scale sc(0.f, g.c);
+  sc.k = (float)all.k;
+  if (abs(all.k) >= DISTILL_FAR) {  // the whole cluster: once more, relative to the row's maximum
+    const float top = maximum();
+    __syncthreads();
+    if (lane == 0) warp_part[warp] = Sum{0, top};
+    __syncthreads();
+    float m = warp_part[0].s;
+    for (int i = 1; i < threads / 32; ++i) m = fmaxf(m, warp_part[i].s);
+    if (ranks > 1) {
+      cluster_arrive();  // all have read the parts before
+      cluster_wait();
+      if (tid < ranks) put_remote(&parts[rank], tid, Sum{0, m});
+      cluster_arrive();
+      cluster_wait();
+      for (int i = 0; i < ranks; ++i) m = fmaxf(m, parts[i].s);
+      cluster_arrive();
+      cluster_wait();
+    }
+    sc = Scale(m, g.c);
+    sc.huge = true;
+    float sum = sum_to(sc);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-    if (lane == 0) g.loss[row] = loss * kLn2;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    all = collect(Sum{0, sum});
+  }
+  const bool any = s_any != 0;
+  const float inv_ts = 1.f / s_ts;
+  if (rank == 0 && warp == 1) {
+    // sum p (log p - log q) = (sum e t - sum e arg) / ts - log ts + log s, e = 2^t unnormalised
+    float cross = 0.f;
+    for (int k = lane; k < g.entries; k += 32)
+      if (s_p[k] != 0.f) cross += s_p[k] * sc.arg(s_z[k]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) cross += __shfl_xor_sync(0xffffffffu, cross, o);
+    if (lane == 0) g.loss[row] = any ? ((entropy - cross) * inv_ts + (log2f(all.s) - log2f(s_ts))) * kLn2 : 0.f;
   }
   if (GRAD) {
     T* out = static_cast<T*>(g.grad) + row * g.grad_stride;
@@ -327,7 +383,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
         copy_wait<0>();
       }
       if (same && any && !sc.huge) {
-#pragma unroll 2
+#pragma unroll 4
         for (int p = base + tid, i = 0; p < end; p += threads, i += threads) {
           float v[E];
           Vec16<T>::up(mine16[i], v);
@@ -357,7 +413,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
         const int piece = i < head ? -1 : (i - head) / E;  // -1 and `pieces`: the edges
         if (piece < 0 ? rank != 0 : piece >= pieces ? !last : piece < p0 || piece >= p1) continue;  // another block's column
         float p = 0.f;
-        bool first = true;
+        bool is_first = true;
         for (int n = 0; n < entries4; ++n) {
           const int4 four = reinterpret_cast<const int4*>(s_i)[n];
           if (four.x != i && four.y != i && four.z != i && four.w != i) continue;
@@ -365,11 +421,11 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (f[j] == i) {
-              first = first && 4 * n + j >= k;
-              p += fast_exp2((s_t[4 * n + j] - tm) * g.c);
+              is_first = is_first && 4 * n + j >= k;
+              p += s_p[4 * n + j];
             }
         }
-        if (first) out[i] = Elem<T>::down(fast_exp2(sc.arg(s_z[k])) * scale - p * inv_ts * w);
+        if (is_first) out[i] = Elem<T>::down(fast_exp2(sc.arg(s_z[k])) * scale - p * inv_ts * w);
       }
   }
 }
