@@ -7,7 +7,7 @@
 // What bounds it: bytes, one read of z and (with the gradient) one write.  Two forms, by the width of a row:
 // up to 1024 entries a group of 4 to 32 lanes holds the row in registers; a wider row is held in the shared memory of a
 // block, or of a cluster of up to eight, between the pass that takes maximum and sum and the pass that writes the
-// gradient, so that z is read once.  Rows that not even a cluster holds (over 864 KB) are read twice.  Sums are in float32 and in a fixed order; no atomics.
+// gradient, so that z is read once.  Rows that not even a cluster holds (over 832 KB) are read twice.  Sums are in float32 and in a fixed order; no atomics.
 
 #include <math.h>
 
@@ -155,19 +155,13 @@ __device__ __forceinline__ void put_remote(Sum* local, int rank, Sum v) {  // th
   asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(v.k), "r"(__float_as_int(v.s)) : "memory");
 }
 
-// 16 bytes of -inf: what a thread holds where the row has ended
-template <typename T> __device__ __forceinline__ uint4 nothing16();
-template <> __device__ __forceinline__ uint4 nothing16<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
-template <> __device__ __forceinline__ uint4 nothing16<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
-template <> __device__ __forceinline__ uint4 nothing16<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
-
 // One row per cluster of `ranks` blocks, in pieces of 16 bytes on 16-byte boundaries; the elements before the first and
 // after the last boundary belong to single threads of the first and the last block.  Shared memory stands in for
 // registers: a thread copies its own pieces there asynchronously and reads only those, first for the sum as they arrive,
 // then for the gradient.  Two blocks of an SM cover one another's waits.  The sum's scale is a warp's maximum over its
 // first pieces alone: float32 has room for 2^100 above it, so no further maximum is taken; a warp whose sum leaves that
 // room (logits far above its first ones, or nothing but masks among those) makes it anew with its true maximum.  Blocks
-// of a cluster send one another their sums and meet once; one warp sees to the teacher's entries while the row is on
+// of a cluster send one another their sums and meet once; the last warp sees to the teacher's entries while the row is on
 // its way.
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_constant__ DistillArgs g, int ranks, int pieces_per_block, int capacity) {
@@ -175,15 +169,17 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   extern __shared__ __align__(16) uint8_t held[];  // [capacity] pieces, then the entries
   __shared__ Sum warp_part[DISTILL_WIDE / 32];
   __shared__ Sum parts[8];  // of every block of the cluster
+  __shared__ uint32_t s_seen[1024];  // one bit per column modulo 2^15: whether an index may be there twice
   __shared__ float s_ts;
-  __shared__ int s_any;
+  __shared__ int s_any, s_twice;
   const int entries4 = (g.entries + 3) / 4;
   int* s_i = reinterpret_cast<int*>(held + (size_t)capacity * 16);
   float* s_p = reinterpret_cast<float*>(s_i + 4 * entries4);  // the entry's probability times s_ts
   float* s_z = s_p + 4 * entries4;                            // the student's logit there
   const int rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
   const int64_t row = blockIdx.x / ranks;
-  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int threads = (int)blockDim.x - 32, warps = threads / 32;  // that work on the row; the last warp has the teacher
   if (ranks > 1) cluster_arrive_relaxed();  // "this block runs": waited for before anything is sent to it
   const T* z = static_cast<const T*>(g.logits) + row * g.row_stride;
   const int head = (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T));  // elements before the first boundary
@@ -196,29 +192,35 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   const uint4* mine16 = reinterpret_cast<const uint4*>(held) + tid;
   const uint32_t mine_at = smem_addr(mine16);
   constexpr int TURN = 4;  // pieces per thread and turn: one group of copies
-  const int turns = (min(capacity, p1 - p0) + TURN * threads - 1) / (TURN * threads);
+  // Turns in which every thread has all its pieces need no test; the rest, at most TURN pieces per thread, is the last group.
   auto fetch = [&](int base) {
-    const int end = min(p1, base + capacity);
-    for (int t = 0; t < turns; ++t) {
+    const int count = min(capacity, p1 - base), full = count / (TURN * threads);
+    const uint4* from = body + base + tid;
+    uint32_t to = mine_at;
+    for (int t = 0; t < full; ++t, from += TURN * threads, to += TURN * threads * 16) {
 #pragma unroll
-      for (int i = 0; i < TURN; ++i) {
-        const int at = (t * TURN + i) * threads;
-        if (base + at + tid < end) copy16(mine_at + at * 16, body + base + at + tid, 16);
-      }
+      for (int i = 0; i < TURN; ++i) copy16(to + i * threads * 16, from + i * threads, 16);
       copy_commit();
     }
+#pragma unroll 1
+    for (int at = full * TURN * threads + tid; at < count; at += threads, from += threads, to += threads * 16) copy16(to, from, 16);
+    copy_commit();
   };
-  fetch(p0);
+  if (warp < warps) fetch(p0);
   const float w = GRAD ? (g.weight ? g.weight[row] : 1.f) * g.inv_t : 0.f;
-  float entropy = 0.f;  // warp 1: sum p log2 p, later the loss
-  if (warp == 1) {
+  float entropy = 0.f;  // the last warp: sum p log2 p
+  if (warp == warps) {
     float tm = -INFINITY, ts = 0.f;
     int any = 0;
+    bool twice = false;
+    for (int k = lane; k < 256; k += 32) reinterpret_cast<uint4*>(s_seen)[k] = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
     for (int k = lane; k < 4 * entries4; k += 32) {
       const int i = k < g.entries ? distill_index(g, row, k) : -1;
       const float t = i >= 0 ? g.teacher[row * g.teacher_stride + k] : -INFINITY;
       s_i[k] = i;
       s_p[k] = t;
+      if (i >= 0) twice |= (atomicOr(&s_seen[(i & 32767) >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
       s_z[k] = i >= 0 ? Elem<T>::up(z[i]) : 0.f;
       any |= t != -INFINITY;
       tm = fmaxf(tm, t);
@@ -226,6 +228,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
     any = __any_sync(0xffffffffu, any);
+    twice = __any_sync(0xffffffffu, twice);
     for (int k = lane; k < 4 * entries4; k += 32) {
       const float t = any ? (s_p[k] - tm) * g.c : -INFINITY, p = fast_exp2(t);
       ts += p;
@@ -237,47 +240,59 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
       ts += __shfl_xor_sync(0xffffffffu, ts, o);
       entropy += __shfl_xor_sync(0xffffffffu, entropy, o);
     }
-    if (lane == 0) { s_ts = ts; s_any = any; }
+    if (lane == 0) { s_ts = ts; s_any = any; s_twice = twice; }
     __syncwarp();
   }
   Sum mine{0, 0.f};
-  {
+  if (warp < warps) {
     const Pair c2 = pair(g.c, g.c);
     Pair k2 = pair(0.f, 0.f), part[2] = {k2, k2};
+    auto add16 = [&](const uint4& raw) {
+      float v[E];
+      Vec16<T>::up(raw, v);
+#pragma unroll
+      for (int j = 0; j < E; j += 2) part[j / 2 & 1] = add2(part[j / 2 & 1], exp2_2(fma2(pair(v[j], v[j + 1]), c2, k2)));
+    };
+    auto scale_from = [&](float top) {  // the first pieces' maximum over the warp
+      top = fmaxf(top, edge_z);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float k = rintf(top * g.c);
+      mine.k = fabsf(k) <= 0x1p20f ? (int)k : 0;
+      k2 = pair(-(float)mine.k, -(float)mine.k);
+      part[0] = pair(fast_exp2(fmaf(edge_z, g.c, -(float)mine.k)), 0.f);
+    };
     for (int base = p0; base == p0 || base < p1; base += capacity) {
       if (base != p0) fetch(base);
-      const int end = min(p1, base + capacity);
-      for (int t = 0; t < turns || (t == 0 && base == p0); ++t) {
-        const int left = turns - 1 - t;  // groups still on their way
+      const int count = min(capacity, p1 - base), full = count / (TURN * threads);
+      const uint4* from = mine16;
+      for (int t = 0; t < full; ++t, from += TURN * threads) {
+        const int left = full - t;  // groups still on their way after this one
         if (left >= 3) copy_wait<3>();
         else if (left == 2) copy_wait<2>();
-        else if (left == 1) copy_wait<1>();
-        else copy_wait<0>();
+        else copy_wait<1>();
         uint4 raw[TURN];
 #pragma unroll
-        for (int i = 0; i < TURN; ++i) {
-          const int at = (t * TURN + i) * threads;
-          raw[i] = base + at + tid < end ? mine16[at] : nothing16<T>();
-        }
+        for (int i = 0; i < TURN; ++i) raw[i] = from[i * threads];
         if (t == 0 && base == p0) {
-          float top = edge_z;
+          float top = Vec16<T>::top(raw[0]);
 #pragma unroll
-          for (int i = 0; i < TURN; ++i) top = fmaxf(top, Vec16<T>::top(raw[i]));
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float k = rintf(top * g.c);
-          mine.k = fabsf(k) <= 0x1p20f ? (int)k : 0;
-          k2 = pair(-(float)mine.k, -(float)mine.k);
-          part[0] = pair(fast_exp2(fmaf(edge_z, g.c, -(float)mine.k)), 0.f);
+          for (int i = 1; i < TURN; ++i) top = fmaxf(top, Vec16<T>::top(raw[i]));
+          scale_from(top);
         }
 #pragma unroll
-        for (int i = 0; i < TURN; ++i) {
-          float v[E];
-          Vec16<T>::up(raw[i], v);
-#pragma unroll
-          for (int j = 0; j < E; j += 2) part[j / 2 & 1] = add2(part[j / 2 & 1], exp2_2(fma2(pair(v[j], v[j + 1]), c2, k2)));
-        }
+        for (int i = 0; i < TURN; ++i) add16(raw[i]);
       }
+      copy_wait<0>();
+      const int rest = full * TURN * threads;
+      if (full == 0 && base == p0) {
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int at = rest; at + tid < count; at += threads) top = fmaxf(top, Vec16<T>::top(mine16[at]));
+        scale_from(top);
+      }
+#pragma unroll 1
+      for (int at = rest; at + tid < count; at += threads) add16(mine16[at]);
     }
     const float2 sum = both(add2(part[0], part[1]));
     mine.s = sum.x + sum.y;
@@ -304,7 +319,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   };
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
-  if (!(mine.s >= 0x1p-40f && mine.s <= 0x1p100f)) {  // the whole warp
+  if (warp < warps && !(mine.s >= 0x1p-40f && mine.s <= 0x1p100f)) {  // the whole warp
     const Scale sc(maximum(), g.c);
     mine.k = sc.huge ? (sc.m > 0.f ? DISTILL_FAR : -DISTILL_FAR) : (int)sc.k;
     mine.s = sc.huge ? 0.f : sum_to(sc);
@@ -319,11 +334,11 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
     __syncthreads();
     if (lane == 0) warp_part[warp] = v;
     __syncthreads();
-    if (ranks == 1) return gather(warp_part, threads / 32);
+    if (ranks == 1) return gather(warp_part, warps);
     if (first) cluster_wait();  // all blocks run
     first = false;
     if (warp == 0) {
-      const Sum whole = gather(warp_part, threads / 32);
+      const Sum whole = gather(warp_part, warps);
       if (lane < ranks) put_remote(&parts[rank], lane, whole);
     }
     cluster_arrive();
@@ -335,12 +350,12 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   Scale sc(0.f, g.c);
   sc.k = (float)all.k;
   if (abs(all.k) >= DISTILL_FAR) {  // the whole cluster: once more, relative to the row's maximum
-    const float top = maximum();
+    const float top = warp < warps ? maximum() : -INFINITY;
     __syncthreads();
     if (lane == 0) warp_part[warp] = Sum{0, top};
     __syncthreads();
     float m = warp_part[0].s;
-    for (int i = 1; i < threads / 32; ++i) m = fmaxf(m, warp_part[i].s);
+    for (int i = 1; i < warps; ++i) m = fmaxf(m, warp_part[i].s);
     if (ranks > 1) {
       cluster_arrive();  // all have read the parts before
       cluster_wait();
@@ -353,14 +368,14 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
     }
     sc = Scale(m, g.c);
     sc.huge = true;
-    float sum = sum_to(sc);
+    float sum = warp < warps ? sum_to(sc) : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     all = collect(Sum{0, sum});
   }
   const bool any = s_any != 0;
   const float inv_ts = 1.f / s_ts;
-  if (rank == 0 && warp == 1) {
+  if (rank == 0 && warp == warps) {
     // sum p (log p - log q) = (sum e t - sum e arg) / ts - log ts + log s, e = 2^t unnormalised
     float cross = 0.f;
     for (int k = lane; k < g.entries; k += 32)
@@ -376,7 +391,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
     if (edge >= 0) out[edge] = Elem<T>::down(any ? fast_exp2(sc.arg(edge_z)) * scale : 0.f);
     T* out_body = out + head;
     const Pair c2 = pair(g.c, g.c), k2 = pair(-sc.k, -sc.k), w2 = pair(scale, scale);
-    for (int base = p0; base < p1; base += capacity) {
+    for (int base = warp < warps ? p0 : p1; base < p1; base += capacity) {
       const int end = min(p1, base + capacity);
       if (p1 - p0 > capacity) {  // the row is not all held
         fetch(base);
@@ -407,14 +422,14 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
     __syncthreads();
     // the entries' columns once more, from float32: the first of equal indices writes, for all of them
     if (any)
-      for (int k = tid; k < g.entries; k += threads) {
+      for (int k = tid; k < g.entries; k += blockDim.x) {
         const int i = s_i[k];
         if (i < 0) continue;
         const int piece = i < head ? -1 : (i - head) / E;  // -1 and `pieces`: the edges
         if (piece < 0 ? rank != 0 : piece >= pieces ? !last : piece < p0 || piece >= p1) continue;  // another block's column
-        float p = 0.f;
+        float p = s_twice ? 0.f : s_p[k];
         bool is_first = true;
-        for (int n = 0; n < entries4; ++n) {
+        for (int n = 0; s_twice && n < entries4; ++n) {
           const int4 four = reinterpret_cast<const int4*>(s_i)[n];
           if (four.x != i && four.y != i && four.z != i && four.w != i) continue;
           const int f[4] = {four.x, four.y, four.z, four.w};
@@ -443,7 +458,7 @@ template <typename T, bool GRAD> int distill_rows(const DistillArgs& g, cudaStre
   return (int)cudaGetLastError();
 }
 
-constexpr int DISTILL_HELD = 108 * 1024;  // bytes of a row per block: two blocks and their entries fit an SM
+constexpr int DISTILL_HELD = 104 * 1024;  // bytes of a row per block: two blocks and 256 entries fit an SM
 template <typename T, bool GRAD> int distill_wide(const DistillArgs& g, int sms, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
   const int rc = raise_smem(k_distill_wide<T, GRAD>, DISTILL_HELD + 12 * MGBS_DISTILL_MAX_ENTRIES, raised);
