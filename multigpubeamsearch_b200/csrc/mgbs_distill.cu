@@ -47,6 +47,8 @@ struct Scale {
 
 constexpr int DISTILL_THREADS = 256;
 
+// A group of `lanes` lanes has a row.  Each lane keeps its first entry in registers from the start, so that a row with no
+// more entries than lanes waits for memory once.
 template <typename T, int NPL, bool GRAD>
 __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_constant__ DistillArgs g, int lanes) {
   const int lane = threadIdx.x & (lanes - 1);
@@ -54,6 +56,10 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
   const bool live = row_any < g.rows;
   const int64_t row = live ? row_any : g.rows - 1;  // idle groups repeat the last row and write nothing
   const T* z = static_cast<const T*>(g.logits) + row * g.row_stride;
+  const float* teacher = g.teacher + row * g.teacher_stride;
+  const int i0 = lane < g.entries ? distill_index(g, row, lane) : -1;
+  const float t0 = i0 >= 0 ? teacher[lane] : -INFINITY;
+  const float w = GRAD ? (g.weight ? g.weight[row] : 1.f) * g.inv_t : 0.f;
   float v[NPL], m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
@@ -61,10 +67,13 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
     v[i] = e < g.width ? Elem<T>::up(z[e]) : -INFINITY;
     m = fmaxf(m, v[i]);
   }
-  float tm = -INFINITY;
-  int any = 0;
-  for (int k = lane; k < g.entries; k += lanes) {
-    const float t = g.teacher[row * g.teacher_stride + k];
+  const float z0 = i0 >= 0 ? Elem<T>::up(z[i0]) : 0.f;
+  auto index = [&](int k) { return k == lane ? i0 : distill_index(g, row, k); };
+  auto logit = [&](int k) { return k == lane ? t0 : teacher[k]; };
+  float tm = t0;
+  int any = t0 != -INFINITY;
+  for (int k = lane + lanes; k < g.entries; k += lanes) {
+    const float t = teacher[k];
     if (distill_index(g, row, k) >= 0 && t != -INFINITY) { any = 1; tm = fmaxf(tm, t); }
   }
   for (int o = lanes >> 1; o > 0; o >>= 1) {
@@ -80,7 +89,7 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
     s += v[i];
   }
   for (int k = lane; k < g.entries; k += lanes)
-    if (distill_index(g, row, k) >= 0) ts += fast_exp2((g.teacher[row * g.teacher_stride + k] - tm) * g.c);
+    if (index(k) >= 0) ts += fast_exp2((logit(k) - tm) * g.c);
   for (int o = lanes >> 1; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     ts += __shfl_xor_sync(0xffffffffu, ts, o);
@@ -89,17 +98,16 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
   float loss = 0.f;
   if (any)
     for (int k = lane; k < g.entries; k += lanes) {
-      const int i = distill_index(g, row, k);
+      const int i = index(k);
       if (i < 0) continue;
-      const float t = (g.teacher[row * g.teacher_stride + k] - tm) * g.c;
+      const float t = (logit(k) - tm) * g.c;
       const float p = fast_exp2(t) * inv_ts;
-      if (p != 0.f) loss += p * (t - sc.arg(Elem<T>::up(z[i])) + log_ratio);
+      if (p != 0.f) loss += p * (t - sc.arg(k == lane ? z0 : Elem<T>::up(z[i])) + log_ratio);
     }
   for (int o = lanes >> 1; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
   if (live && lane == 0) g.loss[row] = loss * kLn2;
   if (GRAD) {
     T* out = static_cast<T*>(g.grad) + row * g.grad_stride;
-    const float w = (g.weight ? g.weight[row] : 1.f) * g.inv_t;
     const float scale = any ? w / s : 0.f;
     if (live) {
 #pragma unroll
@@ -110,19 +118,21 @@ __global__ void __launch_bounds__(DISTILL_THREADS) k_distill_rows(const __grid_c
     }
     __syncwarp();
     // the entries' columns once more, from float32: the first of equal indices writes, for all of them
-    if (live && any)
-      for (int k = lane; k < g.entries; k += lanes) {
-        const int i = distill_index(g, row, k);
-        if (i < 0) continue;
-        float p = 0.f;
-        bool first = true;
-        for (int n = 0; n < g.entries; ++n)
-          if (distill_index(g, row, n) == i) {
-            first = first && n >= k;
-            p += fast_exp2((g.teacher[row * g.teacher_stride + n] - tm) * g.c);
-          }
-        if (first) out[i] = Elem<T>::down(fast_exp2(sc.arg(Elem<T>::up(z[i]))) * scale - p * inv_ts * w);
+    const int group = threadIdx.x & 31 & ~(lanes - 1);
+    for (int k = lane; k - lane < g.entries; k += lanes) {  // whole groups, for the exchange
+      const int i = k < g.entries ? index(k) : -1;
+      float p = 0.f;
+      bool first = true;
+      for (int n = 0; n < g.entries; ++n) {
+        const int other = n < lanes ? __shfl_sync(0xffffffffu, i0, group + n) : distill_index(g, row, n);
+        const float t = n < lanes ? __shfl_sync(0xffffffffu, t0, group + n) : 0.f;
+        if (other == i) {
+          first = first && n >= k;
+          p += fast_exp2(((n < lanes ? t : teacher[n]) - tm) * g.c);
+        }
       }
+      if (live && any && i >= 0 && first) out[i] = Elem<T>::down(fast_exp2(sc.arg(k == lane ? z0 : Elem<T>::up(z[i]))) * scale - p * inv_ts * w);
+    }
   }
 }
 
