@@ -626,6 +626,7 @@ typedef struct MgbsRelAttentionArgs {
   void* dv;
   void* dtable;      /* [num_buckets, heads] */
   void* workspace;   /* mgbs_rel_attention_backward_workspace() bytes, 16-byte aligned */
+  int32_t* error;    /* device word or null: receives the code of the first bounded wait that gave up (the rows concerned are NaN) */
 } MgbsRelAttentionArgs;
 int mgbs_sizeof_rel_attention_args(void);
 int mgbs_rel_attention(const MgbsRelAttentionArgs* args, void* stream);

@@ -19,19 +19,9 @@
 
 #include "mgbs_operators.cuh"
 #include "mgbs_counted.cuh"
+#include "mgbs_rel_attention.cuh"
 
 namespace mgbs {
-
-struct RelArgs {
-  const void* q; const void* k; const void* v; const void* table; const void* dout;
-  const int32_t* map; const int32_t* order; const int32_t* start; const int32_t* lengths;
-  void* out; void* dq; void* dk; void* dv;
-  float2* stats; float* delta; float* partial;
-  int64_t qs[3], ks[3], vs[3], ds[3];
-  const uint32_t* count_dev; int64_t count_offset;
-  int32_t batch, tokens, heads, heads_kv, buckets, reach, causal;  // reach: max_distance
-  float scale, sl2;  // sl2: scale * log2(e)
-};
 
 constexpr int REL_THREADS = 128;
 #ifndef REL_FWD_BLOCKS
@@ -40,29 +30,8 @@ constexpr int REL_THREADS = 128;
 #ifndef REL_BWD_BLOCKS
 #define REL_BWD_BLOCKS 3
 #endif
-constexpr float REL_BIG = 3.0e38f;
 // rows of the short form's matrices are padded by 16 bytes: eight rows then start in distinct banks
 template <int D> struct RelTile { static constexpr int PITCH = D + 8; };
-
-__device__ __forceinline__ int rel_batch(const RelArgs& g) {
-  if (!g.count_dev) return g.batch;
-  const int64_t left = (int64_t)*g.count_dev - g.count_offset;
-  return (int)(left < 0 ? 0 : (left < g.batch ? left : g.batch));
-}
-__device__ __forceinline__ int rel_length(const RelArgs& g, int b) {
-  return g.lengths ? min(max(__ldg(g.lengths + b), 0), g.tokens) : g.tokens;
-}
-__device__ __forceinline__ int rel_bucket(const RelArgs& g, int off) {
-  const int at = min(max(off, -g.reach), g.reach) + g.reach;
-  return min(max(__ldg(g.map + at), 0), g.buckets - 1);
-}
-template <typename T> __device__ __forceinline__ float rel_bias(const RelArgs& g, int off, int h) {
-  return Elem<T>::up(static_cast<const T*>(g.table)[(int64_t)rel_bucket(g, off) * g.heads + h]);
-}
-// x * f where finite values stay finite (the type's lowest value is a usual mask and must not become -inf)
-__device__ __forceinline__ float scaled_bias(float x, float f, float most) {
-  return isinf(x) ? x : fminf(fmaxf(x * f, -most), most);
-}
 
 // lane addresses inside a 16 x 16 block for ldmatrix (elements)
 template <int PITCH> __device__ __forceinline__ int frag_a(int lane) { return ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 8; }
@@ -518,17 +487,9 @@ __global__ void __launch_bounds__(Groups<STRIPS>::THREADS, REL_BWD_BLOCKS) k_rel
 // ------------------------------------------------------------------------------------------------------------------
 
 constexpr int TILE = 64;
-constexpr int REL_RIM = 128;  // offsets inside a tile that is not beyond the reach stay below reach + REL_RIM
-
-template <int D> __host__ __device__ constexpr int tile_bytes() { return TILE * RelTile<D>::PITCH * 2; }
+constexpr int REL_RIM = 2 * TILE;
 inline int rel_bias_floats(int reach) { return 2 * (reach + REL_RIM) + 1; }
-
-// bias * log2(e) by offset: bt[off + reach + REL_RIM]
-template <typename T> __device__ __forceinline__ void fill_bias(const RelArgs& g, int h, float* bt) {
-  const int side = g.reach + REL_RIM;
-  for (int i = threadIdx.x; i < 2 * side + 1; i += REL_THREADS) bt[i] = scaled_bias(rel_bias<T>(g, i - side, h), kLog2e, REL_BIG);
-}
-
+template <int D> __host__ __device__ constexpr int tile_bytes() { return TILE * RelTile<D>::PITCH * 2; }
 // 64 rows from `row` on of one head; rows from `len` on become zeros
 template <typename T, int D> __device__ __forceinline__ void stage_tile(uint32_t dst, const T* head, int64_t token_stride, int row, int len) {
   constexpr int PITCH = RelTile<D>::PITCH, PARTS = D / 8;
@@ -538,12 +499,6 @@ template <typename T, int D> __device__ __forceinline__ void stage_tile(uint32_t
     const bool in = row + t < len;
     copy16(dst + (t * PITCH + part * 8) * 2, head + (in ? (row + t) * token_stride + part * 8 : 0), in ? 16u : 0u);
   }
-}
-
-struct Where { int tile, head, b; };
-__device__ __forceinline__ Where rel_where(int tiles, int heads) {
-  const int64_t n = blockIdx.x;
-  return {(int)(n % tiles), (int)(n / tiles % heads), (int)(n / tiles / heads)};
 }
 
 // Keys of tile j0 against rows of tile i0: 1 = all at least `reach` after, -1 = all at least `reach` before, else 0.
@@ -588,7 +543,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles(const __grid_constant
   stage_tile<T, D>(q_at, q, g.qs[1], i0, len);
   load(0);
   copy_commit();
-  fill_bias<T>(g, w.head, bt);
+  fill_bias<T>(g, w.head, bt, g.reach + REL_RIM, threadIdx.x, REL_THREADS);
   const int side = g.reach + REL_RIM;
   uint32_t qa[D / 16][4];
   float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
@@ -720,7 +675,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_const
   stage_tile<T, D>(do_at, dout, g.ds[1], i0, len);
   load(0);
   copy_commit();
-  fill_bias<T>(g, w.head, bt);
+  fill_bias<T>(g, w.head, bt, g.reach + REL_RIM, threadIdx.x, REL_THREADS);
   for (int i = threadIdx.x; i < span; i += REL_THREADS) dacc[i] = 0.f;
   const bool in0 = row0 < len, in1 = row0 + 8 < len;
   const float2* stats = g.stats + ((int64_t)w.b * g.heads + w.head) * g.tokens;
@@ -905,7 +860,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dkv(const __grid_cons
     const int i0 = (first + n % n_tiles) * TILE;
     if (n % n_tiles == 0) {
       __syncthreads();  // the head before has read its biases
-      fill_bias<T>(g, w.head * share + n / n_tiles, bt);
+      fill_bias<T>(g, w.head * share + n / n_tiles, bt, g.reach + REL_RIM, threadIdx.x, REL_THREADS);
     }
     copy_wait<0>();
     __syncthreads();
@@ -1081,9 +1036,18 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, f
   return rc ? rc : finish_table<T>(g, sums, REL_CHUNKS, REL_CHUNKS, 1, dtable, st);
 }
 
+#ifndef REL_TC
+#define REL_TC 128
+#endif
+template <typename T> struct Type;
+template <> struct Type<__nv_bfloat16> { static constexpr int DT = MGBS_DT_BF16; };
+template <> struct Type<__half> { static constexpr int DT = MGBS_DT_F16; };
 template <typename T, int D> int forward_as(const RelArgs& g, cudaStream_t st) {
   // with statistics asked for, the form whose backward reads them
-  if (g.tokens > REL_SHORT || (g.stats && g.heads != g.heads_kv)) return run_tiles<T, D>(g, st);
+  if (g.tokens > REL_SHORT || (g.stats && g.heads != g.heads_kv)) {
+    if (g.tokens > REL_TC) return rel_attention_tc(g, Type<T>::DT, D, st);
+    return run_tiles<T, D>(g, st);
+  }
   const int strips = short_strips(g.tokens);
   return strips == 1 ? run_short<T, D, 1>(g, st) : strips == 2 ? run_short<T, D, 2>(g, st) : strips == 3 ? run_short<T, D, 3>(g, st) : run_short<T, D, 4>(g, st);
 }
@@ -1123,6 +1087,7 @@ int rel_prepare(const MgbsRelAttentionArgs* a, RelArgs* g) {
   for (int i = 0; i < 3; ++i) { g->qs[i] = a->q_stride[i]; g->ks[i] = a->k_stride[i]; g->vs[i] = a->v_stride[i]; }
   g->batch = (int32_t)a->batch; g->tokens = (int32_t)a->tokens; g->heads = a->heads; g->heads_kv = a->heads_kv;
   g->buckets = a->num_buckets; g->reach = a->max_distance; g->causal = a->causal != 0;
+  g->error = a->error;
   g->scale = a->scale;
   g->sl2 = a->scale * kLog2e;
   return 0;

@@ -1,0 +1,55 @@
+// What the forms of the attention with a relative bias share: the kernels' argument block, lengths, buckets, biases.
+#pragma once
+#include "mgbs_operators.cuh"
+
+namespace mgbs {
+
+struct RelArgs {
+  const void* q; const void* k; const void* v; const void* table; const void* dout;
+  const int32_t* map; const int32_t* order; const int32_t* start; const int32_t* lengths;
+  void* out; void* dq; void* dk; void* dv;
+  float2* stats; float* delta; float* partial;
+  int64_t qs[3], ks[3], vs[3], ds[3];
+  const uint32_t* count_dev; int64_t count_offset;
+  int* error;  // or null: first code of a bounded wait that gave up
+  int32_t batch, tokens, heads, heads_kv, buckets, reach, causal;  // reach: max_distance
+  float scale, sl2;  // sl2: scale * log2(e)
+};
+
+constexpr float REL_BIG = 3.0e38f;
+__device__ __forceinline__ int rel_batch(const RelArgs& g) {
+  if (!g.count_dev) return g.batch;
+  const int64_t left = (int64_t)*g.count_dev - g.count_offset;
+  return (int)(left < 0 ? 0 : (left < g.batch ? left : g.batch));
+}
+__device__ __forceinline__ int rel_length(const RelArgs& g, int b) {
+  return g.lengths ? min(max(__ldg(g.lengths + b), 0), g.tokens) : g.tokens;
+}
+__device__ __forceinline__ int rel_bucket(const RelArgs& g, int off) {
+  const int at = min(max(off, -g.reach), g.reach) + g.reach;
+  return min(max(__ldg(g.map + at), 0), g.buckets - 1);
+}
+template <typename T> __device__ __forceinline__ float rel_bias(const RelArgs& g, int off, int h) {
+  return Elem<T>::up(static_cast<const T*>(g.table)[(int64_t)rel_bucket(g, off) * g.heads + h]);
+}
+// x * f where finite values stay finite (the type's lowest value is a usual mask and must not become -inf)
+__device__ __forceinline__ float scaled_bias(float x, float f, float most) {
+  return isinf(x) ? x : fminf(fmaxf(x * f, -most), most);
+}
+
+// bias * log2(e) by offset: bt[off + side] for offsets of at most `side`, by `threads` threads.  A tile of n x n that is not
+// beyond the reach has offsets below reach + 2 n.
+template <typename T> __device__ __forceinline__ void fill_bias(const RelArgs& g, int h, float* bt, int side, int thread, int threads) {
+  for (int i = thread; i < 2 * side + 1; i += threads) bt[i] = scaled_bias(rel_bias<T>(g, i - side, h), kLog2e, REL_BIG);
+}
+
+struct Where { int tile, head, b; };
+__device__ __forceinline__ Where rel_where(int tiles, int heads) {
+  const int64_t n = blockIdx.x;
+  return {(int)(n % tiles), (int)(n / tiles % heads), (int)(n / tiles / heads)};
+}
+
+// The forward over tiles of 128 x 128 on the fifth-generation tensor cores (tokens > 64).
+int rel_attention_tc(const RelArgs& g, int dtype, int head_dim, cudaStream_t st);
+
+}  // namespace mgbs

@@ -46,7 +46,7 @@ class MgbsRelAttentionArgs(C.Structure):
         ("q", _P), ("k", _P), ("v", _P), ("table", _P), ("bucket_map", _P), ("bucket_order", _P), ("bucket_start", _P),
         ("lengths", _P), ("out", _P), ("stats", _P),
         ("num_buckets", _I32), ("max_distance", _I32), ("causal", _I32), ("scale", C.c_float),
-        ("dout", _P), ("dq", _P), ("dk", _P), ("dv", _P), ("dtable", _P), ("workspace", _P),
+        ("dout", _P), ("dq", _P), ("dk", _P), ("dv", _P), ("dtable", _P), ("workspace", _P), ("error", _P),
     ]
 
 
