@@ -1045,7 +1045,7 @@ template <> struct Type<__half> { static constexpr int DT = MGBS_DT_F16; };
 template <typename T, int D> int forward_as(const RelArgs& g, cudaStream_t st) {
   // with statistics asked for, the form whose backward reads them
   if (g.tokens > REL_SHORT || (g.stats && g.heads != g.heads_kv)) {
-    if (g.tokens > REL_TC) return rel_attention_tc(g, Type<T>::DT, D, st);
+    if (g.tokens > REL_TC && rel_attention_tc_fits(g)) return rel_attention_tc(g, Type<T>::DT, D, st);
     return run_tiles<T, D>(g, st);
   }
   const int strips = short_strips(g.tokens);

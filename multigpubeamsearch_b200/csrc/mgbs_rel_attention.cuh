@@ -49,7 +49,8 @@ __device__ __forceinline__ Where rel_where(int tiles, int heads) {
   return {(int)(n % tiles), (int)(n / tiles % heads), (int)(n / tiles / heads)};
 }
 
-// The forward over tiles of 128 x 128 on the fifth-generation tensor cores (tokens > 64).
+// The forward on the fifth-generation tensor cores, and whether TMA can describe the strides (it knows no stride of 0).
+bool rel_attention_tc_fits(const RelArgs& g);
 int rel_attention_tc(const RelArgs& g, int dtype, int head_dim, cudaStream_t st);
 
 }  // namespace mgbs

@@ -1,19 +1,19 @@
-// Forward attention with a relative bias over tiles of 128 queries x 128 keys on tcgen05.  Per block (128 queries of one
-// head): four softmax warps (a thread owns a query row), four loading warps, one warp that issues the products.
+// Forward attention with a relative bias over tiles of 128 queries x 64 keys on tcgen05.  Per block (128 queries of one
+// head): four softmax warps (a thread owns a query row), one warp that issues the products, one that loads by TMA.
 //
-//   S(t) = Q K(t)^T into tensor memory (128 columns); the softmax warps read it, take the row maximum, write
-//   P(t) = 2^(s - m) as 16-bit pairs into tensor memory (64 columns), from where it is the A operand of O += P(t) V(t).
-//   S(t + 1) is issued before O += P(t) V(t), so that the exponentials of the next tile do not wait for it.
+//   S(t) = Q K(t)^T into tensor memory (two buffers of 64 columns); the softmax warps read it and write
+//   P(t) = 2^(s - m) as 16-bit pairs into tensor memory (two buffers of 32 columns), from where it is the A operand of
+//   O += P(t) V(t).  With two buffers of each, the scores of the next tile are there when a tile's softmax ends.
 //
-// The reference m of a row follows its maximum only when that has grown by more than 2^8 (P then stays within both
-// 16-bit types), so that the accumulator O, which sits in tensor memory too, is rarely rescaled.  256 of the 512 columns
-// and 80 KB: two blocks per SM, one's exponentials over the other's products and waits.  What bounds it: the
-// exponentials, 128 x 128 of them per tile at 16 a clock against 512 clocks of products.
+// The reference m of a row is its maximum over the first tile.  It follows only when a later tile's sum of P exceeds 2^14
+// (up to there P fits both 16-bit types, and float32 sums lose nothing): then the tile is done again from its true
+// maximum and the accumulator O, in tensor memory too, is rescaled.  So a tile takes no maximum as a rule.
+// 256 of the 512 columns and 84 KB: two blocks per SM, one's exponentials over the other's products and waits.  What
+// bounds it: the exponentials, 128 x 64 of them per tile at 16 a clock against 256 clocks of products.
 //
-// Operands lie in shared memory in the layout without swizzle, 16-byte pieces of 8 rows side by side (128 bytes): the
-// same bytes are K-major rows for Q and K and MN-major rows for V, copied asynchronously with zeros for what lies past
-// the length (padding is never read, and P = 0 must not meet a NaN).  Every wait is bounded: a block that gives up
-// writes NaN and the error word.
+// Rows of 128 bytes (64 for heads of 32) in the swizzled layout of that width: K-major for Q and K, MN-major for V.
+// Padding past a length is zeroed in V's last tile (P = 0 must not meet a NaN there); elsewhere it only reaches scores
+// that are hidden.  Every wait is bounded: a block that gives up writes NaN and the error word.
 
 #include <math.h>
 
@@ -22,27 +22,32 @@
 
 namespace mgbs {
 
-constexpr int TC_TILE = 128;
-constexpr int TC_THREADS = 288;
-constexpr int TC_RIM = 2 * TC_TILE;
-constexpr int TC_GROUP = 128;                       // bytes of 8 rows x 16 bytes
-constexpr int TC_CHUNK = TC_TILE / 8 * TC_GROUP;    // bytes between a row's 16-byte pieces
-constexpr float TC_GROWTH = 8.f;                    // log2 of how far P may exceed 1
+constexpr int TC_Q = 128, TC_K = 64;                // rows of a block, keys of a tile
+constexpr int TC_THREADS = 192;
+constexpr int TC_STAGES = 4;                        // tiles of K and of V in shared memory
+constexpr int TC_RIM = 256;                         // a tile that is not beyond the reach has offsets below reach + 2 * TC_Q
+constexpr float TC_GROWTH = 16384.f;                // how far a row's sum over a tile may grow before its reference follows
+constexpr int TC_P_COL = 128, TC_O_COL = 192;       // columns: S at 0 and 64, P at 128 and 160, O at 192
 constexpr int ERR_TC_LOAD = 21, ERR_TC_FREE = 22, ERR_TC_S = 23, ERR_TC_P = 24, ERR_TC_O = 25;
 
-template <int D> struct TcShape {
-  static constexpr int MAT = D / 8 * TC_CHUNK;  // bytes of one 128-row operand
-  static constexpr int P_COL = 128, O_COL = 192;
-};
-
-// Matrix descriptor without swizzle: start, leading and stride byte offsets in 16-byte units, version 1.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) | (1ull << 46);
+// Matrix descriptor of rows of D 16-bit elements, swizzled in their own width: groups of 8 rows D * 16 bytes apart.  The
+// same for K-major (rows are M or N) and MN-major operands (rows are K): the leading offset is unused in both, as a row is
+// one swizzle atom wide.  Version 1; layout 128-byte swizzle = 2, 64-byte swizzle = 4.
+template <int D> __device__ __forceinline__ uint64_t tc_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | (1ull << 16) | ((uint64_t)(D * 16 >> 4) << 32) | (1ull << 46) | ((D == 64 ? 2ull : 4ull) << 61);
 }
-// kind::f16 instruction descriptor: float32 accumulators; operand type (f16 0, bf16 1); B MN-major; N; M = 128
+template <typename T> struct TcType { static constexpr uint32_t FORMAT = 1; };
+template <> struct TcType<__half> { static constexpr uint32_t FORMAT = 0; };
+// kind::f16 instruction descriptor: float32 accumulators; operand types; B MN-major or not; N; M = 128
 template <typename T> __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
-  return (1u << 4) | ((sizeof(T) == 2 && !__is_same(T, __half) ? 1u : 0u) << 7) | ((!__is_same(T, __half) ? 1u : 0u) << 10) |
-         ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TC_TILE >> 4) << 24);
+  return (1u << 4) | (TcType<T>::FORMAT << 7) | (TcType<T>::FORMAT << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(TC_Q >> 4) << 24);
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int row, int head, int batch, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(head), "r"(batch), "r"(bar)
+      : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -90,37 +95,96 @@ static __device__ __noinline__ bool tc_wait_slow(uint32_t bar, uint32_t parity, 
   return false;
 }
 
-// 128 rows from `row` on into the operand layout, by four warps; rows from `len` on become zeros.  A warp's instruction
-// takes 8 rows x 4 pieces: whole 64-byte runs of global memory, and 128-byte runs of shared memory.
-template <typename T, int D> __device__ __forceinline__ void tc_stage(uint32_t dst, const T* head, int64_t token_stride, int row, int len, int warp, int lane) {
-  const int in_group = lane & 7, piece = lane >> 3;
+// A tile as a softmax thread sees it.
+struct TcTile {
+  int far;  // 1 / -1: all keys beyond the reach after / before the queries, so that one bias serves
+  bool edge;
+  int j0, row, len, causal;
+  float fixed;
+  const float* by_offset;  // bias of key j0 + j at [j]
+};
+
+// Scores of 32 keys, scaled and biased.  MODE 0: one bias; 1: by offset; 2: either, and hidden ones at -inf.
+template <int MODE> __device__ __forceinline__ void tc_scores(const TcTile& w, int c, Pair sl2, const uint32_t (&raw)[32], Pair (&s)[16]) {
+  const Pair one = pair(w.fixed, w.fixed);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int group = warp * 4 + g, t = row + group * 8 + in_group;
-    const bool in = t < len;
-    const T* src = head + (in ? t * token_stride : 0) + piece * 8;
-    const uint32_t to = dst + group * TC_GROUP + in_group * 16 + piece * TC_CHUNK;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) copy16(to + c * 4 * TC_CHUNK, src + c * 32, in ? 16u : 0u);
+  for (int j = 0; j < 32; j += 2) {
+    const int at = c * 32 + j;
+    const bool fix = MODE == 0 || (MODE == 2 && w.far);
+    const Pair b = fix ? one : pair(w.by_offset[at], w.by_offset[at + 1]);
+    s[j / 2] = fma2(pair(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), sl2, b);
+    if (MODE == 2) {
+      const int key = w.j0 + at;
+      float2 f = both(s[j / 2]);
+      if (key >= w.len || (w.causal && key > w.row)) f.x = -INFINITY;
+      if (key + 1 >= w.len || (w.causal && key + 1 > w.row)) f.y = -INFINITY;
+      s[j / 2] = pair(f.x, f.y);
+    }
   }
 }
 
+// A row's exact maximum over the tile.
+static __device__ __noinline__ float tc_maximum(uint32_t scores, const TcTile& w, Pair sl2) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < TC_K / 32; ++c) {
+    uint32_t raw[32];
+    Pair s[16];
+    tc_ld32(scores + c * 32, raw);
+    tc_wait_ld();
+    tc_scores<2>(w, c, sl2, raw, s);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 f = both(s[j]);
+      top = fmaxf(top, fmaxf(f.x, f.y));
+    }
+  }
+  return top;
+}
+
+// P of the tile relative to `base` into tensor memory; returns the row's sum.
+template <typename T, int MODE> __device__ __forceinline__ float tc_write_p(uint32_t scores, uint32_t to, const TcTile& w, Pair sl2, float base) {
+  const Pair minus = pair(-base, -base);
+  Pair sum = pair(0.f, 0.f);
+  uint32_t raw[2][32];
+  tc_ld32(scores, raw[0]);
+  tc_ld32(scores + 32, raw[1]);
+  tc_wait_ld();
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    Pair s[16];
+    tc_scores<MODE>(w, c, sl2, raw[c], s);
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const Pair e = exp2_2(add2(s[j], minus));
+      sum = add2(sum, e);
+      const float2 f = both(e);
+      p[j] = pack2<T>(f.x, f.y);
+    }
+    tc_st16(to + c * 16, p);
+  }
+  const float2 f = both(sum);
+  return f.x + f.y;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant__ RelArgs g, int tiles) {
-  using Shape = TcShape<D>;
-  extern __shared__ __align__(128) uint8_t tc_smem[];
-  __shared__ __align__(8) uint64_t bars[7];
+__global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RelArgs g, int tiles) {
+  constexpr int Q_BYTES = TC_Q * D * 2, K_BYTES = TC_K * D * 2;
+  extern __shared__ __align__(1024) uint8_t tc_smem[];
+  __shared__ __align__(8) uint64_t bars[4 * TC_STAGES + 8];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   const Where w0 = rel_where(tiles, g.heads);
   const int tile = tiles - 1 - w0.tile, head = w0.head, batch = w0.b;  // under a causal mask the longest rows start first
   if (batch >= rel_batch(g)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = rel_length(g, batch), i0 = tile * TC_TILE;
+  const int len = rel_length(g, batch), i0 = tile * TC_Q;
   T* out = static_cast<T*>(g.out) + ((int64_t)batch * g.tokens * g.heads + head) * D;
   float2* stats = g.stats ? g.stats + ((int64_t)batch * g.heads + head) * g.tokens : nullptr;
   if (i0 >= len) {
-    for (int r = threadIdx.x; r < TC_TILE && i0 + r < g.tokens; r += TC_THREADS) {
+    for (int r = threadIdx.x; r < TC_Q && i0 + r < g.tokens; r += TC_THREADS) {
       uint4* to = reinterpret_cast<uint4*>(out + (int64_t)(i0 + r) * g.heads * D);
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) to[c] = make_uint4(0u, 0u, 0u, 0u);
@@ -128,18 +192,25 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
     }
     return;
   }
-  const uint32_t q_at = smem_u32(tc_smem), kv_at = q_at + Shape::MAT;
-  float* bt = reinterpret_cast<float*>(tc_smem + 5 * Shape::MAT);
+  const uint32_t q_at = (smem_u32(tc_smem) + 1023u) & ~1023u, k_at = q_at + Q_BYTES, v_at = k_at + TC_STAGES * K_BYTES;
+  uint8_t* v_ptr = tc_smem + (v_at - smem_u32(tc_smem));
+  float* bt = reinterpret_cast<float*>(v_ptr + TC_STAGES * K_BYTES);
   const uint32_t bar = smem_u32(bars);
-  const uint32_t full = bar, empty = bar + 16, s_full = bar + 32, p_full = bar + 40, o_done = bar + 48;
+  const uint32_t k_full = bar, v_full = bar + 8 * TC_STAGES, k_free = bar + 16 * TC_STAGES, v_free = bar + 24 * TC_STAGES;
+  const uint32_t s_full = bar + 32 * TC_STAGES, p_full = s_full + 16, o_done = s_full + 32, q_full = s_full + 48, v_fixed = s_full + 56;
   if (threadIdx.x == 0) {
-    mbar_init(full, 128); mbar_init(full + 8, 128);
-    mbar_init(empty, 1); mbar_init(empty + 8, 1);
-    mbar_init(s_full, 1); mbar_init(p_full, 128); mbar_init(o_done, 1);
+    for (int i = 0; i < 4 * TC_STAGES; ++i) mbar_init(bar + i * 8, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i * 8, 1);
+      mbar_init(p_full + i * 8, 128);
+      mbar_init(o_done + i * 8, 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(v_fixed, 1);
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 4) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(256u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -153,63 +224,66 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int last = g.causal ? min(len, i0 + TC_TILE) : len, n_tiles = (last + TC_TILE - 1) / TC_TILE;
+  const int last = g.causal ? min(len, i0 + TC_Q) : len, n_tiles = (last + TC_K - 1) / TC_K;
+  // rows between the length and the tensor's end are padding that the last tile of V holds: zeroed before it is used
+  const bool fix_v = len < g.tokens && n_tiles * TC_K > len;
 
-  if (warp >= 4 && warp < 8) {
+  if (warp == 5) {
     const int head_kv = head / (g.heads / g.heads_kv);
-    const T* q = static_cast<const T*>(g.q) + batch * g.qs[0] + head * g.qs[2];
-    const T* k = static_cast<const T*>(g.k) + batch * g.ks[0] + head_kv * g.ks[2];
-    const T* v = static_cast<const T*>(g.v) + batch * g.vs[0] + head_kv * g.vs[2];
-    tc_stage<T, D>(q_at, q, g.qs[1], i0, len, warp - 4, lane);
-    auto load = [&](int t) {
-      const uint32_t to = kv_at + (t & 1) * 2 * Shape::MAT;
-      tc_stage<T, D>(to, k, g.ks[1], t * TC_TILE, len, warp - 4, lane);
-      tc_stage<T, D>(to + Shape::MAT, v, g.vs[1], t * TC_TILE, len, warp - 4, lane);
-      copy_commit();
-    };
-    load(0);
-    if (n_tiles > 1) load(1);
-    for (int t = 0; t < n_tiles; ++t) {
-      if (t == 0 && n_tiles > 1) copy_wait<1>();
-      else copy_wait<0>();
-      async_fence();
-      mbar_arrive(full + (t & 1) * 8);
-      // tile t has to be announced before tile t - 1 is waited for: its scores go before the product that frees t - 1
-      if (t > 0 && t + 1 < n_tiles) {
-        if (!wait(empty + ((t - 1) & 1) * 8, ((t - 1) / 2) & 1, ERR_TC_FREE)) break;
-        load(t + 1);
+    bool ok = true;
+    if (lane == 0) {
+      mbar_expect_tx(q_full, Q_BYTES);
+      tma_load_4d(q_at, &map_q, i0, head, batch, q_full);
+      for (int t = 0; t < n_tiles; ++t) {
+        const int s = t % TC_STAGES, turn = t / TC_STAGES;
+        if (turn > 0 && !(ok = wait(k_free + s * 8, (turn - 1) & 1, ERR_TC_FREE))) break;
+        mbar_expect_tx(k_full + s * 8, K_BYTES);
+        tma_load_4d(k_at + s * K_BYTES, &map_k, t * TC_K, head_kv, batch, k_full + s * 8);
+        if (turn > 0 && !(ok = wait(v_free + s * 8, (turn - 1) & 1, ERR_TC_FREE))) break;
+        mbar_expect_tx(v_full + s * 8, K_BYTES);
+        tma_load_4d(v_at + s * K_BYTES, &map_v, t * TC_K, head_kv, batch, v_full + s * 8);
       }
     }
-    copy_wait<0>();
-  } else if (warp == 8) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = tc_idesc<T>(TC_TILE, false), id_o = tc_idesc<T>(D, true);
-      const uint64_t q_desc = tc_desc(q_at, TC_CHUNK, TC_GROUP);
-      auto score = [&](int t) {
-        const uint64_t k_desc = tc_desc(kv_at + (t & 1) * 2 * Shape::MAT, TC_CHUNK, TC_GROUP);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_f16(tmem, q_desc + kk * (2 * TC_CHUNK >> 4), k_desc + kk * (2 * TC_CHUNK >> 4), id_s, kk > 0);
-        tc_commit(s_full);
-      };
-      bool ok = wait(full, 0, ERR_TC_LOAD);
-      if (ok) {
-        tc_fence_after();
-        score(0);
+    ok = __all_sync(0xffffffffu, ok);
+    if (fix_v && ok) {
+      const int t = n_tiles - 1, s = t % TC_STAGES;
+      ok = wait(v_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD);
+      if (__all_sync(0xffffffffu, ok)) {
+        for (int c = (len - t * TC_K) * (D / 8) + lane; c < TC_K * (D / 8); c += 32) reinterpret_cast<uint4*>(v_ptr + s * K_BYTES)[c] = make_uint4(0u, 0u, 0u, 0u);
+        async_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_fixed);
       }
+    }
+  } else if (warp == 4) {
+    if (lane == 0) {
+      constexpr uint32_t id_s = tc_idesc<T>(TC_K, false), id_o = tc_idesc<T>(D, true);
+      const uint64_t q_desc = tc_desc<D>(q_at);
+      auto score = [&](int t) {
+        const int s = t % TC_STAGES;
+        if (!wait(k_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD)) return false;
+        tc_fence_after();
+        const uint64_t k_desc = tc_desc<D>(k_at + s * K_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) tc_mma_f16(tmem + (t & 1) * TC_K, q_desc + kk * 2, k_desc + kk * 2, id_s, kk > 0);
+        tc_commit(k_free + s * 8);
+        tc_commit(s_full + (t & 1) * 8);
+        return true;
+      };
+      bool ok = wait(q_full, 0, ERR_TC_LOAD) && score(0) && (n_tiles < 2 || score(1));
       for (int t = 0; ok && t < n_tiles; ++t) {
-        if (t + 1 < n_tiles) ok = wait(full + ((t + 1) & 1) * 8, ((t + 1) / 2) & 1, ERR_TC_LOAD);
-        ok = ok && wait(p_full, t & 1, ERR_TC_P);
+        const int s = t % TC_STAGES;
+        ok = wait(p_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_P) && wait(v_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD) &&
+             (!fix_v || t + 1 < n_tiles || wait(v_fixed, 0, ERR_TC_LOAD));
         if (!ok) break;
         tc_fence_after();
-        if (t + 1 < n_tiles) score(t + 1);
-        // V: 8 keys of 16 bytes per group, groups of keys TC_GROUP apart, pieces of the head TC_CHUNK apart
-        const uint64_t v_desc = tc_desc(kv_at + (t & 1) * 2 * Shape::MAT + Shape::MAT, TC_GROUP, TC_CHUNK);
+        const uint64_t v_desc = tc_desc<D>(v_at + s * K_BYTES);
 #pragma unroll
-        for (int kk = 0; kk < TC_TILE / 16; ++kk)
-          tc_mma_ts(tmem + Shape::O_COL, tmem + Shape::P_COL + kk * 8, v_desc + kk * (2 * TC_GROUP >> 4), id_o, t > 0 || kk > 0);
-        tc_commit(empty + (t & 1) * 8);
-        tc_commit(o_done);
+        for (int kk = 0; kk < TC_K / 16; ++kk)
+          tc_mma_ts(tmem + TC_O_COL, tmem + TC_P_COL + (t & 1) * 32 + kk * 8, v_desc + kk * (16 * D * 2 >> 4), id_o, t > 0 || kk > 0);
+        tc_commit(v_free + s * 8);
+        tc_commit(o_done + (t & 1) * 8);
+        if (t + 2 < n_tiles) ok = score(t + 2);  // into the buffer that this tile's softmax has left
       }
     }
     __syncwarp();
@@ -220,102 +294,59 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
     const Pair sl2 = pair(g.sl2, g.sl2);
     bool ok = true;
     for (int t = 0; t < n_tiles; ++t) {
-      ok = wait(s_full, t & 1, ERR_TC_S);
+      const int j0 = t * TC_K;
+      const int far = j0 - (i0 + TC_Q - 1) >= g.reach ? 1 : i0 - (j0 + TC_K - 1) >= g.reach ? -1 : 0;
+      const bool edge = j0 + TC_K > len || (g.causal && j0 + TC_K > i0 + 1);
+      const TcTile where{far, edge, j0, row, len, g.causal, far > 0 ? bt[2 * side] : bt[0], bt + j0 - row + side};
+      const uint32_t scores = mine + (t & 1) * TC_K, to = mine + TC_P_COL + (t & 1) * 32;
+      ok = wait(s_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_S) && (t < 2 || wait(o_done + (t & 1) * 8, (t / 2 - 1) & 1, ERR_TC_O));
       if (!ok) break;
       tc_fence_after();
-      const int j0 = t * TC_TILE;
-      const int far = j0 - (i0 + TC_TILE - 1) >= g.reach ? 1 : i0 - (j0 + TC_TILE - 1) >= g.reach ? -1 : 0;
-      const bool edge = j0 + TC_TILE > len || i0 + TC_TILE > len || (g.causal && j0 + TC_TILE > i0 + 1);
-      const float fixed = far > 0 ? bt[2 * side] : bt[0];
-      const float* by_offset = bt + j0 - row + side;
-      // scores of 32 keys, scaled and biased, hidden ones at -inf
-      auto scores = [&](int c, float (&s)[32]) {
-        uint32_t raw[32];
-        tc_ld32(mine + c * 32, raw);
-        tc_wait_ld();
-        if (far) {
-          const Pair b2 = pair(fixed, fixed);
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 f = both(fma2(pair(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), sl2, b2));
-            s[j] = f.x; s[j + 1] = f.y;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 f = both(fma2(pair(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), sl2, pair(by_offset[c * 32 + j], by_offset[c * 32 + j + 1])));
-            s[j] = f.x; s[j + 1] = f.y;
-          }
-        }
-        if (edge) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int key = j0 + c * 32 + j;
-            if (key >= len || row >= len || (g.causal && key > row)) s[j] = -INFINITY;
-          }
-        }
-      };
-      float top = -INFINITY;
+      float sum;
+      for (bool again = t == 0;;) {
+        if (again) {
+          const float top = fmaxf(m, tc_maximum(scores, where, sl2));
+          if (t > 0) {
+            ok = wait(o_done + ((t - 1) & 1) * 8, ((t - 1) / 2) & 1, ERR_TC_O);  // O is still
+            if (!ok) break;
+            tc_fence_after();
+            const float f = top == -INFINITY ? 1.f : fast_exp2(m - top);
+            l *= f;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        scores(c, s);
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t raw[32];
+              tc_ld32(mine + TC_O_COL + c * 32, raw);
+              tc_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) top = fmaxf(top, s[j]);
-      }
-      if (t > 0) {
-        ok = wait(o_done, (t - 1) & 1, ERR_TC_O);
-        if (!ok) break;
-        tc_fence_after();
-      }
-      if (t == 0) m = top;
-      else if (__any_sync(0xffffffffu, top > m + TC_GROWTH)) {
-        const float to = top > m + TC_GROWTH ? top : m;
-        const float f = to == -INFINITY ? 1.f : fast_exp2(m - to);
-        m = to;
-        l *= f;
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t raw[32];
-          tc_ld32(mine + Shape::O_COL + c * 32, raw);
-          tc_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
-          tc_st32(mine + Shape::O_COL + c * 32, raw);
+              for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
+              tc_st32(mine + TC_O_COL + c * 32, raw);
+            }
+          }
+          m = top;
         }
+        const float base = m == -INFINITY ? 0.f : m;  // no key yet: all terms 0
+        sum = edge ? tc_write_p<T, 2>(scores, to, where, sl2, base)
+              : far ? tc_write_p<T, 0>(scores, to, where, sl2, base) : tc_write_p<T, 1>(scores, to, where, sl2, base);
+        // sums within 2^14 (P then fits both 16-bit types) need no new reference
+        if (again || !__any_sync(0xffffffffu, row < len && (!(sum <= TC_GROWTH) || m == -INFINITY))) break;
+        again = true;
+        tc_wait_st();
       }
-      const float base = m == -INFINITY ? 0.f : m;  // no key yet: all terms 0
-      const Pair minus = pair(-base, -base);
-      Pair sum = pair(0.f, 0.f);
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float s[32];
-        scores(c, s);
-        uint32_t p[16];
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const Pair e = exp2_2(add2(pair(s[j], s[j + 1]), minus));
-          sum = add2(sum, e);
-          const float2 f = both(e);
-          p[j / 2] = pack2<T>(f.x, f.y);
-        }
-        tc_st16(mine + Shape::P_COL + c * 16, p);
-      }
-      const float2 both_sums = both(sum);
-      l += both_sums.x + both_sums.y;
+      if (!ok) break;
+      l += sum;
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(p_full + (t & 1) * 8);
     }
-    if (ok) ok = wait(o_done, (n_tiles - 1) & 1, ERR_TC_O);
+    if (ok) ok = wait(o_done + ((n_tiles - 1) & 1) * 8, ((n_tiles - 1) / 2) & 1, ERR_TC_O);
     tc_fence_after();
     const bool some = row < len && l != 0.f;
-    const float inv = ok ? (some ? 1.f / l : 0.f) : NAN;
+    const float inv = some ? 1.f / l : 0.f;
     T* to = out + (int64_t)row * g.heads * D;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t raw[32];
-      tc_ld32(mine + Shape::O_COL + c * 32, raw);
+      tc_ld32(mine + TC_O_COL + c * 32, raw);
       tc_wait_ld();
       if (row < g.tokens) {
 #pragma unroll
@@ -331,7 +362,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 4) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
   }
@@ -339,22 +370,51 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
 
 namespace {
 
+// Rows of one head of a [batch, tokens, heads, D] tensor as TMA boxes of `rows` tokens.
+int tc_map(CUtensorMap* map, const void* base, const int64_t (&stride)[3], const RelArgs& g, int heads, int d, int rows, bool bf16) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return MGBS_ERR_STATE;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)g.tokens, (cuuint64_t)heads, (cuuint64_t)g.batch};
+  const int64_t by[3] = {stride[1], stride[2], stride[0]};  // token, head, batch
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (cuuint64_t)by[i] * 2 : (cuuint64_t)d * 2;
+  const cuuint32_t box[4] = {(cuuint32_t)d, (cuuint32_t)rows, 1, 1}, each[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides,
+                         box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, d == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : MGBS_ERR_STATE;
+}
+
+bool tc_stride_fits(const int64_t (&s)[3], const RelArgs& g, int heads) {
+  const int64_t n[3] = {g.batch, g.tokens, heads};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] >= (1ll << 38))) return false;
+  return true;
+}
+
 template <typename T, int D> int run_tc(const RelArgs& g, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
-  const int most = 113 * 1024;
-  const int rc = raise_smem(k_rel_tc<T, D>, most, raised);
+  int rc = raise_smem(k_rel_tc<T, D>, 113 * 1024, raised);
   if (rc) return rc;
-  const int tiles = (g.tokens + TC_TILE - 1) / TC_TILE;
+  const int tiles = (g.tokens + TC_Q - 1) / TC_Q;
   const int64_t blocks = (int64_t)tiles * g.heads * g.batch;
   if (blocks > 0x7fffffffll) return MGBS_ERR_TOO_LARGE;
+  constexpr bool BF = TcType<T>::FORMAT == 1;
+  CUtensorMap q, k, v;
+  rc = tc_map(&q, g.q, g.qs, g, g.heads, D, TC_Q, BF);
+  if (!rc) rc = tc_map(&k, g.k, g.ks, g, g.heads_kv, D, TC_K, BF);
+  if (!rc) rc = tc_map(&v, g.v, g.vs, g, g.heads_kv, D, TC_K, BF);
+  if (rc) return rc;
   // never more than two blocks on an SM: a third would wait for tensor memory
-  int smem = 5 * TcShape<D>::MAT + (2 * (g.reach + TC_RIM) + 1) * 4;
+  int smem = 1024 + (TC_Q + 2 * TC_STAGES * TC_K) * D * 2 + (2 * (g.reach + TC_RIM) + 1) * 4;
   if (smem < 78 * 1024) smem = 78 * 1024;
-  k_rel_tc<T, D><<<(unsigned)blocks, TC_THREADS, smem, st>>>(g, tiles);
+  k_rel_tc<T, D><<<(unsigned)blocks, TC_THREADS, smem, st>>>(q, k, v, g, tiles);
   return (int)cudaGetLastError();
 }
 
 }  // namespace
+
+bool rel_attention_tc_fits(const RelArgs& g) { return tc_stride_fits(g.qs, g, g.heads) && tc_stride_fits(g.ks, g, g.heads_kv) && tc_stride_fits(g.vs, g, g.heads_kv); }
 
 int rel_attention_tc(const RelArgs& g, int dtype, int head_dim, cudaStream_t st) {
   if (dtype == MGBS_DT_BF16) return head_dim == 32 ? run_tc<__nv_bfloat16, 32>(g, st) : run_tc<__nv_bfloat16, 64>(g, st);
