@@ -82,6 +82,8 @@ __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.
 
 // A wait that ends after a second at most, or as soon as another of the block has given up.
 static __device__ __noinline__ bool tc_wait_slow(uint32_t bar, uint32_t parity, int* gave_up, int* error, int code) {
+  for (int i = 0; i < 256; ++i)  // the clock is slow to read: not in an ordinary wait
+    if (mbar_try_wait(bar, parity)) return true;
   uint64_t start, now;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
   for (;;) {
@@ -93,6 +95,13 @@ static __device__ __noinline__ bool tc_wait_slow(uint32_t bar, uint32_t parity, 
   }
   if (atomicExch(gave_up, 1) == 0 && error) atomicCAS(error, 0, code);
   return false;
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
 }
 
 // A tile as a softmax thread sees it.
@@ -179,7 +188,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
   const Where w0 = rel_where(tiles, g.heads);
   const int tile = tiles - 1 - w0.tile, head = w0.head, batch = w0.b;  // under a causal mask the longest rows start first
   if (batch >= rel_batch(g)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int len = rel_length(g, batch), i0 = tile * TC_Q;
   T* out = static_cast<T*>(g.out) + ((int64_t)batch * g.tokens * g.heads + head) * D;
   float2* stats = g.stats ? g.stats + ((int64_t)batch * g.heads + head) * g.tokens : nullptr;
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
     for (int i = 0; i < 4 * TC_STAGES; ++i) mbar_init(bar + i * 8, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i * 8, 1);
-      mbar_init(p_full + i * 8, 128);
+      mbar_init(p_full + i * 8, 4);
       mbar_init(o_done + i * 8, 1);
     }
     mbar_init(q_full, 1);
@@ -256,35 +265,40 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
       }
     }
   } else if (warp == 4) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = tc_idesc<T>(TC_K, false), id_o = tc_idesc<T>(D, true);
-      const uint64_t q_desc = tc_desc<D>(q_at);
-      auto score = [&](int t) {
-        const int s = t % TC_STAGES;
-        if (!wait(k_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD)) return false;
-        tc_fence_after();
-        const uint64_t k_desc = tc_desc<D>(k_at + s * K_BYTES);
+    // The whole warp walks and waits, one elected lane issues: descriptors then stay in uniform registers.  (With one lane
+    // doing all of it, four products and a commit took 400 to 600 cycles.)
+    constexpr uint32_t id_s = tc_idesc<T>(TC_K, false), id_o = tc_idesc<T>(D, true);
+    const uint64_t q_desc = tc_desc<D>(q_at);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    auto score = [&](int t) {
+      const int s = t % TC_STAGES;
+      if (!wait(k_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD)) return false;
+      tc_fence_after();
+      const uint64_t k_desc = tc_desc<D>(k_at + s * K_BYTES);
+      if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) tc_mma_f16(tmem + (t & 1) * TC_K, q_desc + kk * 2, k_desc + kk * 2, id_s, kk > 0);
+        for (int kk = 0; kk < D / 16; ++kk) tc_mma_f16(tm + (t & 1) * TC_K, q_desc + kk * 2, k_desc + kk * 2, id_s, kk > 0);
         tc_commit(k_free + s * 8);
         tc_commit(s_full + (t & 1) * 8);
-        return true;
-      };
-      bool ok = wait(q_full, 0, ERR_TC_LOAD) && score(0) && (n_tiles < 2 || score(1));
-      for (int t = 0; ok && t < n_tiles; ++t) {
-        const int s = t % TC_STAGES;
-        ok = wait(p_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_P) && wait(v_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD) &&
-             (!fix_v || t + 1 < n_tiles || wait(v_fixed, 0, ERR_TC_LOAD));
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t v_desc = tc_desc<D>(v_at + s * K_BYTES);
+      }
+      return true;
+    };
+    bool ok = wait(q_full, 0, ERR_TC_LOAD) && score(0) && (n_tiles < 2 || score(1));
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      const int s = t % TC_STAGES;
+      ok = wait(v_full + s * 8, (t / TC_STAGES) & 1, ERR_TC_LOAD) && (!fix_v || t + 1 < n_tiles || wait(v_fixed, 0, ERR_TC_LOAD)) &&
+           wait(p_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_P);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t v_desc = tc_desc<D>(v_at + s * K_BYTES);
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < TC_K / 16; ++kk)
-          tc_mma_ts(tmem + TC_O_COL, tmem + TC_P_COL + (t & 1) * 32 + kk * 8, v_desc + kk * (16 * D * 2 >> 4), id_o, t > 0 || kk > 0);
+          tc_mma_ts(tm + TC_O_COL, tm + TC_P_COL + (t & 1) * 32 + kk * 8, v_desc + kk * (16 * D * 2 >> 4), id_o, t > 0 || kk > 0);
         tc_commit(v_free + s * 8);
         tc_commit(o_done + (t & 1) * 8);
-        if (t + 2 < n_tiles) ok = score(t + 2);  // into the buffer that this tile's softmax has left
       }
+      if (t + 2 < n_tiles) ok = score(t + 2);  // into the buffer that this tile's softmax has left
     }
     __syncwarp();
   } else {
@@ -336,7 +350,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
       l += sum;
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(p_full + (t & 1) * 8);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + (t & 1) * 8);
     }
     if (ok) ok = wait(o_done + ((n_tiles - 1) & 1) * 8, ((n_tiles - 1) / 2) & 1, ERR_TC_O);
     tc_fence_after();
