@@ -133,7 +133,7 @@ template <int MODE> __device__ __forceinline__ void tc_scores(const TcTile& w, i
 }
 
 // A row's exact maximum over the tile.
-static __device__ __noinline__ float tc_maximum(uint32_t scores, const TcTile& w, Pair sl2) {
+static __device__ __noinline__ float tc_maximum(uint32_t scores, TcTile w, Pair sl2) {
   float top = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < TC_K / 32; ++c) {
@@ -175,6 +175,11 @@ template <typename T, int MODE> __device__ __forceinline__ float tc_write_p(uint
   }
   const float2 f = both(sum);
   return f.x + f.y;
+}
+
+// The same out of line, for a row's first tile and for new references.
+template <typename T> static __device__ __noinline__ float tc_write_p_again(uint32_t scores, uint32_t to, TcTile w, Pair sl2, float base) {
+  return tc_write_p<T, 2>(scores, to, w, sl2, base);
 }
 
 template <typename T, int D>
@@ -313,40 +318,41 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
       const bool edge = j0 + TC_K > len || (g.causal && j0 + TC_K > i0 + 1);
       const TcTile where{far, edge, j0, row, len, g.causal, far > 0 ? bt[2 * side] : bt[0], bt + j0 - row + side};
       const uint32_t scores = mine + (t & 1) * TC_K, to = mine + TC_P_COL + (t & 1) * 32;
-      ok = wait(s_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_S) && (t < 2 || wait(o_done + (t & 1) * 8, (t / 2 - 1) & 1, ERR_TC_O));
+      // S(t) was issued behind O += P(t - 2) V(t - 2), so that P's buffer is free too
+      ok = wait(s_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_S);
       if (!ok) break;
       tc_fence_after();
-      float sum;
-      for (bool again = t == 0;;) {
-        if (again) {
-          const float top = fmaxf(m, tc_maximum(scores, where, sl2));
-          if (t > 0) {
-            ok = wait(o_done + ((t - 1) & 1) * 8, ((t - 1) / 2) & 1, ERR_TC_O);  // O is still
-            if (!ok) break;
-            tc_fence_after();
-            const float f = top == -INFINITY ? 1.f : fast_exp2(m - top);
-            l *= f;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t raw[32];
-              tc_ld32(mine + TC_O_COL + c * 32, raw);
-              tc_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
-              tc_st32(mine + TC_O_COL + c * 32, raw);
-            }
-          }
-          m = top;
-        }
+      float sum = 0.f;
+      bool again = t == 0;
+      if (!again) {
         const float base = m == -INFINITY ? 0.f : m;  // no key yet: all terms 0
         sum = edge ? tc_write_p<T, 2>(scores, to, where, sl2, base)
               : far ? tc_write_p<T, 0>(scores, to, where, sl2, base) : tc_write_p<T, 1>(scores, to, where, sl2, base);
         // sums within 2^14 (P then fits both 16-bit types) need no new reference
-        if (again || !__any_sync(0xffffffffu, row < len && (!(sum <= TC_GROWTH) || m == -INFINITY))) break;
-        again = true;
-        tc_wait_st();
+        again = __any_sync(0xffffffffu, row < len && (!(sum <= TC_GROWTH) || m == -INFINITY));
       }
-      if (!ok) break;
+      if (again) {
+        tc_wait_st();
+        const float top = fmaxf(m, tc_maximum(scores, where, sl2));
+        if (t > 0) {
+          ok = wait(o_done + ((t - 1) & 1) * 8, ((t - 1) / 2) & 1, ERR_TC_O);  // O is still
+          if (!ok) break;
+          tc_fence_after();
+          const float f = top == -INFINITY ? 1.f : fast_exp2(m - top);
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t raw[32];
+            tc_ld32(mine + TC_O_COL + c * 32, raw);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
+            tc_st32(mine + TC_O_COL + c * 32, raw);
+          }
+        }
+        m = top;
+        sum = tc_write_p_again<T>(scores, to, where, sl2, m == -INFINITY ? 0.f : m);
+      }
       l += sum;
       tc_wait_st();
       tc_fence_before();
