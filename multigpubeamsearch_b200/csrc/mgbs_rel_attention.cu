@@ -24,12 +24,11 @@
 namespace mgbs {
 
 constexpr int REL_THREADS = 128;
-#ifndef REL_FWD_BLOCKS
-#define REL_FWD_BLOCKS 4
-#endif
-#ifndef REL_BWD_BLOCKS
-#define REL_BWD_BLOCKS 3
-#endif
+// Blocks per multiprocessor that a kernel's registers are held to, each the fastest of those tried:
+constexpr int REL_FWD_BLOCKS = 4;  // 3: 806 us against 749 us at 32768 x 54 tokens, 8 heads of 32
+constexpr int REL_BWD_BLOCKS = 3;  // 2: 546 us against 538 us at 8192 x 54 tokens
+constexpr int REL_Q_BLOCKS = 3;    // 2: 112 us against 107 us at 6 x 1501 causal tokens, 8 heads of 64 over 2
+constexpr int REL_KV_BLOCKS = 3;   // 2: 132 us, 4: 154 us against 119 us there, with the heads one after the other
 // rows of the short form's matrices are padded by 16 bytes: eight rows then start in distinct banks
 template <int D> struct RelTile { static constexpr int PITCH = D + 8; };
 
@@ -512,7 +511,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles(const __grid_constant
   extern __shared__ __align__(16) uint8_t rel_smem[];
   T* qs = reinterpret_cast<T*>(rel_smem);
   float* bt = reinterpret_cast<float*>(rel_smem + 5 * tile_bytes<D>());
-  Where w = rel_where(tiles, g.heads);
+  Where w = rel_where(blockIdx.x, tiles, g.heads, g.batch);
   w.tile = tiles - 1 - w.tile;  // under a causal mask the longest rows start first
   if (w.b >= rel_batch(g)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
@@ -634,19 +633,24 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles(const __grid_constant
   }
 }
 
-// dq, delta and the table's gradient: a block owns 64 queries and walks over the keys.
+// dq, delta and the table's gradient: a block owns 64 queries and walks over the keys.  Bound by the latency of a warp's
+// chain of products and exponentials, with 12 warps on a multiprocessor: 107 us at 6 x 1501 causal tokens, 8 heads of 64
+// over 2 (143 us before the longest tiles of all heads started first and dS moved into the place of q and dout).
 constexpr int DS_PITCH = TILE + 1;
+template <int D> __host__ __device__ constexpr int dq_front() {  // q and dout, whose place a tile of dS takes
+  return 2 * tile_bytes<D>() > TILE * DS_PITCH * 4 ? 2 * tile_bytes<D>() : TILE * DS_PITCH * 4;
+}
 template <typename T, int D>
-__global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_constant__ RelArgs g, int tiles) {
+__global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(const __grid_constant__ RelArgs g, int tiles) {
   constexpr int PITCH = RelTile<D>::PITCH, MAT = TILE * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
   __shared__ float far_sum[2][4];
-  float* bt = reinterpret_cast<float*>(rel_smem + 6 * tile_bytes<D>());
+  float* ds = reinterpret_cast<float*>(rel_smem);  // one tile of dS, once q and dout are in registers
+  float* bt = reinterpret_cast<float*>(rel_smem + dq_front<D>() + 4 * tile_bytes<D>());
   const int side = g.reach + REL_RIM, span = 2 * side + 1;
   float* dacc = bt + span;            // dS by offset
-  float* ds = dacc + span;            // one tile of dS
-  Where w = rel_where(tiles, g.heads);
-  w.tile = tiles - 1 - w.tile;
+  Where w = rel_where(blockIdx.x, tiles, g.heads, g.batch);
+  w.tile = tiles - 1 - w.tile;  // the longest first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int len = rel_length(g, w.b), i0 = w.tile * TILE, row0 = i0 + warp * 16 + gid;
   const int64_t head_at = ((int64_t)w.b * g.tokens * g.heads + w.head) * D;
@@ -664,7 +668,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_const
   const T* k = static_cast<const T*>(g.k) + w.b * g.ks[0] + head_kv * g.ks[2];
   const T* v = static_cast<const T*>(g.v) + w.b * g.vs[0] + head_kv * g.vs[2];
   const T* dout = static_cast<const T*>(g.dout) + w.b * g.ds[0] + w.head * g.ds[2];
-  const uint32_t q_at = smem_addr(rel_smem), do_at = q_at + MAT * 2, kv_at = q_at + 2 * MAT * 2;
+  const uint32_t q_at = smem_addr(rel_smem), do_at = q_at + MAT * 2, kv_at = q_at + dq_front<D>();
   const int last = g.causal ? min(len, i0 + TILE) : len, n_tiles = (last + TILE - 1) / TILE;
   auto load = [&](int t) {
     const uint32_t to = kv_at + (t & 1) * 2 * MAT * 2;
@@ -716,6 +720,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_const
         }
       d0 = quad_sum(d0);
       d1 = quad_sum(d1);
+      __syncthreads();  // q and dout make room
     }
     const uint32_t at = kv_at + (t & 1) * 2 * MAT * 2;
     const int j0 = t * TILE;
@@ -727,7 +732,6 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_const
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
       float s[2][4], dp[2][4];
-      uint32_t a[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = dp[0][e] = dp[1][e] = 0.f;
       rows_product<T, D>(s[0], s[1], qa, at + (jj * 16 * PITCH + frag_b<PITCH>(lane)) * 2);
@@ -753,10 +757,18 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_const
 #pragma unroll
           for (int e = 0; e < 4; ++e) ds[(warp * 16 + gid + (e >> 1) * 8) * DS_PITCH + (2 * jj + n) * 8 + 2 * tig + (e & 1)] = dp[n][e];
       }
+      uint32_t a[4], b[4];
       pack_a<T>(a, dp[0], dp[1]);
-      cols_product<T, D>(o, a, at + (jj * 16 * PITCH + frag_a<PITCH>(lane)) * 2);
-      pack_a<T>(a, s[0], s[1]);
-      cols_product<T, D>(pk, a, at + (jj * 16 * PITCH + frag_a<PITCH>(lane)) * 2);
+      pack_a<T>(b, s[0], s[1]);
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t m[4];
+        ldsm4_t(m, at + (jj * 16 * PITCH + frag_a<PITCH>(lane)) * 2 + n * 32);
+        mma16816<T>(o[2 * n], a, m[0], m[1]);
+        mma16816<T>(o[2 * n + 1], a, m[2], m[3]);
+        mma16816<T>(pk[2 * n], b, m[0], m[1]);
+        mma16816<T>(pk[2 * n + 1], b, m[2], m[3]);
+      }
     }
     const float tile_sum = (r0 + r1) - seen;
     if (far > 0) after += tile_sum;
@@ -809,41 +821,53 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dq(const __grid_const
   }
 }
 
-// dk and dv: a block owns 64 keys and walks over the queries of all heads that share them, in transposed products
-// (keys as rows), so that P^T and dS^T come out of the accumulators as operands of the next product.
+__device__ __forceinline__ void rel_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 get_remote(const float* local, int rank) {  // the same address in block `rank` of the cluster
+  uint32_t at;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// dk and dv: a block owns 64 keys and walks over queries, in transposed products (keys as rows), so that P^T and dS^T come
+// out of the accumulators as operands of the next product.  The query heads that share the keys are spread over the
+// `ranks` blocks of a cluster, whose sums are added through distributed shared memory at the end, in a fixed order: one
+// block for all heads left most of the device idle (210 us against 119 us at 6 x 1501 causal tokens, 8 heads over 2; 102 us with the longest tiles
+// first).
 template <typename T, int D>
-__global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dkv(const __grid_constant__ RelArgs g, int tiles) {
+__global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(const __grid_constant__ RelArgs g, int tiles, int ranks) {
   constexpr int PITCH = RelTile<D>::PITCH, MAT = TILE * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
   __shared__ float2 row_stat[2][TILE];  // a stage's queries: maximum and log2 of the sum
   __shared__ float row_delta[2][TILE];
   float* bt = reinterpret_cast<float*>(rel_smem + 6 * tile_bytes<D>());
-  const int side = g.reach + REL_RIM, span = 2 * side + 1;
-  const Where w = rel_where(tiles, g.heads_kv);
+  const int side = g.reach + REL_RIM;
+  const int rank = (int)(blockIdx.x % ranks);
+  const Where w = rel_where(blockIdx.x / ranks, tiles, g.heads_kv, g.batch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int len = rel_length(g, w.b), j0 = w.tile * TILE, row0 = j0 + warp * 16 + gid;
-  const int64_t off0 = (((int64_t)w.b * g.tokens + row0) * g.heads_kv + w.head) * D, off1 = off0 + (int64_t)8 * g.heads_kv * D;
-  const bool have0 = row0 < g.tokens, have1 = row0 + 8 < g.tokens;
-  T* dk = static_cast<T*>(g.dk);
-  T* dv = static_cast<T*>(g.dv);
-  if (j0 >= len) {
-    store_zero_rows<T, D>(have0 ? dk + off0 : nullptr, have1 ? dk + off1 : nullptr);
-    store_zero_rows<T, D>(have0 ? dv + off0 : nullptr, have1 ? dv + off1 : nullptr);
+  auto row_of = [&](void* base, int row) { return row < g.tokens ? static_cast<T*>(base) + (((int64_t)w.b * g.tokens + row) * g.heads_kv + w.head) * D : nullptr; };
+  if (j0 >= len) {  // the whole cluster
+    if (rank == 0) {
+      store_zero_rows<T, D>(row_of(g.dk, row0), row_of(g.dk, row0 + 8));
+      store_zero_rows<T, D>(row_of(g.dv, row0), row_of(g.dv, row0 + 8));
+    }
     return;
   }
-  const int share = g.heads / g.heads_kv;
+  const int share = g.heads / g.heads_kv / ranks;  // heads of this block: rank, rank + ranks, ...
   const uint32_t k_at = smem_addr(rel_smem), v_at = k_at + MAT * 2, qd_at = k_at + 2 * MAT * 2;
   const int first = g.causal ? w.tile : 0, n_tiles = (len + TILE - 1) / TILE - first, steps = n_tiles * share;
   auto load = [&](int n) {
-    const int h = w.head * share + n / n_tiles, row = (first + n % n_tiles) * TILE;
+    const int h = (w.head * share + n / n_tiles) * ranks + rank, row = (first + n % n_tiles) * TILE;
     const uint32_t to = qd_at + (n & 1) * 2 * MAT * 2;
     stage_tile<T, D>(to, static_cast<const T*>(g.q) + w.b * g.qs[0] + h * g.qs[2], g.qs[1], row, len);
     stage_tile<T, D>(to + MAT * 2, static_cast<const T*>(g.dout) + w.b * g.ds[0] + h * g.ds[2], g.ds[1], row, len);
-    if (threadIdx.x < TILE) {
+    if (threadIdx.x < TILE) {  // rows past the length: zeros, and hidden below
       const int i = row + threadIdx.x;
-      const int64_t at = ((int64_t)w.b * g.heads + h) * g.tokens + i;
-      row_stat[n & 1][threadIdx.x] = i < len ? g.stats[at] : make_float2(0.f, INFINITY);
-      row_delta[n & 1][threadIdx.x] = i < len ? g.delta[at] : 0.f;
+      const int64_t at = ((int64_t)w.b * g.heads + h) * g.tokens + (i < len ? i : 0);
+      copy_small<8>(smem_addr(&row_stat[n & 1][threadIdx.x]), g.stats + at, i < len);
+      copy_small<4>(smem_addr(&row_delta[n & 1][threadIdx.x]), g.delta + at, i < len);
     }
   };
   stage_tile<T, D>(k_at, static_cast<const T*>(g.k) + w.b * g.ks[0] + w.head * g.ks[2], g.ks[1], j0, len);
@@ -860,7 +884,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dkv(const __grid_cons
     const int i0 = (first + n % n_tiles) * TILE;
     if (n % n_tiles == 0) {
       __syncthreads();  // the head before has read its biases
-      fill_bias<T>(g, w.head * share + n / n_tiles, bt, g.reach + REL_RIM, threadIdx.x, REL_THREADS);
+      fill_bias<T>(g, (w.head * share + n / n_tiles) * ranks + rank, bt, side, threadIdx.x, REL_THREADS);
     }
     copy_wait<0>();
     __syncthreads();
@@ -877,7 +901,7 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dkv(const __grid_cons
     const int far = rel_side(i0, j0, g.reach);
     const float fixed = far > 0 ? bt[2 * side] : bt[0];
     const float* b0 = bt + row0 - i0 - 2 * tig + side;  // offset of key row0 from query i0 + 2 tig
-    const bool diagonal = g.causal && j0 + TILE > i0 + 1;
+    const bool edge = i0 + TILE > len || (g.causal && j0 + TILE > i0 + 1);
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii) {  // 16 queries each
       float s[2][4], dp[2][4];
@@ -894,7 +918,10 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dkv(const __grid_cons
           const int c = (2 * ii + m) * 8 + (e & 1);
           const float bias = far ? fixed : b0[(e >> 1) * 8 - c];
           float p = fast_exp2((fmaf(s[m][e], g.sl2, bias) - (e & 1 ? st.z : st.x)) - (e & 1 ? st.w : st.y));
-          if (diagonal && row0 + (e >> 1) * 8 > i0 + c + 2 * tig) p = 0.f;
+          if (edge) {
+            const int i = i0 + c + 2 * tig;
+            if (i >= len || (g.causal && row0 + (e >> 1) * 8 > i)) p = 0.f;
+          }
           s[m][e] = p;
           dp[m][e] = p * (dp[m][e] - (e & 1 ? dl.y : dl.x));
         }
@@ -907,9 +934,40 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles_dkv(const __grid_cons
     }
   }
   const float in0 = row0 < len ? 1.f : 0.f, in1 = row0 + 8 < len ? 1.f : 0.f;
-  (void)span;
-  store_rows<T, D>(ov, in0, in1, have0 ? dv + off0 : nullptr, have1 ? dv + off1 : nullptr);
-  store_rows<T, D>(ok, in0 * g.scale, in1 * g.scale, have0 ? dk + off0 : nullptr, have1 ? dk + off1 : nullptr);
+  if (ranks == 1) {
+    store_rows<T, D>(ov, in0, in1, row_of(g.dv, row0), row_of(g.dv, row0 + 8));
+    store_rows<T, D>(ok, in0 * g.scale, in1 * g.scale, row_of(g.dk, row0), row_of(g.dk, row0 + 8));
+    return;
+  }
+  constexpr int SP = D + 4;
+  float* sums = reinterpret_cast<float*>(rel_smem);  // [dv, dk][TILE][SP]
+  static_assert(2 * TILE * SP * 4 <= 6 * tile_bytes<D>(), "the sums fit the stages");
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = (warp * 16 + gid + (e >> 1) * 8) * SP + n * 8 + 2 * tig + (e & 1);
+      sums[at] = ov[n][e];
+      sums[TILE * SP + at] = ok[n][e];
+    }
+  rel_cluster_sync();
+  for (int c = rank * REL_THREADS + threadIdx.x; c < 2 * TILE * (D / 8); c += ranks * REL_THREADS) {
+    const int which = c / (TILE * (D / 8)), row = c / (D / 8) % TILE, part = c % (D / 8) * 8;
+    if (j0 + row >= g.tokens) continue;
+    const float* from = sums + (which * TILE + row) * SP + part;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < ranks; ++r) {
+      const float4 a = get_remote(from, r), b = get_remote(from + 4, r);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    const float f = j0 + row < len ? (which ? g.scale : 1.f) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= f;
+    *reinterpret_cast<uint4*>(row_of(which ? g.dk : g.dv, j0 + row) + part) = Vec16<T>::down(v);
+  }
+  rel_cluster_sync();  // a block's sums stay until all have been read
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -1016,7 +1074,7 @@ template <typename T, int D> int run_tiles(const RelArgs& g, cudaStream_t st) {
 
 template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, float* sums, cudaStream_t st) {
   static std::atomic<uint64_t> raised_q{0}, raised_kv{0};
-  const int fixed_q = 6 * tile_bytes<D>() + TILE * DS_PITCH * 4, fixed_kv = 6 * tile_bytes<D>();
+  const int fixed_q = dq_front<D>() + 4 * tile_bytes<D>(), fixed_kv = 6 * tile_bytes<D>();
   int rc = raise_smem(k_rel_tiles_dq<T, D>, fixed_q + 2 * rel_bias_floats(1024) * 4, raised_q);
   if (!rc) rc = raise_smem(k_rel_tiles_dkv<T, D>, fixed_kv + rel_bias_floats(1024) * 4, raised_kv);
   if (rc) return rc;
@@ -1026,8 +1084,21 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, f
   k_rel_tiles_dq<T, D><<<(unsigned)blocks, REL_THREADS, fixed_q + 2 * rel_bias_floats(g.reach) * 4, st>>>(g, tiles);
   rc = (int)cudaGetLastError();
   if (rc) return rc;
-  k_rel_tiles_dkv<T, D><<<(unsigned)(rows * g.heads_kv), REL_THREADS, fixed_kv + rel_bias_floats(g.reach) * 4, st>>>(g, tiles);
-  rc = (int)cudaGetLastError();
+  int ranks = 1;  // the most blocks that the shared heads can be dealt to
+  for (int r = 2; r <= 8; ++r)
+    if (g.heads / g.heads_kv % r == 0) ranks = r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * g.heads_kv * ranks));
+  cfg.blockDim = dim3(REL_THREADS);
+  cfg.dynamicSmemBytes = fixed_kv + rel_bias_floats(g.reach) * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ranks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  rc = (int)cudaLaunchKernelEx(&cfg, k_rel_tiles_dkv<T, D>, g, tiles, ranks);
   if (rc) return rc;
   if (rows <= 256) return finish_table<T>(g, g.partial, rows, rows, 1, dtable, st);
   const int64_t chunk = (rows + REL_CHUNKS - 1) / REL_CHUNKS;

@@ -43,10 +43,16 @@ template <typename T> __device__ __forceinline__ void fill_bias(const RelArgs& g
   for (int i = thread; i < 2 * side + 1; i += threads) bt[i] = scaled_bias(rel_bias<T>(g, i - side, h), kLog2e, REL_BIG);
 }
 
+// Block n's tile of one (sequence, head).  Tiles are dealt out to groups of 64 heads, the heads fastest: under a causal
+// mask the longest tiles of a whole group start first (dq 143 us against 111 us head by head, the forward 42 us against
+// 34 us, at 6 x 1501 tokens x 8 heads).  The group bounds what the L2 cache has to hold of k and v.
+constexpr int REL_DEAL = 64;
 struct Where { int tile, head, b; };
-__device__ __forceinline__ Where rel_where(int tiles, int heads) {
-  const int64_t n = blockIdx.x;
-  return {(int)(n % tiles), (int)(n / tiles % heads), (int)(n / tiles / heads)};
+__device__ __forceinline__ Where rel_where(int64_t n, int tiles, int heads, int batch) {
+  const int64_t first = n / ((int64_t)tiles * REL_DEAL) * REL_DEAL, left = (int64_t)heads * batch - first;
+  const int in = (int)(n - first * tiles), members = left < REL_DEAL ? (int)left : REL_DEAL;
+  const int64_t unit = first + in % members;
+  return {in / members, (int)(unit % heads), (int)(unit / heads)};
 }
 
 // The forward on the fifth-generation tensor cores, and whether TMA can describe the strides (it knows no stride of 0).

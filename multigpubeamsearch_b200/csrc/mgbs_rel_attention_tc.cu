@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
   __shared__ __align__(8) uint64_t bars[4 * TC_STAGES + 8];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
-  const Where w0 = rel_where(tiles, g.heads);
+  const Where w0 = rel_where(blockIdx.x, tiles, g.heads, g.batch);
   const int tile = tiles - 1 - w0.tile, head = w0.head, batch = w0.b;  // under a causal mask the longest rows start first
   if (batch >= rel_batch(g)) return;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
