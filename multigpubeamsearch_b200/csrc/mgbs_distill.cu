@@ -480,9 +480,11 @@ template <typename T, bool GRAD> int distill_wide(const DistillArgs& g, int sms,
   while (ranks < 8 && g.rows * ranks < sms && pieces > ranks * 1024) ++ranks;
   if (g.rows * ranks > 0x7fffffffll) return MGBS_ERR_TOO_LARGE;
   const int per_block = (int)((pieces + ranks - 1) / ranks);
-  const int capacity = per_block * 16 <= DISTILL_HELD ? per_block : DISTILL_HELD / 16;
   int threads = 128;  // some four pieces per thread and more
   while (threads < DISTILL_WIDE && threads * 8 <= per_block) threads *= 2;
+  // of a row that is not all held, whole turns of the threads: the slow way deals the pieces out without these limits, and
+  // a thread must come to the same pieces on both
+  const int turn = threads - 32, capacity = per_block * 16 <= DISTILL_HELD ? per_block : DISTILL_HELD / 16 / turn * turn;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(g.rows * ranks));
   cfg.blockDim = dim3(threads);

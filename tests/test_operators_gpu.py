@@ -699,3 +699,256 @@ def test_captured_and_replayed(tokens):
         for new, out in zip(fresh, outs):
             want = run_everything(*new, rotary, plan)
             assert all(torch.equal(x, y) for x, y in zip(want, out))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Long sequences: layouts, shared heads, references that have to follow, padding
+# ---------------------------------------------------------------------------------------------------------------
+
+LONG_CASES = [
+    (2, 66, 3, 3, 64, "bf16", False, True, "packed"),
+    (3, 127, 6, 2, 64, "f16", True, False, "shifted"),
+    (2, 130, 6, 1, 64, "bf16", False, True, "transposed"),
+    (1, 200, 12, 1, 64, "f16", True, True, "transposed"),
+    (1, 150, 7, 1, 32, "bf16", True, False, "packed"),
+    (1, 150, 11, 1, 32, "bf16", False, True, "packed"),
+    (1, 150, 16, 1, 32, "f16", True, False, "packed"),
+    (70, 130, 2, 2, 64, "bf16", True, True, "packed"),
+    (2, 330, 9, 3, 32, "bf16", True, True, "transposed"),
+    (3, 385, 2, 2, 32, "f16", False, True, "shifted"),
+    (2, 449, 2, 2, 32, "bf16", False, False, "packed"),
+]
+
+
+@pytest.mark.parametrize("case", LONG_CASES, ids=str)
+def test_long_attention(case):
+    q, k, v, table, plan, lengths, dout = attention_inputs(case, seed=30)
+    attention_check(q, k, v, table, plan, lengths, dout=dout)
+
+
+@pytest.mark.parametrize("tokens,d", [(20, 32), (150, 64), (330, 32)])
+def test_relative_attention_broadcast_inputs(tokens, d):
+    """Sequences, tokens and heads that share memory: strides of 0, and each reader's own gradient."""
+    gen, plan = generator(31), ops.RelativeBuckets()
+    table, dout = normal(gen, 32, 4, dtype=torch.bfloat16), normal(gen, 3, tokens, 4, d, dtype=torch.bfloat16)
+    q = normal(gen, 1, tokens, 4, d, dtype=torch.bfloat16).expand(3, -1, -1, -1)
+    k = normal(gen, 3, tokens, 1, d, dtype=torch.bfloat16).expand(-1, -1, 4, -1)
+    v = normal(gen, 3, 1, 4, d, dtype=torch.bfloat16).expand(-1, tokens, -1, -1)
+    attention_check(q, k, v, table, plan, dout=dout)
+    whole = [x[:1].clone() for x in (q, k, v)]
+    base = [x.requires_grad_(True) for x in whole]
+    out = ops.relative_attention(*(x.expand(3, -1, -1, -1) for x in base), table, plan)
+    assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])
+    grads = torch.autograd.grad(out, base, dout[:1].expand(3, -1, -1, -1))
+    # the same call with a gradient per reader: strides decide between two forms, whose float32 sums differ
+    each = [x.detach().expand(3, -1, -1, -1).requires_grad_(True) for x in base]
+    per = torch.autograd.grad(ops.relative_attention(*each, table, plan), each, dout[:1].expand(3, -1, -1, -1))
+    for three, one in zip(grads, per):  # three equal 16-bit gradients: two roundings of their sum
+        one = one[:1].double()
+        within(three, 3 * one, 2 * half_step(torch.bfloat16) * 3 * one.abs(), "sum over the readers")
+
+
+@pytest.mark.parametrize("tokens,d", [(300, 64), (700, 32)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("way", ["rising", "falling", "leap"])
+def test_long_attention_scores_that_grow(tokens, d, dtype, way):
+    """Rows whose largest score comes late, early, or in one leap far beyond all before."""
+    q, k, v, table, plan, _, dout = attention_inputs((2, tokens, 2, 2, d, dtype, False, False, "packed"), seed=32)
+    grow = torch.linspace(0.05, 6.0, tokens, device="cuda")
+    if way == "leap":
+        grow = torch.where(torch.arange(tokens, device="cuda") == tokens - 9, 10.0, 0.2)
+    k = (k.float() * (grow.flip(0) if way == "falling" else grow)[:, None, None]).to(k.dtype)
+    ref = attention_reference(q, k, v, table, plan, None, d ** -0.5)
+    out = ops.relative_attention(q, k, v, table, plan)
+    u = half_step(k.dtype)
+    # P is relative to a reference that some key reaches, so the sum is at least 1, and P below the type's smallest
+    # normal number is off by half its spacing at most
+    small = 2.0 ** -25 * v.double().abs().sum(1, keepdim=True) if dtype == "f16" else 0.0
+    within(out, ref["out"], (2 * u + SLACK) * ref["out_abs"] + small + 2.0 ** -24, "out")
+    if dtype == "bf16":
+        attention_check(q, k, v, table, plan, dout=dout)
+
+
+@pytest.mark.parametrize("tokens,d", [(321, 64), (700, 32), (130, 32)])
+@pytest.mark.parametrize("open_", ["near", "far before", "far after", "tall"])
+def test_long_attention_closed_distances(tokens, d, open_):
+    """Tiles in which every bias is -inf, rows that see their first key late or none, a bias far above the scores."""
+    q, k, v, table, plan, lengths, dout = attention_inputs((3, tokens, 2, 2, d, "bf16", False, True, "packed"), seed=33)
+    table = table.clone()
+    before, after = int(plan.map[0]), int(plan.map[-1])
+    if open_ == "near":
+        table[before] = table[after] = -math.inf
+    elif open_ == "tall":
+        table[after] = 80.0
+    else:
+        keep = before if open_ == "far before" else after
+        table[torch.arange(32, device="cuda") != keep] = -math.inf
+    attention_check(q, k, v, table, plan, lengths, dout=dout)
+
+
+@pytest.mark.parametrize("tokens,d,shared", [(150, 64, 1), (150, 64, 3), (400, 32, 1)])
+def test_long_attention_never_reads_padding(tokens, d, shared):
+    q, k, v, table, plan, lengths, dout = attention_inputs((4, tokens, 3, 3 // shared, d, "bf16", False, True, "packed"), seed=34)
+    gone = torch.arange(tokens, device="cuda") >= lengths[:, None]
+    results = []
+    for fill in (math.nan, math.inf, 0.0):
+        xs = [x.clone() for x in (q, k, v, dout)]
+        for x in xs:
+            x[gone] = fill
+        leaves = [x.requires_grad_(True) for x in xs[:3]] + [table.clone().requires_grad_(True)]
+        out = ops.relative_attention(*leaves, plan, lengths=lengths)
+        results.append([out] + list(torch.autograd.grad(out, leaves, xs[3])))
+    for other in results[:2]:
+        assert all(torch.equal(x, y) for x, y in zip(results[2], other))
+    assert all(torch.isfinite(x).all() for x in results[2])
+    assert not any(x[gone].any() for x in results[2][:4])
+
+
+@pytest.mark.parametrize("tokens,d", [(20, 32), (100, 32), (100, 64)])
+def test_relative_attention_length_out_of_range(tokens, d):
+    """Lengths below 0 count as 0 and lengths above the tokens as all of them."""
+    q, k, v, table, plan, _, _ = attention_inputs((3, tokens, 2, 2, d, "bf16", True, False, "packed"), seed=35)
+    lengths = torch.tensor([-5, tokens + 7, 9], device="cuda", dtype=torch.int32)
+    held = torch.tensor([0, tokens, 9], device="cuda", dtype=torch.int32)
+    assert torch.equal(ops.relative_attention(q, k, v, table, plan, lengths=lengths), ops.relative_attention(q, k, v, table, plan, lengths=held))
+
+
+@pytest.mark.parametrize("tokens,d", [(20, 32), (100, 64), (100, 32)])
+def test_relative_attention_offsets_past_32_bits(tokens, d):
+    """Sequences that lie 2^31 elements apart."""
+    gen, apart = generator(36), (1 << 31) + 64
+    room = torch.empty(apart + tokens * 6 * d, dtype=torch.bfloat16, device="cuda")
+    x = room.as_strided((2, tokens, 6, d), (apart, 6 * d, d, 1))
+    x.copy_(normal(gen, 2, tokens, 6, d, dtype=torch.bfloat16))
+    table, plan = normal(gen, 32, 2, dtype=torch.bfloat16), ops.RelativeBuckets()
+    near, leaves = x.clone(), []
+    for y in (x, near):
+        leaves.append([y[:, :, 2 * n:2 * n + 2].detach().requires_grad_(True) for n in range(3)])
+    dout = normal(gen, 2, tokens, 2, d, dtype=torch.bfloat16)
+    outs = [ops.relative_attention(*y, table, plan) for y in leaves]
+    assert torch.equal(outs[0], outs[1])
+    far_dout = torch.empty(apart + tokens * 2 * d, dtype=torch.bfloat16, device="cuda").as_strided((2, tokens, 2, d), (apart, 2 * d, d, 1))
+    far_dout.copy_(dout)
+    for a, b in zip(torch.autograd.grad(outs[0], leaves[0], far_dout), torch.autograd.grad(outs[1], leaves[1], dout)):
+        assert torch.equal(a, b)
+
+
+def test_qk_norm_rope_offsets_past_32_bits():
+    gen, apart = generator(37), (1 << 31) + 64
+    x = torch.empty(apart + 30 * 64, dtype=torch.bfloat16, device="cuda").as_strided((2, 10, 3, 64), (apart, 192, 64, 1))
+    x.copy_(normal(gen, 2, 10, 3, 64, dtype=torch.bfloat16))
+    gain, rotary = torch.rand(64, generator=gen, device="cuda"), ops.RotaryFrequencies(64)
+    far, near = (ops.qk_norm_rope(y[:, :, :2], y[:, :, 2:], gain, gain, rotary) for y in (x, x.clone()))
+    assert torch.equal(far[0], near[0]) and torch.equal(far[1], near[1])
+
+
+def test_distill_offsets_past_32_bits():
+    """More logits than 32 bits count, in rows that a few blocks hold and in rows that a few lanes hold."""
+    gen = generator(38)
+    for rows, width in ((17000, 131072), (9000000, 240)):
+        logits = torch.empty(rows, width, dtype=torch.bfloat16, device="cuda")
+        part = [slice(0, 20), slice(rows - 20, rows)]
+        logits.zero_()
+        for p in part:
+            logits[p] = normal(gen, 20, width, dtype=torch.bfloat16)
+        teacher, index = normal(gen, rows, 2), torch.randint(0, width, (rows, 2), generator=gen, device="cuda")
+        loss, grad = ops.distill_top_logits_step(logits, teacher, index)
+        for p in part:
+            one, some = ops.distill_top_logits_step(logits[p].clone(), teacher[p], index[p])
+            assert torch.equal(loss[p], one) and torch.equal(grad[p], some)
+        del logits, loss, grad
+
+
+def long_step(seed):
+    gen = generator(seed)
+    x = normal(gen, 2, 200, 8, 64, dtype=torch.bfloat16)
+    leaves = [y.detach().requires_grad_(True) for y in (x[:, :, :6], x[:, :, 6:7], x[:, :, 7:])] + [normal(gen, 32, 6, dtype=torch.bfloat16).requires_grad_(True)]
+    return leaves, normal(gen, 2, 200, 6, 64, dtype=torch.bfloat16), torch.tensor([200, 133], device="cuda", dtype=torch.int32)
+
+
+def run_long_step(leaves, dout, lengths, plan):
+    out = ops.relative_attention(*leaves, plan, lengths=lengths)
+    return [out, *torch.autograd.grad(out, leaves, dout)]
+
+
+def test_long_attention_on_streams_and_replayed():
+    plan = ops.RelativeBuckets(causal=True)
+    sets = [long_step(s) for s in range(40, 44)]
+    want = [[t.detach().clone() for t in run_long_step(*s, plan)] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None] * len(sets)
+    for _ in range(5):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[n] = run_long_step(*sets[n], plan)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    del got, b  # a backward pass is captured only while no eager graph of its leaves lives
+    graphs, outs = [], []
+    for s in sets[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run_long_step(*s, plan))
+        graphs.append(g)
+    with torch.no_grad():
+        for held, new in zip(sets[:2], sets[2:]):
+            for x, y in zip((*held[0], *held[1:]), (*new[0], *new[1:])):
+                x.copy_(y)
+    for st, g in zip(streams, graphs):  # both in flight
+        with torch.cuda.stream(st):
+            g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want[2:], outs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_distill_wide_on_streams_and_replayed():
+    sets = [distill_inputs((40, 50021, 33, "bf16", torch.int64), seed=s) for s in range(50, 54)]
+    run = lambda s: ops.distill_top_logits_step(*s[:3], temperature=1.5, row_weight=s[3])  # noqa: E731
+    want = [[t.clone() for t in run(s)] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None] * len(sets)
+    for _ in range(5):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[n] = run(sets[n])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run(sets[0])
+    for x, y in zip(sets[0], sets[1]):
+        x.copy_(y)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[1][0]) and torch.equal(out[1], want[1][1])
+
+
+@pytest.mark.parametrize("width", [50021, 131072, 300007])
+@pytest.mark.parametrize("fill", [-math.inf, "lowest", 1e4])
+def test_distill_wide_closed_columns(width, fill):
+    """Rows that several blocks hold: closed columns, one entry far above the rest, rows closed altogether."""
+    logits, teacher, index, weight = distill_inputs((4, width, 5, "f32", torch.int64), seed=55)
+    index[:] = torch.tensor([0, 7, width // 2, width - 2, width - 1], device="cuda")
+    if fill == 1e4:
+        logits[:, width // 3] = fill
+        distill_check(logits[:, :], teacher, index, 1.0, weight)
+        return
+    fill = torch.finfo(torch.float32).min if fill == "lowest" else fill
+    hide = torch.ones(width, dtype=torch.bool, device="cuda")
+    hide[index[0]] = False
+    hide[100:200] = False
+    logits[:, hide] = fill
+    distill_check(logits, teacher, index, 1.0, weight)
+    logits[2] = fill
+    loss, grad = ops.distill_top_logits_step(logits, teacher, index)
+    assert loss[[0, 1, 3]].isfinite().all() and grad[[0, 1, 3]].isfinite().all()
+    if fill == -math.inf:
+        assert loss[2].isnan() and grad[2].isnan().all()
+    else:
+        want = (teacher[2].double().softmax(0) * teacher[2].double().log_softmax(0)).sum() + math.log(width)
+        assert abs(loss[2].double() - want) < 1e-4
