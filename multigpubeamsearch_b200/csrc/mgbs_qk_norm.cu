@@ -27,7 +27,6 @@ struct QkTensor {
   const float* gain;
   int64_t xs[3], ys[3], ds[3];  // strides of x, y (dx) and dy in elements: batch, token, head
   int32_t heads;
-  int32_t pad;
 };
 struct QkArgs {
   QkTensor t[2];  // queries, keys
@@ -346,7 +345,6 @@ int qk_prepare(const MgbsQkNormArgs* a, bool bwd, QkArgs* g, bool* vec, int* ele
     t.heads = i ? a->heads_k : a->heads_q;
     const int64_t *xs = i ? a->k_stride : a->q_stride, *ys = i ? a->k_out_stride : a->q_out_stride, *ds = i ? a->dk_out_stride : a->dq_out_stride;
     for (int j = 0; j < 3; ++j) { t.xs[j] = xs[j]; t.ys[j] = ys[j]; t.ds[j] = bwd ? ds[j] : 0; }
-    t.pad = 0;
     *vec = *vec && aligned16(t.x, t.xs, *elem) && aligned16(t.y, t.ys, *elem) && (!bwd || aligned16(t.dy, t.ds, *elem));
   }
   g->phase = a->phase;

@@ -4,16 +4,17 @@
 //   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij do_i
 //   dtable[b, h] = sum over sequences and pairs with bucket(j - i) = b of dS_ij
 //
-// The products run on the warp-level matrix instruction (m16n8k16, 16-bit operands, float32 accumulators): with heads
-// of 32 and 64 elements the exponentials and the float32 work on the score matrix cost as much issue time as the
-// products, and for the scorer's 54 tokens the bytes of q, k, v bound the pass.  Scores, softmax statistics, delta and
-// all sums stay in float32; P and dS are rounded to the operands' 16 bits only as inputs of the next product (the
-// rounding errors of a row's terms are independent, so a sum over a row keeps more than the output's own 16 bits).
+// The forward of long sequences is in the file of the tcgen05 form; the rest is here, on the warp-level matrix instruction
+// (m16n8k16, 16-bit operands, float32 accumulators).  For the scorer's 54 tokens the bytes of q, k, v bound the pass and
+// not the products: 749 us at 32768 x 54 tokens, 8 heads of 32, against 560 us for the bytes.  Scores, softmax
+// statistics, delta and all sums stay in float32; P and dS are rounded to the operands' 16 bits only as inputs of the next
+// product (the rounding errors of a row's terms are independent, so a sum over a row keeps more than the output's own 16
+// bits).
 //
 // Sequences of up to 64 tokens are one tile: a warp owns 16 query rows of one (sequence, head), a group of warps walks
 // over the sequences of ONE head, so that the head's biases live in registers as the products' initial accumulators,
 // and the backward pass sums dS over its sequences in registers (one add per score) and bins it by bucket once at its
-// end.  Longer sequences go tile by tile with a running maximum and sum.  Every sum is in a fixed order: no atomics.
+// end.  Longer sequences go in tiles of 64 x 64 with a running maximum and sum.  Every sum is in a fixed order: no atomics.
 
 #include <math.h>
 
@@ -1107,16 +1108,18 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, f
   return rc ? rc : finish_table<T>(g, sums, REL_CHUNKS, REL_CHUNKS, 1, dtable, st);
 }
 
-#ifndef REL_TC
-#define REL_TC 128
-#endif
+// Sequences from here on go forward on tcgen05: 442368 tokens, 8 heads, in sequences of T
+//   heads of 64:  T = 65: 1404 us against 1580 us, 128: 707 against 797, 129: 1584 against 1553, 256: 863 against 1267
+//   heads of 32:  T = 65: 1380 against 947, 256: 785 against 712, 320: 1030 against 841, 384: 932 against 971, 512: 1057
+//                 against 1233 (half the products per exponential, so that a block's fixed costs weigh more)
+template <int D> constexpr int rel_tc_tokens() { return D == 64 ? 65 : 321; }
 template <typename T> struct Type;
 template <> struct Type<__nv_bfloat16> { static constexpr int DT = MGBS_DT_BF16; };
 template <> struct Type<__half> { static constexpr int DT = MGBS_DT_F16; };
 template <typename T, int D> int forward_as(const RelArgs& g, cudaStream_t st) {
   // with statistics asked for, the form whose backward reads them
   if (g.tokens > REL_SHORT || (g.stats && g.heads != g.heads_kv)) {
-    if (g.tokens > REL_TC && rel_attention_tc_fits(g)) return rel_attention_tc(g, Type<T>::DT, D, st);
+    if (g.tokens >= rel_tc_tokens<D>() && rel_attention_tc_fits(g)) return rel_attention_tc(g, Type<T>::DT, D, st);
     return run_tiles<T, D>(g, st);
   }
   const int strips = short_strips(g.tokens);
