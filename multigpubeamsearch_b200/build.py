@@ -19,8 +19,9 @@ CSRC = PKG / "csrc"
 ROOT = PKG.parent
 LIB = PKG / "libmgbs_b200.so"
 SOURCES = ["mgbs_step.cu", "mgbs_engine.cu", "mgbs_scorer.cu", "mgbs_transformer.cu", "mgbs_nvfp4.cu",
-           "mgbs_qk_norm.cu", "mgbs_rel_attention.cu", "mgbs_rel_attention_tc.cu", "mgbs_distill.cu"]
-HEADERS = ["mgbs_device.cuh", "mgbs_internal.cuh", "mgbs_tc.cuh", "mgbs_nvfp4.cuh", "mgbs_operators.cuh", "mgbs_counted.cuh", "mgbs_rel_attention.cuh"]
+           "mgbs_qk_norm.cu", "mgbs_rel_attention.cu", "mgbs_rel_attention_tc.cu", "mgbs_rel_attention_tc_bwd.cu", "mgbs_distill.cu"]
+HEADERS = ["mgbs_device.cuh", "mgbs_internal.cuh", "mgbs_tc.cuh", "mgbs_nvfp4.cuh", "mgbs_operators.cuh", "mgbs_counted.cuh", "mgbs_rel_attention.cuh",
+           "mgbs_rel_attention_tc.cuh"]
 
 
 def _nccl_include() -> str:

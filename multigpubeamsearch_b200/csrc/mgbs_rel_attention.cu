@@ -822,15 +822,6 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
   }
 }
 
-__device__ __forceinline__ void rel_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float4 get_remote(const float* local, int rank) {  // the same address in block `rank` of the cluster
-  uint32_t at;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
-}
-
 // dk and dv: a block owns 64 keys and walks over queries, in transposed products (keys as rows), so that P^T and dS^T come
 // out of the accumulators as operands of the next product.  The query heads that share the keys are spread over the
 // `ranks` blocks of a cluster, whose sums are added through distributed shared memory at the end, in a fixed order: one
@@ -1073,7 +1064,7 @@ template <typename T, int D> int run_tiles(const RelArgs& g, cudaStream_t st) {
   return (int)cudaGetLastError();
 }
 
-template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, float* sums, cudaStream_t st) {
+template <typename T, int D> int run_tiles_bwd(const RelArgs& g, cudaStream_t st) {
   static std::atomic<uint64_t> raised_q{0}, raised_kv{0};
   const int fixed_q = dq_front<D>() + 4 * tile_bytes<D>(), fixed_kv = 6 * tile_bytes<D>();
   int rc = raise_smem(k_rel_tiles_dq<T, D>, fixed_q + 2 * rel_bias_floats(1024) * 4, raised_q);
@@ -1085,9 +1076,7 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, f
   k_rel_tiles_dq<T, D><<<(unsigned)blocks, REL_THREADS, fixed_q + 2 * rel_bias_floats(g.reach) * 4, st>>>(g, tiles);
   rc = (int)cudaGetLastError();
   if (rc) return rc;
-  int ranks = 1;  // the most blocks that the shared heads can be dealt to
-  for (int r = 2; r <= 8; ++r)
-    if (g.heads / g.heads_kv % r == 0) ranks = r;
+  const int ranks = rel_ranks(g);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * g.heads_kv * ranks));
   cfg.blockDim = dim3(REL_THREADS);
@@ -1099,12 +1088,16 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, f
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  rc = (int)cudaLaunchKernelEx(&cfg, k_rel_tiles_dkv<T, D>, g, tiles, ranks);
-  if (rc) return rc;
+  return (int)cudaLaunchKernelEx(&cfg, k_rel_tiles_dkv<T, D>, g, tiles, ranks);
+}
+
+// The table's gradient from a row of sums per head, sequence and tile of queries.
+template <typename T> int sum_table(const RelArgs& g, int tile, void* dtable, float* sums, cudaStream_t st) {
+  const int64_t rows = (int64_t)g.batch * ((g.tokens + tile - 1) / tile);
   if (rows <= 256) return finish_table<T>(g, g.partial, rows, rows, 1, dtable, st);
   const int64_t chunk = (rows + REL_CHUNKS - 1) / REL_CHUNKS;
   k_rel_table_sum<float><<<dim3(g.heads, REL_CHUNKS), 256, 0, st>>>(g.partial, rows, chunk, rows, 1, g.buckets, sums, false);
-  rc = (int)cudaGetLastError();
+  const int rc = (int)cudaGetLastError();
   return rc ? rc : finish_table<T>(g, sums, REL_CHUNKS, REL_CHUNKS, 1, dtable, st);
 }
 
@@ -1113,6 +1106,10 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, void* dtable, f
 //   heads of 32:  T = 65: 1380 against 947, 256: 785 against 712, 320: 1030 against 841, 384: 932 against 971, 512: 1057
 //                 against 1233 (half the products per exponential, so that a block's fixed costs weigh more)
 template <int D> constexpr int rel_tc_tokens() { return D == 64 ? 65 : 321; }
+#ifndef TCB
+#define TCB 65
+#endif
+template <int D> constexpr int rel_tc_backward_tokens() { return TCB; }
 template <typename T> struct Type;
 template <> struct Type<__nv_bfloat16> { static constexpr int DT = MGBS_DT_BF16; };
 template <> struct Type<__half> { static constexpr int DT = MGBS_DT_F16; };
@@ -1126,7 +1123,11 @@ template <typename T, int D> int forward_as(const RelArgs& g, cudaStream_t st) {
   return strips == 1 ? run_short<T, D, 1>(g, st) : strips == 2 ? run_short<T, D, 2>(g, st) : strips == 3 ? run_short<T, D, 3>(g, st) : run_short<T, D, 4>(g, st);
 }
 template <typename T, int D> int backward_as(const RelArgs& g, bool is_short, void* dtable, float* sums, cudaStream_t st) {
-  if (!is_short) return run_tiles_bwd<T, D>(g, dtable, sums, st);
+  if (!is_short) {
+    const bool tc = g.tokens >= rel_tc_backward_tokens<D>() && rel_attention_tc_backward_fits(g);
+    const int rc = tc ? rel_attention_tc_backward(g, Type<T>::DT, D, st) : run_tiles_bwd<T, D>(g, st);
+    return rc ? rc : sum_table<T>(g, tc ? REL_TC_ROWS : TILE, dtable, sums, st);
+  }
   const int strips = short_strips(g.tokens);
   return strips == 1 ? run_short_bwd<T, D, 1>(g, dtable, st) : strips == 2 ? run_short_bwd<T, D, 2>(g, dtable, st)
          : strips == 3 ? run_short_bwd<T, D, 3>(g, dtable, st) : run_short_bwd<T, D, 4>(g, dtable, st);

@@ -40,6 +40,7 @@ __device__ __forceinline__ float scaled_bias(float x, float f, float most) {
 // bias * log2(e) by offset: bt[off + side] for offsets of at most `side`, by `threads` threads.  A tile of n x n that is not
 // beyond the reach has offsets below reach + 2 n.
 template <typename T> __device__ __forceinline__ void fill_bias(const RelArgs& g, int h, float* bt, int side, int thread, int threads) {
+#pragma unroll 4
   for (int i = thread; i < 2 * side + 1; i += threads) bt[i] = scaled_bias(rel_bias<T>(g, i - side, h), kLog2e, REL_BIG);
 }
 
@@ -55,8 +56,28 @@ __device__ __forceinline__ Where rel_where(int64_t n, int tiles, int heads, int 
   return {in / members, (int)(unit % heads), (int)(unit / heads)};
 }
 
+__device__ __forceinline__ void rel_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 get_remote(const float* local, int rank) {  // the same address in block `rank` of the cluster
+  uint32_t at;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+inline int rel_ranks(const RelArgs& g) {  // the most blocks of a cluster that the heads of one key head can be dealt to
+  int ranks = 1;
+  for (int r = 2; r <= 8; ++r)
+    if (g.heads / g.heads_kv % r == 0) ranks = r;
+  return ranks;
+}
+
+constexpr int REL_TC_ROWS = 128;  // rows of a tile of the tcgen05 forms
+
 // The forward on the fifth-generation tensor cores, and whether TMA can describe the strides (it knows no stride of 0).
 bool rel_attention_tc_fits(const RelArgs& g);
 int rel_attention_tc(const RelArgs& g, int dtype, int head_dim, cudaStream_t st);
+// dq, dk, dv, delta and the table's partial sums, where the same holds for dout's strides.
+bool rel_attention_tc_backward_fits(const RelArgs& g);
+int rel_attention_tc_backward(const RelArgs& g, int dtype, int head_dim, cudaStream_t st);
 
 }  // namespace mgbs

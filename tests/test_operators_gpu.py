@@ -6,6 +6,9 @@ is float32 with sums of at most a few hundred dependent terms, covered by SLACK 
 (2^-24 per operation, exponentials of arguments up to 2^8 whose own error is 2^-24 of the argument)."""
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -902,6 +905,25 @@ def test_long_attention_on_streams_and_replayed():
     torch.cuda.synchronize()
     for a, b in zip(want[2:], outs):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_long_attention_first_in_a_process():
+    """Forward and backward as a process's first calls, the backward on autograd's thread; then on threads of its own."""
+    code = """
+import threading, torch
+from multigpubeamsearch_b200 import operators as ops
+x = torch.randn(2, 200, 3, 64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+t, plan = torch.zeros(32, 1, device="cuda", dtype=torch.bfloat16), ops.RelativeBuckets(device="cuda")
+step = lambda: torch.autograd.grad(ops.relative_attention(x[:, :, :1], x[:, :, 1:2], x[:, :, 2:], t, plan), x, torch.ones_like(x[:, :, :1]))[0]
+first, later = step(), []
+threads = [threading.Thread(target=lambda: later.append(step())) for _ in range(3)]
+[n.start() for n in threads]; [n.join() for n in threads]
+torch.cuda.synchronize()
+assert len(later) == 3 and first.isfinite().all() and all(torch.equal(first, y) for y in later)
+"""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_distill_wide_on_streams_and_replayed():
