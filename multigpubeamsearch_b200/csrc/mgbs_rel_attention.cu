@@ -4,8 +4,8 @@
 //   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij do_i
 //   dtable[b, h] = sum over sequences and pairs with bucket(j - i) = b of dS_ij
 //
-// The forward of long sequences is in the file of the tcgen05 form; the rest is here, on the warp-level matrix instruction
-// (m16n8k16, 16-bit operands, float32 accumulators).  For the scorer's 54 tokens the bytes of q, k, v bound the pass and
+// Long sequences are in the files of the tcgen05 forms; the rest is here, on the warp-level matrix instruction (m16n8k16,
+// 16-bit operands, float32 accumulators): short sequences, and strides that TMA cannot describe.  For the scorer's 54 tokens the bytes of q, k, v bound the pass and
 // not the products: 749 us at 32768 x 54 tokens, 8 heads of 32, against 560 us for the bytes.  Scores, softmax
 // statistics, delta and all sums stay in float32; P and dS are rounded to the operands' 16 bits only as inputs of the next
 // product (the rounding errors of a row's terms are independent, so a sum over a row keeps more than the output's own 16
@@ -636,7 +636,8 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles(const __grid_constant
 
 // dq, delta and the table's gradient: a block owns 64 queries and walks over the keys.  Bound by the latency of a warp's
 // chain of products and exponentials, with 12 warps on a multiprocessor: 107 us at 6 x 1501 causal tokens, 8 heads of 64
-// over 2 (143 us before the longest tiles of all heads started first and dS moved into the place of q and dout).
+// over 2 (143 us before the longest tiles of all heads started first and dS moved into the place of q and dout; the
+// tcgen05 form takes 57 us).
 constexpr int DS_PITCH = TILE + 1;
 template <int D> __host__ __device__ constexpr int dq_front() {  // q and dout, whose place a tile of dS takes
   return 2 * tile_bytes<D>() > TILE * DS_PITCH * 4 ? 2 * tile_bytes<D>() : TILE * DS_PITCH * 4;
@@ -826,7 +827,7 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
 // out of the accumulators as operands of the next product.  The query heads that share the keys are spread over the
 // `ranks` blocks of a cluster, whose sums are added through distributed shared memory at the end, in a fixed order: one
 // block for all heads left most of the device idle (210 us against 119 us at 6 x 1501 causal tokens, 8 heads over 2; 102 us with the longest tiles
-// first).
+// first; the tcgen05 form takes 56 us).
 template <typename T, int D>
 __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(const __grid_constant__ RelArgs g, int tiles, int ranks) {
   constexpr int PITCH = RelTile<D>::PITCH, MAT = TILE * PITCH;
@@ -1106,10 +1107,10 @@ template <typename T> int sum_table(const RelArgs& g, int tile, void* dtable, fl
 //   heads of 32:  T = 65: 1380 against 947, 256: 785 against 712, 320: 1030 against 841, 384: 932 against 971, 512: 1057
 //                 against 1233 (half the products per exponential, so that a block's fixed costs weigh more)
 template <int D> constexpr int rel_tc_tokens() { return D == 64 ? 65 : 321; }
-#ifndef TCB
-#define TCB 65
-#endif
-template <int D> constexpr int rel_tc_backward_tokens() { return TCB; }
+// The backward is on tcgen05 from there on for every head size: 221184 tokens, 8 heads of 64 in sequences of T = 65: 1844 us
+// against 3361 us, 192: 1556 against 2157, 1000: 3303 against 7826; heads of 32: 65: 1636 against 2446, 192: 1341 against
+// 1479; 33 tokens, 8 heads of 64 over 2: 3214 against 2931.
+constexpr int REL_TC_BACKWARD_TOKENS = 65;
 template <typename T> struct Type;
 template <> struct Type<__nv_bfloat16> { static constexpr int DT = MGBS_DT_BF16; };
 template <> struct Type<__half> { static constexpr int DT = MGBS_DT_F16; };
@@ -1124,7 +1125,7 @@ template <typename T, int D> int forward_as(const RelArgs& g, cudaStream_t st) {
 }
 template <typename T, int D> int backward_as(const RelArgs& g, bool is_short, void* dtable, float* sums, cudaStream_t st) {
   if (!is_short) {
-    const bool tc = g.tokens >= rel_tc_backward_tokens<D>() && rel_attention_tc_backward_fits(g);
+    const bool tc = g.tokens >= REL_TC_BACKWARD_TOKENS && rel_attention_tc_backward_fits(g);
     const int rc = tc ? rel_attention_tc_backward(g, Type<T>::DT, D, st) : run_tiles_bwd<T, D>(g, st);
     return rc ? rc : sum_table<T>(g, tc ? REL_TC_ROWS : TILE, dtable, sums, st);
   }

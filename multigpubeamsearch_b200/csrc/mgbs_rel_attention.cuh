@@ -76,7 +76,7 @@ constexpr int REL_TC_ROWS = 128;  // rows of a tile of the tcgen05 forms
 // The forward on the fifth-generation tensor cores, and whether TMA can describe the strides (it knows no stride of 0).
 bool rel_attention_tc_fits(const RelArgs& g);
 int rel_attention_tc(const RelArgs& g, int dtype, int head_dim, cudaStream_t st);
-// dq, dk, dv, delta and the table's partial sums, where the same holds for dout's strides.
+// Its backward: dq, dk, dv, delta and the table's partial sums; the same for dout's strides.
 bool rel_attention_tc_backward_fits(const RelArgs& g);
 int rel_attention_tc_backward(const RelArgs& g, int dtype, int head_dim, cudaStream_t st);
 

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
                                                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RelArgs g, int tiles) {
   constexpr int Q_BYTES = TC_Q * D * 2, K_BYTES = TC_K * D * 2;
   extern __shared__ __align__(1024) uint8_t tc_smem[];
-  __shared__ __align__(8) uint64_t bars[4 * TC_STAGES + 8];
+  __shared__ __align__(8) uint64_t bars[4 * TC_STAGES + 9];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   const Where w0 = rel_where(blockIdx.x, tiles, g.heads, g.batch);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
   float* bt = reinterpret_cast<float*>(v_ptr + TC_STAGES * K_BYTES);
   const uint32_t bar = smem_u32(bars);
   const uint32_t k_full = bar, v_full = bar + 8 * TC_STAGES, k_free = bar + 16 * TC_STAGES, v_free = bar + 24 * TC_STAGES;
-  const uint32_t s_full = bar + 32 * TC_STAGES, p_full = s_full + 16, o_done = s_full + 32, q_full = s_full + 48, v_fixed = s_full + 56;
+  const uint32_t s_full = bar + 32 * TC_STAGES, p_full = s_full + 16, o_done = s_full + 32, q_full = s_full + 48, v_fixed = s_full + 56, drained = s_full + 64;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4 * TC_STAGES; ++i) mbar_init(bar + i * 8, 1);
     for (int i = 0; i < 2; ++i) {
@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
     }
     mbar_init(q_full, 1);
     mbar_init(v_fixed, 1);
+    mbar_init(drained, 1);
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -169,14 +170,22 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
     if (lane == 0) {
       mbar_expect_tx(q_full, Q_BYTES);
       tma_load_4d(q_at, &map_q, i0, head, batch, q_full);
-      for (int t = 0; t < n_tiles; ++t) {
-        const int s = t % TC_STAGES, turn = t / TC_STAGES;
+      int keys = 0, values = 0;  // tiles asked for
+      while (values < n_tiles) {
+        const int t = values, s = t % TC_STAGES, turn = t / TC_STAGES;
         if (turn > 0 && !(ok = wait(k_free + s * 8, (turn - 1) & 1, ERR_TC_FREE))) break;
         mbar_expect_tx(k_full + s * 8, K_BYTES);
         tma_load_4d(k_at + s * K_BYTES, &map_k, t * TC_K, head_kv, batch, k_full + s * 8);
+        ++keys;
         if (turn > 0 && !(ok = wait(v_free + s * 8, (turn - 1) & 1, ERR_TC_FREE))) break;
         mbar_expect_tx(v_full + s * 8, K_BYTES);
         tma_load_4d(v_at + s * K_BYTES, &map_v, t * TC_K, head_kv, batch, v_full + s * 8);
+        ++values;
+      }
+      if (!ok) {  // what has been asked for comes before the block ends
+        tc_settle(q_full, 0);
+        for (int t = max(0, keys - TC_STAGES); t < keys; ++t) tc_settle(k_full + t % TC_STAGES * 8, (t / TC_STAGES) & 1);
+        for (int t = max(0, values - TC_STAGES); t < values; ++t) tc_settle(v_full + t % TC_STAGES * 8, (t / TC_STAGES) & 1);
       }
     }
     ok = __all_sync(0xffffffffu, ok);
@@ -227,6 +236,11 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
       }
       if (t + 2 < n_tiles) ok = score(t + 2);  // into the buffer that this tile's softmax has left
     }
+    if (!ok) {  // products on their way end before the tensor memory is given back
+      if (elect_one()) tc_commit(drained);
+      __syncwarp();
+      tc_settle(drained, 0);
+    }
     __syncwarp();
   } else {
     const int row = i0 + threadIdx.x;
@@ -241,7 +255,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
       const TcTile where{far, edge, j0, row, len, g.causal, far > 0 ? bt[2 * side] : bt[0], bt + j0 - row + side};
       const uint32_t scores = mine + (t & 1) * TC_K, to = mine + TC_P_COL + (t & 1) * 32;
       // S(t) was issued behind O += P(t - 2) V(t - 2), so that P's buffer is free too
-      ok = wait(s_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_S);
+      ok = __all_sync(0xffffffffu, wait(s_full + (t & 1) * 8, (t / 2) & 1, ERR_TC_S));
       if (!ok) break;
       tc_fence_after();
       float sum = 0.f;
@@ -257,7 +271,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
         tc_wait_st();
         const float top = fmaxf(m, tc_maximum(scores, where, sl2));
         if (t > 0) {
-          ok = wait(o_done + ((t - 1) & 1) * 8, ((t - 1) / 2) & 1, ERR_TC_O);  // O is still
+          ok = __all_sync(0xffffffffu, wait(o_done + ((t - 1) & 1) * 8, ((t - 1) / 2) & 1, ERR_TC_O));  // O is still
           if (!ok) break;
           tc_fence_after();
           const float f = top == -INFINITY ? 1.f : fast_exp2(m - top);
@@ -281,7 +295,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc(const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + (t & 1) * 8);
     }
-    if (ok) ok = wait(o_done + ((n_tiles - 1) & 1) * 8, ((n_tiles - 1) / 2) & 1, ERR_TC_O);
+    if (ok) ok = __all_sync(0xffffffffu, wait(o_done + ((n_tiles - 1) & 1) * 8, ((n_tiles - 1) / 2) & 1, ERR_TC_O));
     tc_fence_after();
     const bool some = row < len && l != 0.f;
     const float inv = some ? 1.f / l : 0.f;
