@@ -908,13 +908,16 @@ def test_long_attention_on_streams_and_replayed():
 
 
 def test_long_attention_first_in_a_process():
-    """Forward and backward as a process's first calls, the backward on autograd's thread; then on threads of its own."""
+    """Forward and backward as a process's first calls, the backward on autograd's thread, for which torch's allocator has
+    memory at hand, so that this is its first call of the runtime; then on threads of its own."""
     code = """
 import threading, torch
 from multigpubeamsearch_b200 import operators as ops
-x = torch.randn(2, 200, 3, 64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
-t, plan = torch.zeros(32, 1, device="cuda", dtype=torch.bfloat16), ops.RelativeBuckets(device="cuda")
-step = lambda: torch.autograd.grad(ops.relative_attention(x[:, :, :1], x[:, :, 1:2], x[:, :, 2:], t, plan), x, torch.ones_like(x[:, :, :1]))[0]
+leaves = [torch.randn(*s, device="cuda", dtype=torch.bfloat16).requires_grad_(True) for s in [(2, 200, 1, 64)] * 3 + [(32, 1)]]
+plan, ones = ops.RelativeBuckets(device="cuda"), torch.ones(2, 200, 1, 64, device="cuda", dtype=torch.bfloat16)
+room = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in (1 << 26, 1 << 20, 1 << 20, 1 << 19, 1 << 19)]
+del room
+step = lambda: torch.autograd.grad(ops.relative_attention(*leaves, plan), leaves, ones)[0]
 first, later = step(), []
 threads = [threading.Thread(target=lambda: later.append(step())) for _ in range(3)]
 [n.start() for n in threads]; [n.join() for n in threads]
