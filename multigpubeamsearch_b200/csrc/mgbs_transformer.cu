@@ -693,7 +693,6 @@ static int tf_rel_attention(const MgbsTfConfig& c, const MgbsTfLayer& L, const u
   a.num_buckets = c.rel_buckets; a.max_distance = c.rel_distance;
   a.out = c.att;
   a.scale = 0.17677669529663687f;  // 1 / sqrt(32)
-  a.error = c.err;
   return mgbs::rel_attention_counted(&a, count_dev, first, stream);
 }
 

@@ -7,7 +7,7 @@
 All three run hand-written kernels of libmgbs_b200.so and take part in autograd (first derivatives).  Wrong shapes, types
 or devices raise RuntimeError before anything is enqueued; there is no CPU fallback.  Nothing is kept between calls,
 outputs and workspaces come from torch's allocator, equal calls give equal bits, and every call may be captured in a
-CUDA graph.  TransformerValueScorer, TransformerValueNet and MLPActionScorer.distillation_loss call them.
+CUDA graph (a backward pass only while no eager autograd graph of the same leaves is alive, a rule of autograd's own).  TransformerValueScorer, TransformerValueNet and MLPActionScorer.distillation_loss call them.
 """
 
 from __future__ import annotations
@@ -286,7 +286,8 @@ def relative_bucket(offset: int, num_buckets: int, max_distance: int, causal: bo
 class RelativeBuckets:
     """Which learned bias a pair of positions takes: ``num_buckets`` buckets of key minus query, exact for near
     distances and growing by equal factors up to ``max_distance`` (see relative_bucket).  ``causal`` also hides keys
-    after their query.  Built once per model."""
+    after their query.  Built once per model.  ``error_code()`` is 0 unless a kernel of a call with these buckets gave up
+    waiting for its own copies or products, which leaves NaN in the rows concerned."""
 
     def __init__(self, num_buckets: int = 32, max_distance: int = 128, causal: bool = False, device=None):
         self.num_buckets, self.max_distance, self.causal = int(num_buckets), int(max_distance), bool(causal)
@@ -304,9 +305,14 @@ class RelativeBuckets:
         for b in range(self.num_buckets):
             start[b + 1] += start[b]
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        packed = torch.tensor(buckets + order + start, dtype=torch.int32, device=dev)
+        packed = torch.tensor(buckets + order + start + [0], dtype=torch.int32, device=dev)
         n = 2 * m + 1
-        self.map, self.order, self.start = packed[:n], packed[n:2 * n], packed[2 * n:]
+        self.map, self.order, self.start = packed[:n], packed[n:2 * n], packed[2 * n:-1]
+        self.error = packed[-1:]
+
+    def error_code(self) -> int:
+        """Waits for the calls before it."""
+        return int(self.error.item())
 
 
 def _rel_args(q, k, v, table, buckets, lengths, scale) -> MgbsRelAttentionArgs:
@@ -316,6 +322,7 @@ def _rel_args(q, k, v, table, buckets, lengths, scale) -> MgbsRelAttentionArgs:
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
     a.q, a.k, a.v, a.table = q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr()
     a.bucket_map, a.bucket_order, a.bucket_start = buckets.map.data_ptr(), buckets.order.data_ptr(), buckets.start.data_ptr()
+    a.error = buckets.error.data_ptr()
     a.num_buckets, a.max_distance, a.causal = buckets.num_buckets, buckets.max_distance, int(buckets.causal)
     if lengths is not None:
         a.lengths = lengths.data_ptr()

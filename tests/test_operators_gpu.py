@@ -727,6 +727,7 @@ LONG_CASES = [
 def test_long_attention(case):
     q, k, v, table, plan, lengths, dout = attention_inputs(case, seed=30)
     attention_check(q, k, v, table, plan, lengths, dout=dout)
+    assert plan.error_code() == 0
 
 
 @pytest.mark.parametrize("tokens,d", [(20, 32), (150, 64), (330, 32)])
