@@ -140,7 +140,7 @@ template <bool FAST> __device__ __forceinline__ void qk_angles(const QkArgs& g, 
   }
 }
 
-// Rotation coefficients of a lane's eight pairs; pairs past `half` read nothing.
+// Rotation coefficients of a lane's eight pairs; the first of them is below `half`, others past it read nothing.
 template <bool VEC> __device__ __forceinline__ void qk_read_cs(const float2* cs, int chunk, int half, float (&c)[8], float (&s)[8]) {
   if (VEC) {
     const float4* p = reinterpret_cast<const float4*>(cs + chunk * 8);
@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(QK_THREADS, BWD ? 2 : 3) k_qk_norm_rope(const 
       for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + bb[i] * bb[i];
       ss = group_sum(ss, lanes);
       const float r = rsqrtf(ss * inv_d + g.eps);
-      qk_read_cs<VEC>(cs + (live ? SHARED ? at[u] : u * g.step + tok : 0) * half, chunk, half, c, s);
+      // lanes past the head's pairs take part in its sums: with zeros, which only finite coefficients keep
+      qk_read_cs<VEC>(cs + (live ? SHARED ? at[u] : u * g.step + tok : 0) * half, chunk * 8 < half ? chunk : 0, half, c, s);
       if (!BWD) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

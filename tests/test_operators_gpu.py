@@ -167,6 +167,16 @@ def test_qk_norm_rope_backward(case):
         within(got[2 + i], dg, (40 + additions) * 2.0 ** -24 * spread + 1e-30, "dgain")
 
 
+@pytest.mark.parametrize("d", [48, 80, 96, 112, 144, 160, 176, 192, 208, 224, 240])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_qk_norm_rope_partly_used_lanes(d, dtype):
+    """Head sizes of 16-byte pieces that are no power of two: lanes of a head's group that have none of it."""
+    for b, t, h, hk, inter, where in ((65, 1, 7, 6, False, "negative"), (1, 203, 19, 3, True, "far"), (9, 54, 8, 8, False, None)):
+        case = (b, t, h, hk, d, dtype, inter, where, "packed")
+        test_qk_norm_rope_forward(case)
+        test_qk_norm_rope_backward(case)
+
+
 def test_qk_norm_rope_gradient_against_differences():
     q, k, qg, kg, _ = qk_inputs((2, 11, 3, 1, 32, "f32", False, None, "packed"))
     rotary = ops.RotaryFrequencies(32)
