@@ -9,7 +9,9 @@
 // (up to there P fits both 16-bit types, and float32 sums lose nothing): then the tile is done again from its true
 // maximum and the accumulator O, in tensor memory too, is rescaled.  So a tile takes no maximum as a rule.
 // 256 of the 512 columns and 84 KB: two blocks per SM, one's exponentials over the other's products and waits.  What
-// bounds it: the exponentials, 128 x 64 of them per tile at 16 a clock against 256 clocks of products.
+// bounds it: the exponentials, 128 x 64 of them per tile at 16 a clock against 256 clocks of products, and the blocks'
+// number (512 over 296 places): 117 us at 2 x 4096 tokens, 8 heads of 64, of which the exponentials alone are 60 and with
+// a quarter of them on the multiply-add pipe 45.
 //
 // Rows of 128 bytes (64 for heads of 32) in the swizzled layout of that width: K-major for Q and K, MN-major for V.
 // Padding past a length is zeroed in V's last tile (P = 0 must not meet a NaN there); elsewhere it only reaches scores
@@ -25,6 +27,8 @@ constexpr int TC_STAGES = 4;                        // tiles of K and of V in sh
 constexpr float TC_GROWTH = 16384.f;                // how far a row's sum over a tile may grow before its reference follows
 constexpr int TC_P_COL = 128, TC_O_COL = 192;       // columns: S at 0 and 64, P at 128 and 160, O at 192
 
+constexpr int TC_EVERY = 4;  // one pair of exponentials in so many goes to the multiply-add pipe (none 124 us, 3: 118, 5: 118, 4: 117)
+
 // A tile as a softmax thread sees it.
 struct TcTile {
   int far;  // 1 / -1: all keys beyond the reach after / before the queries, so that one bias serves
@@ -34,23 +38,13 @@ struct TcTile {
   const float* by_offset;  // bias of key j0 + j at [j]
 };
 
-// Scores of 32 keys, scaled and biased.  MODE 0: one bias; 1: by offset; 2: either, and hidden ones at -inf.
-template <int MODE> __device__ __forceinline__ void tc_scores(const TcTile& w, int c, Pair sl2, const uint32_t (&raw)[32], Pair (&s)[16]) {
-  const Pair one = pair(w.fixed, w.fixed);
-#pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    const int at = c * 32 + j;
-    const bool fix = MODE == 0 || (MODE == 2 && w.far);
-    const Pair b = fix ? one : pair(w.by_offset[at], w.by_offset[at + 1]);
-    s[j / 2] = fma2(pair(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), sl2, b);
-    if (MODE == 2) {
-      const int key = w.j0 + at;
-      float2 f = both(s[j / 2]);
-      if (key >= w.len || (w.causal && key > w.row)) f.x = -INFINITY;
-      if (key + 1 >= w.len || (w.causal && key + 1 > w.row)) f.y = -INFINITY;
-      s[j / 2] = pair(f.x, f.y);
-    }
-  }
+// Two scores of the tile, hidden ones at -inf.
+__device__ __forceinline__ Pair tc_hide(const TcTile& w, int at, Pair s) {
+  const int key = w.j0 + at;
+  float2 f = both(s);
+  if (key >= w.len || (w.causal && key > w.row)) f.x = -INFINITY;
+  if (key + 1 >= w.len || (w.causal && key + 1 > w.row)) f.y = -INFINITY;
+  return pair(f.x, f.y);
 }
 
 // A row's exact maximum over the tile.
@@ -59,40 +53,61 @@ static __device__ __noinline__ float tc_maximum(uint32_t scores, TcTile w, Pair 
 #pragma unroll 1
   for (int c = 0; c < TC_K / 32; ++c) {
     uint32_t raw[32];
-    Pair s[16];
     tc_ld32(scores + c * 32, raw);
     tc_wait_ld();
-    tc_scores<2>(w, c, sl2, raw, s);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float2 f = both(s[j]);
+    for (int j = 0; j < 32; j += 2) {
+      const int at = c * 32 + j;
+      const Pair b = w.far ? pair(w.fixed, w.fixed) : pair(w.by_offset[at], w.by_offset[at + 1]);
+      const float2 f = both(tc_hide(w, at, fma2(pair(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), sl2, b)));
       top = fmaxf(top, fmaxf(f.x, f.y));
     }
   }
   return top;
 }
 
+// 2^x on the multiply-add pipe, for x up to 127: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with the least
+// largest relative error (2^-18.5, by exchange of its extreme points), n added to the exponent.  From -125 down the result
+// stays 2^-125 or so, -inf included.
+__device__ __forceinline__ Pair exp2_fma(Pair x) {
+  float2 f = both(x);
+  x = pair(fmaxf(f.x, -125.f), fmaxf(f.y, -125.f));
+  const Pair round = pair(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
+  const Pair t = add2(x, round), n = add2(t, pair(-12582912.f, -12582912.f));
+  const Pair r = fma2(n, pair(-1.f, -1.f), x);
+  Pair y = fma2(r, pair(9.57010186330317e-3f, 9.57010186330317e-3f), pair(5.591786034055708e-2f, 5.591786034055708e-2f));
+  y = fma2(r, y, pair(0.2402474483148465f, 0.2402474483148465f));
+  y = fma2(r, y, pair(0.693121814743091f, 0.693121814743091f));
+  y = fma2(r, y, pair(0.9999992614416005f, 0.9999992614416005f));
+  f = both(y);
+  const float2 e = both(t);
+  return pair(__int_as_float(__float_as_int(f.x) + (__float_as_int(e.x) << 23)), __int_as_float(__float_as_int(f.y) + (__float_as_int(e.y) << 23)));
+}
+
 // P of the tile relative to `base` into tensor memory; returns the row's sum.
 template <typename T, int MODE> __device__ __forceinline__ float tc_write_p(uint32_t scores, uint32_t to, const TcTile& w, Pair sl2, float base) {
-  const Pair minus = pair(-base, -base);
+  const Pair minus = pair(-base, -base), one = pair(w.fixed, w.fixed);
   Pair sum = pair(0.f, 0.f);
-  uint32_t raw[2][32];
-  tc_ld32(scores, raw[0]);
-  tc_ld32(scores + 32, raw[1]);
-  tc_wait_ld();
+  uint32_t raw[2][16];
+  tc_ld16(scores, raw[0]);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    Pair s[16];
-    tc_scores<MODE>(w, c, sl2, raw[c], s);
-    uint32_t p[16];
+  for (int i = 0; i < TC_K / 16; ++i) {
+    tc_wait_ld();
+    if (i + 1 < TC_K / 16) tc_ld16(scores + (i + 1) * 16, raw[(i + 1) & 1]);  // the next columns come while these are worked on
+    uint32_t p[8];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const Pair e = exp2_2(add2(s[j], minus));
+    for (int j = 0; j < 8; ++j) {
+      const int at = i * 16 + 2 * j;
+      const bool fix = MODE == 0 || (MODE == 2 && w.far);
+      const Pair b = fix ? one : pair(w.by_offset[at], w.by_offset[at + 1]);
+      Pair s = fma2(pair(__uint_as_float(raw[i & 1][2 * j]), __uint_as_float(raw[i & 1][2 * j + 1])), sl2, b);
+      if (MODE == 2) s = tc_hide(w, at, s);
+      const Pair x = add2(s, minus), e = MODE != 2 && j % TC_EVERY == TC_EVERY - 1 ? exp2_fma(x) : exp2_2(x);
       sum = add2(sum, e);
       const float2 f = both(e);
       p[j] = pack2<T>(f.x, f.y);
     }
-    tc_st16(to + c * 16, p);
+    tc_st8(to + i * 8, p);
   }
   const float2 f = both(sum);
   return f.x + f.y;
