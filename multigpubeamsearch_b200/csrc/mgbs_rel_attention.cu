@@ -1103,9 +1103,9 @@ template <typename T> int sum_table(const RelArgs& g, int tile, void* dtable, fl
 }
 
 // Sequences from here on go forward on tcgen05: 442368 tokens, 8 heads, in sequences of T
-//   heads of 64:  T = 65: 1404 us against 1580 us, 128: 707 against 797, 129: 1584 against 1553, 256: 863 against 1267
-//   heads of 32:  T = 65: 1380 against 947, 256: 785 against 712, 320: 1030 against 841, 384: 932 against 971, 512: 1057
-//                 against 1233 (half the products per exponential, so that a block's fixed costs weigh more)
+//   heads of 64:  T = 65: 1419 us against 1580 us, 256: 868 against 1267, 512: 1158 against 2220
+//   heads of 32:  T = 65: 1355 against 947, 256: 785 against 712, 384: 932 against 972, 512: 1056 against 1233 (half the
+//                 products per exponential, so that a block's fixed costs weigh more)
 template <int D> constexpr int rel_tc_tokens() { return D == 64 ? 65 : 321; }
 // The backward is on tcgen05 from there on for every head size: 221184 tokens, 8 heads of 64 in sequences of T = 65: 1844 us
 // against 3361 us, 192: 1556 against 2157, 1000: 3303 against 7826; heads of 32: 65: 1636 against 2446, 192: 1341 against

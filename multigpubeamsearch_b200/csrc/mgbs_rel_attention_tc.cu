@@ -10,7 +10,7 @@
 // maximum and the accumulator O, in tensor memory too, is rescaled.  So a tile takes no maximum as a rule.
 // 256 of the 512 columns and 84 KB: two blocks per SM, one's exponentials over the other's products and waits.  What
 // bounds it: the exponentials, 128 x 64 of them per tile at 16 a clock against 256 clocks of products, and the blocks'
-// number (512 over 296 places): 117 us at 2 x 4096 tokens, 8 heads of 64, of which the exponentials alone are 60 and with
+// number (512 over 296 places): 115 us at 2 x 4096 tokens, 8 heads of 64, of which the exponentials alone are 60 and with
 // a quarter of them on the multiply-add pipe 45.
 //
 // Rows of 128 bytes (64 for heads of 32) in the swizzled layout of that width: K-major for Q and K, MN-major for V.
@@ -27,7 +27,8 @@ constexpr int TC_STAGES = 4;                        // tiles of K and of V in sh
 constexpr float TC_GROWTH = 16384.f;                // how far a row's sum over a tile may grow before its reference follows
 constexpr int TC_P_COL = 128, TC_O_COL = 192;       // columns: S at 0 and 64, P at 128 and 160, O at 192
 
-constexpr int TC_EVERY = 4;  // one pair of exponentials in so many goes to the multiply-add pipe (none 124 us, 3: 118, 5: 118, 4: 117)
+constexpr int TC_EVERY = 4;  // one pair of exponentials in so many goes to the multiply-add pipe (none 124 us,
+                             // 3: 118, 5: 118, 4: 117 at 2 x 4096 tokens) where one bias serves a tile
 
 // A tile as a softmax thread sees it.
 struct TcTile {
@@ -88,26 +89,40 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
 template <typename T, int MODE> __device__ __forceinline__ float tc_write_p(uint32_t scores, uint32_t to, const TcTile& w, Pair sl2, float base) {
   const Pair minus = pair(-base, -base), one = pair(w.fixed, w.fixed);
   Pair sum = pair(0.f, 0.f);
-  uint32_t raw[2][16];
-  tc_ld16(scores, raw[0]);
+  auto two = [&](int at, uint32_t lo, uint32_t hi) {  // P of columns at and at + 1
+    const bool fix = MODE == 0 || (MODE == 2 && w.far);
+    Pair s = fma2(pair(__uint_as_float(lo), __uint_as_float(hi)), sl2, fix ? one : pair(w.by_offset[at], w.by_offset[at + 1]));
+    if (MODE == 2) s = tc_hide(w, at, s);
+    const Pair x = add2(s, minus), e = MODE == 0 && at / 2 % TC_EVERY == TC_EVERY - 1 ? exp2_fma(x) : exp2_2(x);
+    sum = add2(sum, e);
+    const float2 f = both(e);
+    return pack2<T>(f.x, f.y);
+  };
+  if (MODE == 0) {  // the next 16 columns come while these are worked on
+    uint32_t raw[2][16];
+    tc_ld16(scores, raw[0]);
 #pragma unroll
-  for (int i = 0; i < TC_K / 16; ++i) {
-    tc_wait_ld();
-    if (i + 1 < TC_K / 16) tc_ld16(scores + (i + 1) * 16, raw[(i + 1) & 1]);  // the next columns come while these are worked on
-    uint32_t p[8];
+    for (int i = 0; i < TC_K / 16; ++i) {
+      tc_wait_ld();
+      if (i + 1 < TC_K / 16) tc_ld16(scores + (i + 1) * 16, raw[(i + 1) & 1]);
+      uint32_t p[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = i * 16 + 2 * j;
-      const bool fix = MODE == 0 || (MODE == 2 && w.far);
-      const Pair b = fix ? one : pair(w.by_offset[at], w.by_offset[at + 1]);
-      Pair s = fma2(pair(__uint_as_float(raw[i & 1][2 * j]), __uint_as_float(raw[i & 1][2 * j + 1])), sl2, b);
-      if (MODE == 2) s = tc_hide(w, at, s);
-      const Pair x = add2(s, minus), e = MODE != 2 && j % TC_EVERY == TC_EVERY - 1 ? exp2_fma(x) : exp2_2(x);
-      sum = add2(sum, e);
-      const float2 f = both(e);
-      p[j] = pack2<T>(f.x, f.y);
+      for (int j = 0; j < 8; ++j) p[j] = two(i * 16 + 2 * j, raw[i & 1][2 * j], raw[i & 1][2 * j + 1]);
+      tc_st8(to + i * 8, p);
     }
-    tc_st8(to + i * 8, p);
+  } else {  // with biases to load as well, all at once is the faster: 8 heads of 64, 442368 tokens in sequences
+           // of 512: 1158 us against 1204 us
+    uint32_t raw[2][32];
+    tc_ld32(scores, raw[0]);
+    tc_ld32(scores + 32, raw[1]);
+    tc_wait_ld();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint32_t p[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) p[j] = two(c * 32 + 2 * j, raw[c][2 * j], raw[c][2 * j + 1]);
+      tc_st16(to + c * 16, p);
+    }
   }
   const float2 f = both(sum);
   return f.x + f.y;
