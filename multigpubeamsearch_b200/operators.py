@@ -376,7 +376,9 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     heads]: bfloat16 or float16 (one type), head_dim 32 or 64, heads a multiple of the key heads.  Any strides (a copy
     is made only where rows do not lie on 16-byte boundaries).  ``lengths`` (int32 [batch]): tokens of a sequence from
     its length on are padding: never read, their outputs and gradients are 0.  ``scale``: head_dim ** -0.5 by default.
-    A row whose biases leave no key (all -inf) gives 0.  Differentiable in q, k, v and table."""
+    A row whose biases leave no key (all -inf) gives 0.  Differentiable in q, k, v and table; P and the scores' gradients
+    P (dP - delta) are rounded to the inputs' type on the way, so with float16 a loss scale has to keep the latter below
+    65504."""
     what, dtype, device = "relative_attention", q.dtype, q.device
     if not q.is_cuda or q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         _refuse(what, "q, k and v must be [batch, tokens, heads, head_dim] CUDA tensors")
