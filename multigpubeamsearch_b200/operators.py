@@ -115,6 +115,16 @@ def _refuse(what: str, why: str):
     raise RuntimeError(f"{what}: {why}")
 
 
+def _once(backward):
+    """once_differentiable where a graph of the gradient is being built; without its five microseconds elsewhere."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 def _same_device(what: str, device: torch.device, *tensors) -> None:
     for t in tensors:
         if t is not None and t.device != device:
@@ -204,7 +214,7 @@ class _QkNormRope(torch.autograd.Function):
         return _qk_forward(q, k, q_gain, k_gain, rotary, positions, eps, interleaved)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dq_out, dk_out):
         q, k, q_gain, k_gain, positions = ctx.saved_tensors
         lib = _load()
@@ -351,14 +361,14 @@ class _RelativeAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         q, k, v, table, lengths, out, stats = ctx.saved_tensors
         lib = _load()
         a = _rel_args(q, k, v, table, ctx.buckets, lengths, ctx.scale)
         dout = _aligned(dout)
         dq, dk, dv, dtable = _dense(q), _dense(k), _dense(v), _dense(table)
-        work = torch.empty((max(16, lib.mgbs_rel_attention_backward_workspace(C.byref(a))),), dtype=torch.uint8, device=q.device)
+        work = table.new_empty(max(16, lib.mgbs_rel_attention_backward_workspace(C.byref(a))) // 2)  # 16-bit elements
         a.dout_stride[:] = _strides(dout)
         a.out, a.dout = out.data_ptr(), dout.data_ptr()
         if stats is not None:
@@ -460,7 +470,7 @@ class _DistillTopLogits(torch.autograd.Function):
         return _distill_run("distill_top_logits", logits, teacher, index, temperature, None, False)[0]
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dloss):
         logits, teacher, index = ctx.saved_tensors
         weight = dloss.to(torch.float32).contiguous()

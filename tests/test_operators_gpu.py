@@ -873,6 +873,23 @@ def test_distill_offsets_past_32_bits():
         del logits, loss, grad
 
 
+def test_second_derivatives_are_refused():
+    """With a graph of the gradient the first derivative is the same and the second raises."""
+    gen = generator(39)
+    x = [normal(gen, 2, 10, 2, 32, dtype=torch.bfloat16).requires_grad_(True) for _ in range(3)]
+    table, gain = normal(gen, 32, 2, dtype=torch.bfloat16).requires_grad_(True), torch.ones(32, device="cuda", requires_grad=True)
+    z, index = normal(gen, 5, 20).requires_grad_(True), torch.zeros(5, 2, device="cuda", dtype=torch.int64)
+    plan, rotary = ops.RelativeBuckets(), ops.RotaryFrequencies(32)
+    for value, leaf in ((lambda: ops.relative_attention(*x, table, plan).float().square().sum(), x[0]),
+                        (lambda: ops.qk_norm_rope(x[0], x[1], gain, gain, rotary)[0].float().square().sum(), x[0]),
+                        (lambda: ops.distill_top_logits(z, torch.ones(5, 2, device="cuda"), index).sum(), z)):
+        plain, = torch.autograd.grad(value(), leaf)
+        grad, = torch.autograd.grad(value(), leaf, create_graph=True)
+        assert torch.equal(plain, grad)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(grad.float().sum(), leaf)
+
+
 def long_step(seed):
     gen = generator(seed)
     x = normal(gen, 2, 200, 8, 64, dtype=torch.bfloat16)
