@@ -10,7 +10,7 @@
 // maximum and the accumulator O, in tensor memory too, is rescaled.  So a tile takes no maximum as a rule.
 // 256 of the 512 columns and 84 KB: two blocks per SM, one's exponentials over the other's products and waits.  What
 // bounds it: the exponentials, 128 x 64 of them per tile at 16 a clock against 256 clocks of products, and the blocks'
-// number (512 over 296 places): 115 us at 2 x 4096 tokens, 8 heads of 64, of which the exponentials alone are 60 and with
+// number (512 over 296 places): 110 us at 2 x 4096 tokens, 8 heads of 64, of which the exponentials alone are 60 and with
 // a quarter of them on the multiply-add pipe 45.
 //
 // Rows of 128 bytes (64 for heads of 32) in the swizzled layout of that width: K-major for Q and K, MN-major for V.
@@ -67,12 +67,16 @@ static __device__ __noinline__ float tc_maximum(uint32_t scores, TcTile w, Pair 
   return top;
 }
 
-// 2^x on the multiply-add pipe, for x up to 127: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with the least
-// largest relative error (2^-18.5, by exchange of its extreme points), n added to the exponent.  From -125 down the result
-// stays 2^-125 or so, -inf included.
+__device__ __forceinline__ float clamp_exponent(float x) {  // NaN stays
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(x));  // -125, 127
+  return x;
+}
+// 2^x on the multiply-add pipe: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with the least largest relative
+// error (2^-18.5, by exchange of its extreme points), n added to the exponent.  From -125 down the result stays 2^-125 or
+// so, -inf included; from 127 up, and for a NaN, it is far above the growth that makes the tile anew.
 __device__ __forceinline__ Pair exp2_fma(Pair x) {
   float2 f = both(x);
-  x = pair(fmaxf(f.x, -125.f), fmaxf(f.y, -125.f));
+  x = pair(clamp_exponent(f.x), clamp_exponent(f.y));
   const Pair round = pair(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
   const Pair t = add2(x, round), n = add2(t, pair(-12582912.f, -12582912.f));
   const Pair r = fma2(n, pair(-1.f, -1.f), x);

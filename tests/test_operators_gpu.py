@@ -783,6 +783,25 @@ def test_long_attention_scores_that_grow(tokens, d, dtype, way):
         attention_check(q, k, v, table, plan, dout=dout)
 
 
+@pytest.mark.parametrize("d", [32, 64])
+@pytest.mark.parametrize("at", [400, 401, 403, 405, 406, 407, 408, 414, 415])
+def test_long_attention_one_key_beyond_all_range(d, at):
+    """One key whose scores leave float32's exponents against the rows' references, and one that is NaN, at the places of
+    a tile that take different ways to their exponential."""
+    q, k, v, table, _, _, _ = attention_inputs((1, 700, 2, 2, d, "bf16", False, False, "packed"), seed=60)
+    plan = ops.RelativeBuckets(32, 20)  # most tiles lie beyond the reach
+    k, q = k.clone(), q.clone()
+    q[:, torch.arange(700, device="cuda") % 32 != 5] = 0  # one row in 32, so that no neighbour notices for it
+    keep = k[:, at].clone()
+    k[:, at] *= 100
+    ref = attention_reference(q, k, v, table, plan, None, d ** -0.5)
+    # arguments of 2^9: twice the slack
+    within(ops.relative_attention(q, k, v, table, plan), ref["out"], (2 * half_step(k.dtype) + 2 * SLACK) * ref["out_abs"] + 1e-30, "out")
+    k[:, at] = keep
+    k[:, at, :, 3] = math.nan
+    assert ops.relative_attention(q, k, v, table, plan).isnan().all()
+
+
 @pytest.mark.parametrize("tokens,d", [(321, 64), (700, 32), (130, 32)])
 @pytest.mark.parametrize("open_", ["near", "far before", "far after", "tall"])
 def test_long_attention_closed_distances(tokens, d, open_):
