@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(QK_THREADS, BWD ? 2 : 3) k_qk_norm_rope(const 
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + bb[i] * bb[i];
       ss = group_sum(ss, lanes);
-      const float r = rsqrtf(ss * inv_d + g.eps);
+      // lanes without a vector hold zeros, which an infinite factor (eps of 0) would make NaN in the gains' gradients
+      const float r = live ? rsqrtf(ss * inv_d + g.eps) : 0.f;
       // lanes past the head's pairs take part in its sums: with zeros, which only finite coefficients keep
       qk_read_cs<VEC>(cs + (live ? SHARED ? at[u] : u * g.step + tok : 0) * half, chunk * 8 < half ? chunk : 0, half, c, s);
       if (!BWD) {

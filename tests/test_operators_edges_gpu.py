@@ -1,0 +1,51 @@
+"""GPU tests of the operators at edges of what their documentation allows: values with a common mean, eps of 0, NaN among
+masks, huge values behind masks, calls whose results must not depend on earlier ones."""
+
+import math
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+from multigpubeamsearch_b200 import operators as ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def normal(gen, *shape, dtype=torch.float32, mean=0.0):
+    return (torch.randn(shape, generator=gen, device="cuda") + mean).to(dtype)
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Query and key norm
+# ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("b,t,h,hk,d,dtype", [(1, 1, 1, 1, 32, torch.bfloat16), (1, 1, 3, 1, 96, torch.float32), (3, 11, 5, 2, 48, torch.float16),
+                                              (2, 333, 8, 8, 32, torch.bfloat16), (1, 65, 2, 2, 256, torch.float32)])
+def test_qk_norm_rope_without_eps(b, t, h, hk, d, dtype):
+    """eps = 0 and no zero vector: all results are the definition's, whatever slots of the last block have no token."""
+    gen = generator(b * t)
+    x = [normal(gen, b, t, n, d, dtype=dtype).requires_grad_(True) for n in (h, hk)]
+    gain = [(1 + 0.2 * normal(gen, d)).requires_grad_(True) for _ in range(2)]
+    dy = [normal(gen, *y.shape, dtype=dtype) for y in x]
+    rotary = ops.RotaryFrequencies(d, inv_freq=[0.0] * (d // 2))  # turns nothing
+    out = ops.qk_norm_rope(*x, *gain, rotary, eps=0.0)
+    got = torch.autograd.grad(out, [*x, *gain], dy)
+    u = torch.finfo(dtype).eps / 2
+    for i in range(2):
+        xd, gd = x[i].detach().double().requires_grad_(True), gain[i].detach().double().requires_grad_(True)
+        y = gd * xd / xd.square().mean(-1, keepdim=True).sqrt()
+        dx, dg = torch.autograd.grad(y, (xd, gd), dy[i].double())
+        # one rounding of each result, and 2^-18 for the float32 steps (sums of at most 666 terms and of 256 squares)
+        assert ((out[i].double() - y).abs() <= (u + 2.0 ** -18) * y.abs()).all()
+        assert (got[i].double() - dx).norm() <= (u + 2.0 ** -18) * dx.norm()
+        assert (got[2 + i].double() - dg).norm() <= 2.0 ** -18 * dg.norm()
