@@ -382,25 +382,28 @@ int qk_layout(QkArgs& g, int in_flight) {
 
 constexpr int QK_BWD_BLOCKS = 592;  // at most, also the number of partial sums of the gains' gradients
 
-// Blocks per SM of a kernel at this size; asked once per size class.
-template <typename K> int qk_resident(K kernel, int threads, size_t smem) {
-  static std::atomic<int> known[9][8];
-  std::atomic<int>& n = known[threads / 32][smem >> 13 > 7 ? 7 : smem >> 13];
+// Blocks per SM of one kernel (a template argument, because all of them have one type), asked once per number of warps and
+// 8 KB of shared memory at the most of both: the grid, and with it the order of the gains' partial sums, depends on
+// nothing that was called before.
+template <void (*KERNEL)(QkArgs)> int qk_resident(int threads, size_t smem) {
+  static std::atomic<int> known[9][9];
+  const size_t step = (smem + 8191) / 8192;  // of at most 49152 bytes without a raised limit
+  std::atomic<int>& n = known[threads / 32][step > 8 ? 8 : step];
   int v = n.load(std::memory_order_relaxed);
   if (!v) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, kernel, threads, smem) != cudaSuccess || v < 1) v = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, KERNEL, threads, step * 8192) != cudaSuccess || v < 1) v = 1;
     n.store(v, std::memory_order_relaxed);
   }
   return v;
 }
 
 template <typename T, bool INTER, bool VEC, int U, bool BWD, bool SHARED> int qk_start(QkArgs& g, int parts, int* blocks, cudaStream_t st) {
-  const auto kernel = k_qk_norm_rope<T, INTER, VEC, U, BWD, SHARED>;
+  constexpr auto kernel = k_qk_norm_rope<T, INTER, VEC, U, BWD, SHARED>;
   const int threads = (g.cols * g.step + 31) / 32 * 32;
   size_t smem = (size_t)(SHARED ? g.tokens : 2 * g.span) * (g.head_dim / 2) * sizeof(float2);
   if (BWD && smem < QK_THREADS * 17 * sizeof(float)) smem = QK_THREADS * 17 * sizeof(float);
   const int64_t turns = ((int64_t)g.batch * g.tokens + g.span - 1) / g.span;
-  int64_t most = (int64_t)device_sms() * qk_resident(kernel, threads, smem);  // one wave: every block has the same work
+  int64_t most = (int64_t)device_sms() * qk_resident<k_qk_norm_rope<T, INTER, VEC, U, BWD, SHARED>>(threads, smem);  // one wave: every block has the same work
   if (BWD && most > QK_BWD_BLOCKS) most = QK_BWD_BLOCKS;
   most = most < parts ? 1 : most / parts;
   if (BWD && parts > QK_BWD_BLOCKS) return MGBS_ERR_TOO_LARGE;

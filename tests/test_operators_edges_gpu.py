@@ -49,3 +49,28 @@ def test_qk_norm_rope_without_eps(b, t, h, hk, d, dtype):
         assert ((out[i].double() - y).abs() <= (u + 2.0 ** -18) * y.abs()).all()
         assert (got[i].double() - dx).norm() <= (u + 2.0 ** -18) * dx.norm()
         assert (got[2 + i].double() - dg).norm() <= 2.0 ** -18 * dg.norm()
+
+
+EARLIER_CALLS = """
+import hashlib, sys, torch
+from multigpubeamsearch_b200 import operators as ops
+
+def call(b, t, h, hk, train):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = [torch.randn((b, t, n, 32), generator=gen, device="cuda").bfloat16().requires_grad_(train) for n in (h, hk)]
+    gain = [torch.ones(32, device="cuda", requires_grad=train) for _ in range(2)]
+    out = ops.qk_norm_rope(*x, *gain, ops.RotaryFrequencies(32))
+    return torch.autograd.grad(out, [*x, *gain], [torch.randn(y.shape, generator=gen, device="cuda").bfloat16() for y in out]) if train else out
+
+if sys.argv[1] == "other":
+    call(4, 128, 8, 8, False)
+print(hashlib.sha256(b"".join(g.view(torch.uint8).cpu().numpy().tobytes() for g in call(1, 100001, 2, 1, True))).hexdigest())
+"""
+
+
+def test_qk_norm_rope_does_not_depend_on_earlier_calls():
+    """A gradient's bits in a process of its own and in one that called a forward of another shape first."""
+    root = Path(__file__).resolve().parents[1]
+    said = [subprocess.run([sys.executable, "-c", EARLIER_CALLS, first], cwd=root, capture_output=True, text=True, timeout=600, check=True).stdout
+            for first in ("nothing", "other")]
+    assert said[0] == said[1]
