@@ -335,7 +335,7 @@ int qk_prepare(const MgbsQkNormArgs* a, bool bwd, QkArgs* g, bool* vec, int* ele
   else if (!a->q || !a->k || !a->q_out || !a->k_out || (bwd && (!a->dq_out || !a->dk_out))) return MGBS_ERR_ARG;
   if (!a->q_gain || !a->k_gain || !a->phase) return MGBS_ERR_ARG;
   if (a->position_bits != 0 && a->position_bits != 32 && a->position_bits != 64) return MGBS_ERR_ARG;
-  if (a->position_bits != 0 && !a->positions) return MGBS_ERR_ARG;
+  if (a->position_bits != 0 && !a->positions && a->batch > 0 && a->tokens > 0) return MGBS_ERR_ARG;  // no token: null is an empty tensor's address
   *elem = a->dtype == MGBS_DT_F32 ? 4 : 2;
   *vec = a->head_dim % 16 == 0;
   for (int i = 0; i < 2; ++i) {

@@ -74,3 +74,16 @@ def test_qk_norm_rope_does_not_depend_on_earlier_calls():
     said = [subprocess.run([sys.executable, "-c", EARLIER_CALLS, first], cwd=root, capture_output=True, text=True, timeout=600, check=True).stdout
             for first in ("nothing", "other")]
     assert said[0] == said[1]
+
+
+def test_qk_norm_rope_no_tokens_with_positions():
+    """Batches without a sequence and sequences without a token, with positions given: empty results, zero gradients."""
+    rotary = ops.RotaryFrequencies(32)
+    for b, t, shape in ((0, 5, (0, 5)), (3, 0, (3, 0)), (2, 0, (0,)), (0, 5, (5,))):
+        for dtype in (torch.int32, torch.int64):
+            q = torch.zeros(b, t, 2, 32, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+            gain = torch.ones(32, device="cuda", requires_grad=True)
+            out = ops.qk_norm_rope(q, q[:, :, :1], gain, gain, rotary, positions=torch.zeros(shape, device="cuda", dtype=dtype))
+            assert out[0].shape == q.shape and out[1].shape == (b, t, 1, 32)
+            grads = torch.autograd.grad(out, (q, gain), [torch.zeros_like(y) for y in out])
+            assert grads[0].shape == q.shape and not grads[1].any()
