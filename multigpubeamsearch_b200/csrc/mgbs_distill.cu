@@ -329,7 +329,8 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   };
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
-  if (warp < warps && !(mine.s >= 0x1p-40f && mine.s <= 0x1p100f)) {  // the whole warp
+  // The whole warp; a NaN stays, as every sum and the row's results are NaN with it, while a maximum would pass over it.
+  if (warp < warps && (mine.s < 0x1p-40f || mine.s > 0x1p100f)) {
     const Scale sc(maximum(), g.c);
     mine.k = sc.huge ? (sc.m > 0.f ? DISTILL_FAR : -DISTILL_FAR) : (int)sc.k;
     mine.s = sc.huge ? 0.f : sum_to(sc);

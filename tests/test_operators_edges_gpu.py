@@ -87,3 +87,28 @@ def test_qk_norm_rope_no_tokens_with_positions():
             assert out[0].shape == q.shape and out[1].shape == (b, t, 1, 32)
             grads = torch.autograd.grad(out, (q, gain), [torch.zeros_like(y) for y in out])
             assert grads[0].shape == q.shape and not grads[1].any()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Distillation: a NaN among closed columns
+# ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("width", [1000, 1025, 3001, 50021, 300007])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fill", [-math.inf, -3.0e38, -1.0e7])
+def test_distill_nan_among_closed_columns(width, dtype, fill):
+    """All columns from 6 on closed but for a NaN somewhere among them: loss and gradient of that row are NaN, others are not."""
+    gen = generator(width)
+    places = sorted({7, 2064 % width, width // 3, width // 2, width - 130, width - 1})
+    logits = normal(gen, len(places) + 1, width, dtype=dtype)
+    logits[:, 6:] = fill
+    for row, at in enumerate(places):
+        logits[row, max(at, 6)] = math.nan
+    teacher = normal(gen, len(places) + 1, 3)
+    index = torch.tensor([0, 3, 5], device="cuda").expand(len(places) + 1, 3).contiguous()
+    alone = ops.distill_top_logits(logits, teacher, index)
+    loss, grad = ops.distill_top_logits_step(logits, teacher, index)
+    for got in (alone, loss):
+        assert got[:-1].isnan().all() and got[-1].isfinite(), (places, got)
+    assert grad[:-1].isnan().all() and grad[-1].isfinite().all()
