@@ -142,7 +142,7 @@ constexpr int DISTILL_WIDE = 512;  // threads of a block at most
 
 // Sum of 2^(x c - k) over some logits, k whole: sums of different k differ by exact powers of two, and a term costs one
 // fused step without an error of its own in k.
-struct Sum { int k; float s; };
+struct __align__(8) Sum { int k; float s; };  // one 8-byte store to another block
 constexpr int DISTILL_FAR = 1 << 24;  // |k| of logits out of all proportion: the row takes the slow way
 
 // n <= 32 of them in shared memory, in a fixed order; the whole warp calls.
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(DISTILL_WIDE, 2) k_distill_wide(const __grid_c
   extern __shared__ __align__(16) uint8_t held[];  // [capacity] pieces, then the entries
   __shared__ Sum warp_part[DISTILL_WIDE / 32];
   __shared__ Sum parts[8];  // of every block of the cluster
-  __shared__ uint32_t s_seen[1024];  // one bit per column modulo 2^15: whether an index may be there twice
+  __shared__ __align__(16) uint32_t s_seen[1024];  // one bit per column modulo 2^15: whether an index may be there twice; cleared 16 bytes at a time
   __shared__ float s_ts;
   __shared__ int s_any, s_twice;
   const int entries4 = (g.entries + 3) / 4;

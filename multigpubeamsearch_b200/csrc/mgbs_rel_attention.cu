@@ -832,8 +832,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(const __grid_constant__ RelArgs g, int tiles, int ranks) {
   constexpr int PITCH = RelTile<D>::PITCH, MAT = TILE * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
-  __shared__ float2 row_stat[2][TILE];  // a stage's queries: maximum and log2 of the sum
-  __shared__ float row_delta[2][TILE];
+  __shared__ __align__(16) float2 row_stat[2][TILE];  // a stage's queries: maximum and log2 of the sum
+  __shared__ __align__(16) float row_delta[2][TILE];
   float* bt = reinterpret_cast<float*>(rel_smem + 6 * tile_bytes<D>());
   const int side = g.reach + REL_RIM;
   const int rank = (int)(blockIdx.x % ranks);
