@@ -67,16 +67,21 @@ static __device__ __noinline__ float tc_maximum(uint32_t scores, TcTile w, Pair 
   return top;
 }
 
-__device__ __forceinline__ float clamp_exponent(float x) {  // NaN stays
-  asm("max.NaN.f32 %0, %0, 0fC2FA0000;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(x));  // -125, 127
+__device__ __forceinline__ float clamp_above(float x) {  // NaN stays
+  asm("min.NaN.f32 %0, %0, 0f42FE0000;" : "+f"(x));  // 127
   return x;
 }
+__device__ __forceinline__ float scaled(float y, float t, float x) {  // y 2^n, n in the low bits of t; whatever comes of an x below -125
+  return x < -125.f ? 0.f : __int_as_float(__float_as_int(y) + (__float_as_int(t) << 23));
+}
 // 2^x on the multiply-add pipe: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with the least largest relative
-// error (2^-18.5, by exchange of its extreme points), n added to the exponent.  From -125 down the result stays 2^-125 or
-// so, -inf included; from 127 up, and for a NaN, it is far above the growth that makes the tile anew.
+// error (2^-18.5, by exchange of its extreme points), n added to the exponent.  Below -125 the result is 0, as what weighs
+// nothing must not be multiplied by a value near the type's largest; from 127 up, and for a NaN, it is far above the
+// growth that makes the tile anew.
 __device__ __forceinline__ Pair exp2_fma(Pair x) {
   float2 f = both(x);
-  x = pair(clamp_exponent(f.x), clamp_exponent(f.y));
+  f = make_float2(clamp_above(f.x), clamp_above(f.y));
+  x = pair(f.x, f.y);
   const Pair round = pair(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
   const Pair t = add2(x, round), n = add2(t, pair(-12582912.f, -12582912.f));
   const Pair r = fma2(n, pair(-1.f, -1.f), x);
@@ -84,9 +89,8 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
   y = fma2(r, y, pair(0.2402474483148465f, 0.2402474483148465f));
   y = fma2(r, y, pair(0.693121814743091f, 0.693121814743091f));
   y = fma2(r, y, pair(0.9999992614416005f, 0.9999992614416005f));
-  f = both(y);
-  const float2 e = both(t);
-  return pair(__int_as_float(__float_as_int(f.x) + (__float_as_int(e.x) << 23)), __int_as_float(__float_as_int(f.y) + (__float_as_int(e.y) << 23)));
+  const float2 v = both(y), e = both(t);
+  return pair(scaled(v.x, e.x, f.x), scaled(v.y, e.y, f.y));
 }
 
 // P of the tile relative to `base` into tensor memory; returns the row's sum.

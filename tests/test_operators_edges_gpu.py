@@ -112,3 +112,32 @@ def test_distill_nan_among_closed_columns(width, dtype, fill):
     for got in (alone, loss):
         assert got[:-1].isnan().all() and got[-1].isfinite(), (places, got)
     assert grad[:-1].isnan().all() and grad[-1].isfinite().all()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Attention: huge values behind masks
+# ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("closed", [-math.inf, -3.0e38, -1.0e4])
+@pytest.mark.parametrize("tokens,d", [(40, 32), (700, 64), (700, 32)])
+def test_relative_attention_huge_values_behind_a_mask(tokens, d, closed):
+    """Keys beyond a distance closed by the table hold values near the type's largest: they weigh nothing."""
+    gen = generator(tokens + d)
+    b, h, dtype, u = 1, 2, torch.bfloat16, 2.0 ** -8
+    q, k = normal(gen, b, tokens, h, d, dtype=dtype), normal(gen, b, tokens, h, d, dtype=dtype)
+    plan = ops.RelativeBuckets(32, 16 if tokens < 64 else 128)
+    table = normal(gen, 32, h, dtype=dtype)
+    table[15] = table[31] = closed  # the last bucket of either side
+    reach = next(i for i in range(plan.max_distance + 1) if int(plan.map[plan.max_distance + i]) == 31)
+    v = normal(gen, b, tokens, h, d, dtype=dtype)
+    rows = max(1, tokens // 2 - reach)  # the first rows see none of the last tokens
+    v[:, tokens // 2:] = 1.0e38
+    out = ops.relative_attention(q, k, v, table, plan)[:, :rows].double()
+    off = torch.arange(tokens, device="cuda")[None] - torch.arange(rows, device="cuda")[:, None]
+    index = plan.map.long()[off.clamp(-plan.max_distance, plan.max_distance) + plan.max_distance]
+    s = torch.einsum("bihd,bjhd->bhij", q[:, :rows].double(), k.double()) * d ** -0.5 + table.double()[index].permute(2, 0, 1)
+    p = s.softmax(-1)
+    p = torch.where(index == 31, 0.0, p)  # exp(-1e4 + a few) is 0 in any format that holds 1e38 finite
+    want, size = torch.einsum("bhij,bjhd->bihd", p, v.double()), torch.einsum("bhij,bjhd->bihd", p, v.double().abs())
+    assert ((out - want).abs() <= (2 * u + 2.0 ** -14) * size).all()
