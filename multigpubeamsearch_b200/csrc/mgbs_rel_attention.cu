@@ -28,8 +28,8 @@ constexpr int REL_THREADS = 128;
 // Blocks per multiprocessor that a kernel's registers are held to, each the fastest of those tried:
 constexpr int REL_FWD_BLOCKS = 4;  // 3: 806 us against 749 us at 32768 x 54 tokens, 8 heads of 32
 constexpr int REL_BWD_BLOCKS = 3;  // 2: 546 us against 538 us at 8192 x 54 tokens
-constexpr int REL_Q_BLOCKS = 3;    // 2: 112 us against 107 us at 6 x 1501 causal tokens, 8 heads of 64 over 2
-constexpr int REL_KV_BLOCKS = 3;   // 2: 132 us, 4: 154 us against 119 us there, with the heads one after the other
+constexpr int REL_Q_BLOCKS = 2;    // 3: 93 us, 4: 121 us against 88 us at 6 x 1501 causal padded tokens, 8 heads of 64 over 2
+constexpr int REL_KV_BLOCKS = 3;   // 2: 164 us, 4: 152 us against 134 us there
 // rows of the short form's matrices are padded by 16 bytes: eight rows then start in distinct banks
 template <int D> struct RelTile { static constexpr int PITCH = D + 8; };
 
@@ -634,23 +634,15 @@ __global__ void __launch_bounds__(REL_THREADS) k_rel_tiles(const __grid_constant
   }
 }
 
-// dq, delta and the table's gradient: a block owns 64 queries and walks over the keys.  Bound by the latency of a warp's
-// chain of products and exponentials, with 12 warps on a multiprocessor: 107 us at 6 x 1501 causal tokens, 8 heads of 64
-// over 2 (143 us before the longest tiles of all heads started first and dS moved into the place of q and dout; the
-// tcgen05 form takes 57 us).
-constexpr int DS_PITCH = TILE + 1;
-template <int D> __host__ __device__ constexpr int dq_front() {  // q and dout, whose place a tile of dS takes
-  return 2 * tile_bytes<D>() > TILE * DS_PITCH * 4 ? 2 * tile_bytes<D>() : TILE * DS_PITCH * 4;
-}
+// dq and delta: a block owns 64 queries and walks over the keys.  Bound by the latency of a warp's chain of products and
+// exponentials, with 8 warps on a multiprocessor: 88 us at 6 x 1501 causal padded tokens, 8 heads of 64 over 2 (40 us in
+// the tcgen05 form).
 template <typename T, int D>
 __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(const __grid_constant__ RelArgs g, int tiles) {
   constexpr int PITCH = RelTile<D>::PITCH, MAT = TILE * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
-  __shared__ float far_sum[2][4];
-  float* ds = reinterpret_cast<float*>(rel_smem);  // one tile of dS, once q and dout are in registers
-  float* bt = reinterpret_cast<float*>(rel_smem + dq_front<D>() + 4 * tile_bytes<D>());
-  const int side = g.reach + REL_RIM, span = 2 * side + 1;
-  float* dacc = bt + span;            // dS by offset
+  float* bt = reinterpret_cast<float*>(rel_smem + 6 * tile_bytes<D>());
+  const int side = g.reach + REL_RIM;
   Where w = rel_where(blockIdx.x, tiles, g.heads, g.batch);
   w.tile = tiles - 1 - w.tile;  // the longest first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
@@ -659,10 +651,8 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
   const int64_t off0 = head_at + (int64_t)row0 * g.heads * D, off1 = off0 + (int64_t)8 * g.heads * D;
   T* p0 = row0 < g.tokens ? static_cast<T*>(g.dq) + off0 : nullptr;
   T* p1 = row0 + 8 < g.tokens ? static_cast<T*>(g.dq) + off1 : nullptr;
-  float* partial = g.partial + ((int64_t)w.head * g.batch * tiles + (int64_t)w.b * tiles + w.tile) * g.buckets;
   if (i0 >= len) {
     store_zero_rows<T, D>(p0, p1);
-    for (int k = threadIdx.x; k < g.buckets; k += REL_THREADS) partial[k] = 0.f;
     return;  // dk and dv walk over queries below the length only: delta is not read here
   }
   const int head_kv = w.head / (g.heads / g.heads_kv);
@@ -670,7 +660,7 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
   const T* k = static_cast<const T*>(g.k) + w.b * g.ks[0] + head_kv * g.ks[2];
   const T* v = static_cast<const T*>(g.v) + w.b * g.vs[0] + head_kv * g.vs[2];
   const T* dout = static_cast<const T*>(g.dout) + w.b * g.ds[0] + w.head * g.ds[2];
-  const uint32_t q_at = smem_addr(rel_smem), do_at = q_at + MAT * 2, kv_at = q_at + dq_front<D>();
+  const uint32_t q_at = smem_addr(rel_smem), do_at = q_at + MAT * 2, kv_at = q_at + 2 * MAT * 2;
   const int last = g.causal ? min(len, i0 + TILE) : len, n_tiles = (last + TILE - 1) / TILE;
   auto load = [&](int t) {
     const uint32_t to = kv_at + (t & 1) * 2 * MAT * 2;
@@ -682,12 +672,11 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
   load(0);
   copy_commit();
   fill_bias<T>(g, w.head, bt, g.reach + REL_RIM, threadIdx.x, REL_THREADS);
-  for (int i = threadIdx.x; i < span; i += REL_THREADS) dacc[i] = 0.f;
   const bool in0 = row0 < len, in1 = row0 + 8 < len;
   const float2* stats = g.stats + ((int64_t)w.b * g.heads + w.head) * g.tokens;
   const float2 none = make_float2(0.f, INFINITY), st0 = in0 ? stats[row0] : none, st1 = in1 ? stats[row0 + 8] : none;
   uint32_t qa[D / 16][4], da[D / 16][4];
-  float o[D / 8][4], pk[D / 8][4], d0 = 0.f, d1 = 0.f, r0 = 0.f, r1 = 0.f, before = 0.f, after = 0.f;
+  float o[D / 8][4], pk[D / 8][4], d0 = 0.f, d1 = 0.f, r0 = 0.f, r1 = 0.f;
 #pragma unroll
   for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -722,7 +711,6 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
         }
       d0 = quad_sum(d0);
       d1 = quad_sum(d1);
-      __syncthreads();  // q and dout make room
     }
     const uint32_t at = kv_at + (t & 1) * 2 * MAT * 2;
     const int j0 = t * TILE;
@@ -730,7 +718,6 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
     const bool edge = j0 + TILE > len || i0 + TILE > len || (g.causal && j0 + TILE > i0 + 1);
     const float fixed = far > 0 ? bt[2 * side] : bt[0];
     const float* b0 = bt + j0 + 2 * tig - row0 + side;
-    const float seen = r0 + r1;
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
       float s[2][4], dp[2][4];
@@ -753,12 +740,6 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
           dp[n][e] = p * (dp[n][e] - (e >> 1 ? d1 : d0));
           if (e >> 1) r1 += dp[n][e]; else r0 += dp[n][e];
         }
-      if (!far) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ds[(warp * 16 + gid + (e >> 1) * 8) * DS_PITCH + (2 * jj + n) * 8 + 2 * tig + (e & 1)] = dp[n][e];
-      }
       uint32_t a[4], b[4];
       pack_a<T>(a, dp[0], dp[1]);
       pack_a<T>(b, s[0], s[1]);
@@ -771,19 +752,6 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
         mma16816<T>(pk[2 * n], b, m[0], m[1]);
         mma16816<T>(pk[2 * n + 1], b, m[2], m[3]);
       }
-    }
-    const float tile_sum = (r0 + r1) - seen;
-    if (far > 0) after += tile_sum;
-    else if (far < 0) before += tile_sum;
-    else {
-      __syncthreads();
-      const int off = (int)threadIdx.x - (TILE - 1);  // this thread's diagonal of the tile
-      if (off < TILE) {
-        float sum = 0.f;
-        for (int i = max(0, -off); i < min(TILE, TILE - off); ++i) sum += ds[i * DS_PITCH + i + off];
-        dacc[j0 - i0 + off + side] += sum;
-      }
-      // the next tile's sums come after two barriers, its scores after one
     }
   }
   r0 = quad_sum(r0);
@@ -799,60 +767,49 @@ __global__ void __launch_bounds__(REL_THREADS, REL_Q_BLOCKS) k_rel_tiles_dq(cons
     if (in0) delta[row0] = d0 + r0;
     if (in1) delta[row0 + 8] = d1 + r1;
   }
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, m);
-    after += __shfl_xor_sync(0xffffffffu, after, m);
-  }
-  if (lane == 0) { far_sum[0][warp] = before; far_sum[1][warp] = after; }
-  __syncthreads();
-  // offsets past the reach join its ends
-  if (warp < 2) {
-    float sum = 0.f;
-    for (int i = lane; i < REL_RIM; i += 32) sum += warp ? dacc[span - 1 - i] : dacc[i];
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    if (lane == 0) dacc[warp ? span - 1 - REL_RIM : REL_RIM] += sum + (far_sum[warp][0] + far_sum[warp][1]) + (far_sum[warp][2] + far_sum[warp][3]);
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < g.buckets; b += REL_THREADS) {
-    float sum = 0.f;
-    const int n0 = min(max(__ldg(g.start + b), 0), 2 * g.reach + 1), n1 = min(__ldg(g.start + b + 1), 2 * g.reach + 1);
-    for (int n = n0; n < n1; ++n) sum += dacc[min(max(__ldg(g.order + n), 0), 2 * g.reach) + REL_RIM];
-    partial[b] = sum;
-  }
 }
 
-// dk and dv: a block owns 64 keys and walks over queries, in transposed products (keys as rows), so that P^T and dS^T come
-// out of the accumulators as operands of the next product.  The query heads that share the keys are spread over the
-// `ranks` blocks of a cluster, whose sums are added through distributed shared memory at the end, in a fixed order: one
-// block for all heads left most of the device idle (210 us against 119 us at 6 x 1501 causal tokens, 8 heads over 2; 102 us with the longest tiles
-// first; the tcgen05 form takes 56 us).
+// dk, dv and the table's gradient: a block owns 64 keys and walks over queries, in transposed products (keys as rows), so that
+// P^T and dS^T come out of the accumulators as operands of the next product.  The query heads that share the keys are spread
+// over the `ranks` blocks of a cluster, whose sums are added through distributed shared memory at the end, in a fixed order:
+// one block for all heads left most of the device idle (210 us against 119 us at 6 x 1501 causal tokens, 8 heads over 2).
+// The table is summed here, from the corrected delta: by diagonals of a tile of dS in shared memory, whole tiles beyond the
+// reach in registers.  134 us at 6 x 1501 causal padded tokens, 8 heads of 64 over 2 (77 us in the tcgen05 form).
+constexpr int DS_PITCH = TILE + 1;
+template <int D> __host__ __device__ constexpr int dkv_front() {  // k and v, whose place a tile of dS takes
+  return 2 * tile_bytes<D>() > TILE * DS_PITCH * 4 ? 2 * tile_bytes<D>() : TILE * DS_PITCH * 4;
+}
 template <typename T, int D>
 __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(const __grid_constant__ RelArgs g, int tiles, int ranks) {
   constexpr int PITCH = RelTile<D>::PITCH, MAT = TILE * PITCH;
   extern __shared__ __align__(16) uint8_t rel_smem[];
   __shared__ __align__(16) float2 row_stat[2][TILE];  // a stage's queries: maximum and log2 of the sum
   __shared__ __align__(16) float row_delta[2][TILE];
-  float* bt = reinterpret_cast<float*>(rel_smem + 6 * tile_bytes<D>());
-  const int side = g.reach + REL_RIM;
+  __shared__ float far_sum[2][4];
+  float* ds = reinterpret_cast<float*>(rel_smem);  // one tile of dS, keys as rows, once k and v are in registers
+  float* bt = reinterpret_cast<float*>(rel_smem + dkv_front<D>() + 4 * tile_bytes<D>());
+  const int side = g.reach + REL_RIM, span = 2 * side + 1;
+  float* dacc = bt + span;                         // dS by offset
   const int rank = (int)(blockIdx.x % ranks);
   const Where w = rel_where(blockIdx.x / ranks, tiles, g.heads_kv, g.batch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int len = rel_length(g, w.b), j0 = w.tile * TILE, row0 = j0 + warp * 16 + gid;
   auto row_of = [&](void* base, int row) { return row < g.tokens ? static_cast<T*>(base) + (((int64_t)w.b * g.tokens + row) * g.heads_kv + w.head) * D : nullptr; };
+  const int share = g.heads / g.heads_kv / ranks;  // heads of this block: rank, rank + ranks, ...
+  auto head_of = [&](int n) { return (w.head * share + n) * ranks + rank; };
+  auto partial_of = [&](int head) { return g.partial + ((int64_t)head * g.batch * tiles + (int64_t)w.b * tiles + w.tile) * g.buckets; };
   if (j0 >= len) {  // the whole cluster
+    for (int k = threadIdx.x; k < share * g.buckets; k += REL_THREADS) partial_of(head_of(k / g.buckets))[k % g.buckets] = 0.f;
     if (rank == 0) {
       store_zero_rows<T, D>(row_of(g.dk, row0), row_of(g.dk, row0 + 8));
       store_zero_rows<T, D>(row_of(g.dv, row0), row_of(g.dv, row0 + 8));
     }
     return;
   }
-  const int share = g.heads / g.heads_kv / ranks;  // heads of this block: rank, rank + ranks, ...
-  const uint32_t k_at = smem_addr(rel_smem), v_at = k_at + MAT * 2, qd_at = k_at + 2 * MAT * 2;
+  const uint32_t k_at = smem_addr(rel_smem), v_at = k_at + MAT * 2, qd_at = k_at + dkv_front<D>();
   const int first = g.causal ? w.tile : 0, n_tiles = (len + TILE - 1) / TILE - first, steps = n_tiles * share;
   auto load = [&](int n) {
-    const int h = (w.head * share + n / n_tiles) * ranks + rank, row = (first + n % n_tiles) * TILE;
+    const int h = head_of(n / n_tiles), row = (first + n % n_tiles) * TILE;
     const uint32_t to = qd_at + (n & 1) * 2 * MAT * 2;
     stage_tile<T, D>(to, static_cast<const T*>(g.q) + w.b * g.qs[0] + h * g.qs[2], g.qs[1], row, len);
     stage_tile<T, D>(to + MAT * 2, static_cast<const T*>(g.dout) + w.b * g.ds[0] + h * g.ds[2], g.ds[1], row, len);
@@ -873,11 +830,40 @@ __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(co
   for (int n = 0; n < D / 8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) ok[n][e] = ov[n][e] = 0.f;
+  float before = 0.f, after = 0.f;  // sums of dS in tiles beyond the reach
+  // The table's partial sums of one query head, from what its tiles have left by offset.
+  auto finish_table = [&](int head) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, m);
+      after += __shfl_xor_sync(0xffffffffu, after, m);
+    }
+    if (lane == 0) { far_sum[0][warp] = before; far_sum[1][warp] = after; }
+    before = after = 0.f;
+    __syncthreads();
+    // offsets past the reach join its ends
+    if (warp < 2) {
+      float sum = 0.f;
+      for (int i = lane; i < REL_RIM; i += 32) sum += warp ? dacc[span - 1 - i] : dacc[i];
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      if (lane == 0) dacc[warp ? span - 1 - REL_RIM : REL_RIM] += sum + (far_sum[warp][0] + far_sum[warp][1]) + (far_sum[warp][2] + far_sum[warp][3]);
+    }
+    __syncthreads();
+    float* partial = partial_of(head);
+    for (int b = threadIdx.x; b < g.buckets; b += REL_THREADS) {
+      float sum = 0.f;
+      const int n0 = min(max(__ldg(g.start + b), 0), 2 * g.reach + 1), n1 = min(__ldg(g.start + b + 1), 2 * g.reach + 1);
+      for (int n = n0; n < n1; ++n) sum += dacc[min(max(__ldg(g.order + n), 0), 2 * g.reach) + REL_RIM];
+      partial[b] = sum;
+    }
+  };
   for (int n = 0; n < steps; ++n) {
     const int i0 = (first + n % n_tiles) * TILE;
     if (n % n_tiles == 0) {
-      __syncthreads();  // the head before has read its biases
-      fill_bias<T>(g, (w.head * share + n / n_tiles) * ranks + rank, bt, side, threadIdx.x, REL_THREADS);
+      __syncthreads();  // the head before has read its biases and sums
+      fill_bias<T>(g, head_of(n / n_tiles), bt, side, threadIdx.x, REL_THREADS);
+      for (int i = threadIdx.x; i < span; i += REL_THREADS) dacc[i] = 0.f;
     }
     copy_wait<0>();
     __syncthreads();
@@ -889,12 +875,14 @@ __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(co
         ldsm4(ka[kk], k_at + (warp * 16 * PITCH + frag_a<PITCH>(lane)) * 2 + kk * 32);
         ldsm4(va[kk], v_at + (warp * 16 * PITCH + frag_a<PITCH>(lane)) * 2 + kk * 32);
       }
+      __syncthreads();  // k and v make room
     }
     const uint32_t at = qd_at + (n & 1) * 2 * MAT * 2;
     const int far = rel_side(i0, j0, g.reach);
     const float fixed = far > 0 ? bt[2 * side] : bt[0];
     const float* b0 = bt + row0 - i0 - 2 * tig + side;  // offset of key row0 from query i0 + 2 tig
-    const bool edge = i0 + TILE > len || (g.causal && j0 + TILE > i0 + 1);
+    const bool edge = i0 + TILE > len || j0 + TILE > len || (g.causal && j0 + TILE > i0 + 1);
+    float tile_sum = 0.f;
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii) {  // 16 queries each
       float s[2][4], dp[2][4];
@@ -912,11 +900,13 @@ __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(co
           const float bias = far ? fixed : b0[(e >> 1) * 8 - c];
           float p = fast_exp2((fmaf(s[m][e], g.sl2, bias) - (e & 1 ? st.z : st.x)) - (e & 1 ? st.w : st.y));
           if (edge) {
-            const int i = i0 + c + 2 * tig;
-            if (i >= len || (g.causal && row0 + (e >> 1) * 8 > i)) p = 0.f;
+            const int i = i0 + c + 2 * tig, j = row0 + (e >> 1) * 8;
+            if (i >= len || j >= len || (g.causal && j > i)) p = 0.f;
           }
           s[m][e] = p;
           dp[m][e] = p * (dp[m][e] - (e & 1 ? dl.y : dl.x));
+          tile_sum += dp[m][e];
+          if (!far) ds[(warp * 16 + gid + (e >> 1) * 8) * DS_PITCH + c + 2 * tig] = dp[m][e];
         }
       }
       uint32_t a[4];
@@ -924,6 +914,22 @@ __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(co
       cols_product<T, D>(ov, a, at + (MAT + ii * 16 * PITCH + frag_a<PITCH>(lane)) * 2);
       pack_a<T>(a, dp[0], dp[1]);
       cols_product<T, D>(ok, a, at + (ii * 16 * PITCH + frag_a<PITCH>(lane)) * 2);
+    }
+    if (far > 0) after += tile_sum;
+    else if (far < 0) before += tile_sum;
+    else {
+      __syncthreads();
+      const int off = (int)threadIdx.x - (TILE - 1);  // key minus query of this thread's diagonal, within the tile
+      if (off < TILE) {
+        float sum = 0.f;
+        for (int i = max(0, -off); i < min(TILE, TILE - off); ++i) sum += ds[(i + off) * DS_PITCH + i];
+        dacc[j0 - i0 + off + side] += sum;
+      }
+      // the next tile's sums come after two barriers, its scores after one
+    }
+    if (n % n_tiles == n_tiles - 1) {
+      __syncthreads();
+      finish_table(head_of(n / n_tiles));
     }
   }
   const float in0 = row0 < len ? 1.f : 0.f, in1 = row0 + 8 < len ? 1.f : 0.f;
@@ -934,7 +940,7 @@ __global__ void __launch_bounds__(REL_THREADS, REL_KV_BLOCKS) k_rel_tiles_dkv(co
   }
   constexpr int SP = D + 4;
   float* sums = reinterpret_cast<float*>(rel_smem);  // [dv, dk][TILE][SP]
-  static_assert(2 * TILE * SP * 4 <= 6 * tile_bytes<D>(), "the sums fit the stages");
+  static_assert(2 * TILE * SP * 4 <= dkv_front<D>() + 4 * tile_bytes<D>(), "the sums fit the stages");
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < D / 8; ++n)
@@ -1067,21 +1073,21 @@ template <typename T, int D> int run_tiles(const RelArgs& g, cudaStream_t st) {
 
 template <typename T, int D> int run_tiles_bwd(const RelArgs& g, cudaStream_t st) {
   static std::atomic<uint64_t> raised_q{0}, raised_kv{0};
-  const int fixed_q = dq_front<D>() + 4 * tile_bytes<D>(), fixed_kv = 6 * tile_bytes<D>();
-  int rc = raise_smem(k_rel_tiles_dq<T, D>, fixed_q + 2 * rel_bias_floats(1024) * 4, raised_q);
-  if (!rc) rc = raise_smem(k_rel_tiles_dkv<T, D>, fixed_kv + rel_bias_floats(1024) * 4, raised_kv);
+  const int fixed_q = 6 * tile_bytes<D>(), fixed_kv = dkv_front<D>() + 4 * tile_bytes<D>();
+  int rc = raise_smem(k_rel_tiles_dq<T, D>, fixed_q + rel_bias_floats(1024) * 4, raised_q);
+  if (!rc) rc = raise_smem(k_rel_tiles_dkv<T, D>, fixed_kv + 2 * rel_bias_floats(1024) * 4, raised_kv);
   if (rc) return rc;
   const int tiles = (g.tokens + TILE - 1) / TILE;
   const int64_t rows = (int64_t)g.batch * tiles, blocks = rows * g.heads;
   if (blocks > 0x7fffffffll) return MGBS_ERR_TOO_LARGE;
-  k_rel_tiles_dq<T, D><<<(unsigned)blocks, REL_THREADS, fixed_q + 2 * rel_bias_floats(g.reach) * 4, st>>>(g, tiles);
+  k_rel_tiles_dq<T, D><<<(unsigned)blocks, REL_THREADS, fixed_q + rel_bias_floats(g.reach) * 4, st>>>(g, tiles);
   rc = (int)cudaGetLastError();
   if (rc) return rc;
   const int ranks = rel_ranks(g);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * g.heads_kv * ranks));
   cfg.blockDim = dim3(REL_THREADS);
-  cfg.dynamicSmemBytes = fixed_kv + rel_bias_floats(g.reach) * 4;
+  cfg.dynamicSmemBytes = fixed_kv + 2 * rel_bias_floats(g.reach) * 4;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1092,7 +1098,7 @@ template <typename T, int D> int run_tiles_bwd(const RelArgs& g, cudaStream_t st
   return (int)cudaLaunchKernelEx(&cfg, k_rel_tiles_dkv<T, D>, g, tiles, ranks);
 }
 
-// The table's gradient from a row of sums per head, sequence and tile of queries.
+// The table's gradient from a row of sums per head, sequence and tile of keys.
 template <typename T> int sum_table(const RelArgs& g, int tile, void* dtable, float* sums, cudaStream_t st) {
   const int64_t rows = (int64_t)g.batch * ((g.tokens + tile - 1) / tile);
   if (rows <= 256) return finish_table<T>(g, g.partial, rows, rows, 1, dtable, st);
@@ -1107,9 +1113,10 @@ template <typename T> int sum_table(const RelArgs& g, int tile, void* dtable, fl
 //   heads of 32:  T = 65: 1355 against 947, 256: 785 against 712, 384: 932 against 972, 512: 1056 against 1233 (half the
 //                 products per exponential, so that a block's fixed costs weigh more)
 template <int D> constexpr int rel_tc_tokens() { return D == 64 ? 65 : 321; }
-// The backward is on tcgen05 from there on for every head size: 221184 tokens, 8 heads of 64 in sequences of T = 65: 1844 us
-// against 3361 us, 192: 1556 against 2157, 1000: 3303 against 7826; heads of 32: 65: 1636 against 2446, 192: 1341 against
-// 1479; 33 tokens, 8 heads of 64 over 2: 3214 against 2931.
+// The backward is on tcgen05 from 65 tokens on for every head size: 221184 tokens, 8 heads of 64 in sequences of T = 65:
+// 1776 us against 3447 us, 129: 2250 against 3418, 192: 1526 against 2182, 1000: 3397 against 8488; heads of 32: 65: 1569
+// against 2604, 129: 1998 against 2539, 192: 1343 against 1522.  Below, where only shared key heads come here, the other
+// form is ahead: 33 tokens, 8 heads of 64 over 2: 3216 against 2963, 64 tokens: 1836 against 1661.
 constexpr int REL_TC_BACKWARD_TOKENS = 65;
 template <typename T> struct Type;
 template <> struct Type<__nv_bfloat16> { static constexpr int DT = MGBS_DT_BF16; };

@@ -10,19 +10,22 @@
 // steps follow one another; the second block of the multiprocessor (256 of the 512 columns each) fills the waits.
 //
 // delta = sum_j P_ij dP_ij.  A first delta is dout . out from the 16-bit output.  A row of dS has to sum to 0, so the sum r
-// of the rows made with it is the error of that delta: at the end dq loses r P k, and the other form gets delta + r.  The
-// table's gradient keeps the first delta: its error, sums of r P over rows, is of the size of its own rounding to 16 bits.
+// of the rows made with it is the error of that delta: at the end dq loses r P k, and the other form gets delta + r.
 //
-// The table's gradient is summed in the dq form: tiles beyond the reach in registers, nearer ones by diagonals of a warp's
-// 32 x 32 through shared memory into the warp's own sums by offset, in a fixed order.  The query heads that share a key head are spread over the blocks of a cluster, whose
-// sums are added through distributed shared memory.  Rows past a length are zeroed in shared memory where they are B
-// operands of the second products; elsewhere they only reach scores that are hidden and rows that are not written.
+// The table's gradient is summed in the dk, dv form, from the corrected delta: where values have a common mean, the first
+// delta's error (the output's rounding) is large beside what is left of a row's dS over many keys, 23 u of the table's
+// 2-norm for v of mean 4 and spread 1 at 1001 tokens.  Tiles beyond the reach are summed in registers, nearer ones by
+// diagonals of 16 x 16 through shared memory into the warp's own sums by offset, in a fixed order.  The query heads that
+// share a key head are spread over the blocks of a cluster, whose dk and dv are added through distributed shared memory.
+// Rows past a length are zeroed in shared memory where they are B operands of the second products; elsewhere they only
+// reach scores that are hidden and rows that are not written.
 // Every wait is bounded: a block that gives up writes NaN and the error word.
 //
-// At 6 x 1501 causal tokens, 8 heads of 64 over 2: 57 us for dq and 56 us for dk and dv, against 107 us and 102 us on the
-// warp-level instruction (8 us of exponentials each).  What bounds them: the chain of a tile (products 800 to 1000
-// clocks with their hand-overs, the row's arithmetic 1250) and the blocks' beginnings and ends, 10 us of 57; in the dq
-// form the diagonals take 13 us.
+// At 6 x 1501 causal padded tokens, 8 heads of 64 over 2: 40 us for dq, 77 us for dk, dv and the table, against 88 us and
+// 134 us on the warp-level instruction (8 us of exponentials each).  What bounds them: the chain of a tile (products 800
+// to 1000 clocks with their hand-overs, the row's arithmetic 1250), since the scores of the next tile are issued only
+// when this one's second products are done, and the blocks' beginnings and ends; the table's diagonals take 20 us of the 77.
+// (Summed in the dq form, with the first delta, the two were 57 and 56 us.)
 
 #include <math.h>
 
@@ -34,12 +37,13 @@ namespace mgbs {
 
 constexpr int TB_DP_COL = 64, TB_ACC1_COL = 128, TB_ACC2_COL = 192;  // S at 0; P and dS in the places of S and dP
 constexpr int TB_RIM = 192;  // a tile that is not beyond the reach has offsets below reach + TC_Q + TC_K
-constexpr int TB_HALF = TC_K / 2, TB_DS_PITCH = TB_HALF + 2;  // dS by half tiles: pairs of a row in one store, half a warp over all banks
+// A warp's 32 rows of 16 columns of dS: pairs of a row in one store, 16 rows over all banks, the other 16 half of them apart.
+constexpr int TB_COLS = 16, TB_DS_PITCH = TB_COLS + 2, TB_DS_HALF = 16 * TB_DS_PITCH + 16, TB_DS = 2 * TB_DS_HALF;
 template <bool KV> __host__ __device__ constexpr int tb_stages() { return KV ? 3 : 2; }
 __host__ __device__ inline int tb_bias_floats(int reach) { return 2 * (reach + TB_RIM) + 1; }
 template <int D, bool KV> __host__ __device__ constexpr int tb_operands() { return (2 * TC_Q + tb_stages<KV>() * 2 * TC_K) * D * 2; }
 template <int D, bool KV> inline int tb_smem(int reach, int buckets) {
-  const int table = KV ? tb_bias_floats(reach) : 5 * tb_bias_floats(reach) + 1 + TC_Q * TB_DS_PITCH + 2 * reach + 1 + buckets + 1;
+  const int table = KV ? 5 * tb_bias_floats(reach) + 1 + 4 * TB_DS + 2 * reach + 1 + buckets + 1 : tb_bias_floats(reach);
   const int all = 1024 + tb_operands<D, KV>() + table * 4;
   return all < 78 * 1024 ? 78 * 1024 : all;  // never more than two blocks on an SM: a third would wait for tensor memory
 }
@@ -54,7 +58,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
   extern __shared__ __align__(1024) uint8_t tc_smem[];
   __shared__ __align__(8) uint64_t bars[4 * STAGES + 6];
   __shared__ __align__(16) float stat[KV ? STAGES : 1][3][TC_K];  // a stage's queries: -maximum, -log2 of the sum, -delta
-  __shared__ float row_delta[KV ? 1 : TC_Q], far_sum[2][4], far_all[2];
+  __shared__ float row_delta[KV ? 1 : TC_Q], far_sum[2][4], far_all[2];  // the second and third: dk, dv form
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   const int rank = (int)(blockIdx.x % ranks);
@@ -67,7 +71,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
   auto row_of = [&](void* base, int row) {
     return row < g.tokens ? static_cast<T*>(base) + (((int64_t)w.b * g.tokens + row) * (KV ? g.heads_kv : g.heads) + w.head) * D : nullptr;
   };
-  float* partial = KV ? nullptr : g.partial + ((int64_t)w.head * g.batch * tiles + (int64_t)w.b * tiles + w.tile) * g.buckets;
+  auto partial_of = [&](int head) { return g.partial + ((int64_t)head * g.batch * tiles + (int64_t)w.b * tiles + w.tile) * g.buckets; };
   if (a0 >= len) {  // the whole cluster
     if (rank == 0)
       for (int c = threadIdx.x; c < TC_Q * (D / 8); c += TC_THREADS) {
@@ -76,17 +80,17 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
         *reinterpret_cast<uint4*>(row_of(KV ? g.dk : g.dq, row) + part) = make_uint4(0u, 0u, 0u, 0u);
         if (KV) *reinterpret_cast<uint4*>(row_of(g.dv, row) + part) = make_uint4(0u, 0u, 0u, 0u);
       }
-    if (!KV)
-      for (int i = threadIdx.x; i < g.buckets; i += TC_THREADS) partial[i] = 0.f;
+    if (KV)
+      for (int i = threadIdx.x; i < share * g.buckets; i += TC_THREADS) partial_of(head_of(i / g.buckets))[i % g.buckets] = 0.f;
     return;  // the other form walks over queries below the length only: delta is not read here
   }
   const uint32_t a_at = (smem_u32(tc_smem) + 1023u) & ~1023u, b_at = a_at + 2 * A_BYTES;
   uint8_t* operands = tc_smem + (a_at - smem_u32(tc_smem));
   float* bt = reinterpret_cast<float*>(operands + tb_operands<D, KV>());
   const int side = g.reach + TB_RIM, span = 2 * side + 1;
-  float* dacc = bt + span;        // dq form: dS by offset, for each softmax warp's rows,
-  float* ds = dacc + 4 * span + 1;  // the warps' rows of half a tile of it,
-  int* order = reinterpret_cast<int*>(ds + TC_Q * TB_DS_PITCH);  // the offsets by bucket and where a bucket begins
+  float* dacc = bt + span;        // dk, dv form: dS by offset, for each softmax warp's rows,
+  float* ds = dacc + 4 * span + 1;  // 16 columns of it for each of them,
+  int* order = reinterpret_cast<int*>(ds + 4 * TB_DS);  // the offsets by bucket and where a bucket begins
   int* begin = order + 2 * g.reach + 1;
   const uint32_t bar = smem_u32(bars);
   const uint32_t full = bar, free_ = bar + 8 * STAGES, stat_full = bar + 16 * STAGES, fixed = bar + 24 * STAGES;
@@ -236,10 +240,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
       }
       const float2 st = in ? g.stats[((int64_t)w.b * g.heads + w.head) * g.tokens + row] : make_float2(0.f, INFINITY);
       fill_bias<T>(g, w.head, bt, side, threadIdx.x, 128);
-      for (int i = threadIdx.x; i < 4 * span; i += 128) dacc[i] = 0.f;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < 2 * g.reach + 1; i += 128) order[i] = min(max(__ldg(g.order + i), 0), 2 * g.reach);
-      for (int i = threadIdx.x; i <= g.buckets; i += 128) begin[i] = min(max(__ldg(g.start + i), 0), 2 * g.reach + 1);
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         float a[8], b[8], dot = 0.f;
@@ -256,7 +256,54 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
       nm = pair(-st.x, -st.x);
       nl = pair(-st.y, -st.y);
       nd = pair(-d, -d);
+    } else {
+      for (int i = threadIdx.x; i < 4 * span; i += 128) dacc[i] = 0.f;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < 2 * g.reach + 1; i += 128) order[i] = min(max(__ldg(g.order + i), 0), 2 * g.reach);
+      for (int i = threadIdx.x; i <= g.buckets; i += 128) begin[i] = min(max(__ldg(g.start + i), 0), 2 * g.reach + 1);
     }
+    // The table's partial sums of one query head, from what its tiles have left by offset.
+    auto finish_table = [&](int head) {
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, m);
+        after += __shfl_xor_sync(0xffffffffu, after, m);
+      }
+      if (lane == 0) { far_sum[0][warp] = before; far_sum[1][warp] = after; }
+      before = after = 0.f;
+      softmax_sync();
+      auto by_offset_sum = [&](int i) { return (dacc[i] + dacc[span + i]) + (dacc[2 * span + i] + dacc[3 * span + i]); };
+      if (warp < 2) {  // offsets past the reach join its ends
+        float rim = 0.f;
+        for (int i = lane; i < TB_RIM; i += 32) rim += by_offset_sum(warp ? span - 1 - i : i);
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) rim += __shfl_xor_sync(0xffffffffu, rim, m);
+        if (lane == 0) far_all[warp] = rim + (far_sum[warp][0] + far_sum[warp][1]) + (far_sum[warp][2] + far_sum[warp][3]);
+      }
+      softmax_sync();
+      float* sorted = ds;  // the sums in the order of their buckets
+      static_assert(4 * TB_DS >= 2 * 1024 + 1, "the largest reach fits");
+      for (int n = threadIdx.x; n < 2 * g.reach + 1; n += 128) {
+        const int i = order[n];
+        sorted[n] = by_offset_sum(i + TB_RIM) + (i == 0 ? far_all[0] : i == 2 * g.reach ? far_all[1] : 0.f);
+      }
+      softmax_sync();
+      float* partial = partial_of(head);
+      for (int base = 0; base < g.buckets; base += 32) {  // four lanes per bucket
+        const int b = base + threadIdx.x / 4;
+        float all = 0.f;
+        if (b < g.buckets)
+#pragma unroll 4
+          for (int n = begin[b] + (lane & 3); n < begin[b + 1]; n += 4) all += sorted[n];
+        all += __shfl_xor_sync(0xffffffffu, all, 1);
+        all += __shfl_xor_sync(0xffffffffu, all, 2);
+        if (b < g.buckets && (lane & 3) == 0) partial[b] = ok ? all : NAN;
+      }
+      for (int i = threadIdx.x; i < 4 * span; i += 128) dacc[i] = 0.f;  // for the next head, which begins with a barrier
+    };
+    // A softmax thread's row in ds, and its lane's way down the diagonals of its half of the warp's rows.
+    float* ds_row = ds + warp * TB_DS + (lane >> 4) * TB_DS_HALF + (lane & 15) * TB_DS_PITCH;
+    const float* ds_walk = ds + warp * TB_DS + (lane >> 4) * TB_DS_HALF + (lane & 15);
     for (int n = 0; n < steps; ++n) {
       const int tile = n % n_tiles, b0 = first + tile * TC_K, s = n % STAGES;
       if (KV && tile == 0) {
@@ -267,9 +314,9 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
       // key minus query: at least the reach for the whole tile, or at most minus the reach
       const int low = KV ? a0 - (b0 + TC_K - 1) : b0 - (a0 + TC_Q - 1), high = KV ? a0 + TC_Q - 1 - b0 : b0 + TC_K - 1 - a0;
       const int far = low >= g.reach ? 1 : -high >= g.reach ? -1 : 0;
-      const bool edge = b0 + TC_K > len || (g.causal && high > 0);
-      // of the tile's columns the row has those from `lo` on, `held` of them
-      const int lo = KV && g.causal ? max(0, row - b0) : 0, held = (!KV && g.causal ? min(len, row + 1) : len) - b0 - lo;
+      const bool edge = b0 + TC_K > len || (g.causal && high > 0) || (KV && a0 + TC_Q > len);
+      // of the tile's columns the row has those from `lo` on, `held` of them; keys past the length have none (the table)
+      const int lo = KV && g.causal ? max(0, row - b0) : 0, held = KV && !in ? 0 : (!KV && g.causal ? min(len, row + 1) : len) - b0 - lo;
       const float one = far > 0 ? bt[2 * side] : bt[0];
       const float* by_offset = KV ? bt + row - b0 + side : bt + b0 - row + side;
       const float *s_m = stat[KV ? s : 0][0], *s_l = stat[KV ? s : 0][1], *s_d = stat[KV ? s : 0][2];
@@ -324,30 +371,28 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
               const float2 fp = both(prob), fg = both(grad);
               p[k / 2] = pack2<T>(fp.x, fp.y);
               z[k / 2] = pack2<T>(fg.x, fg.y);
-              if (!KV) {
-                sum = add2(sum, grad);
-                if (MODE == 1 || (MODE == 2 && !far)) *reinterpret_cast<float2*>(ds + threadIdx.x * TB_DS_PITCH + at % TB_HALF) = fg;
-              }
+              if (!KV || MODE != 1) sum = add2(sum, grad);
+              if (KV && (MODE == 1 || (MODE == 2 && !far))) *reinterpret_cast<float2*>(ds_row + k) = fg;
             }
           }
           tc_st8(mine + c / 2, p);  // over columns that have been read
           tc_st8(mine + TB_DP_COL + c / 2, z);
-          if (!KV && c % TB_HALF == TB_HALF - 16 && (MODE == 1 || (MODE == 2 && !far))) {
-            // The warp's 32 x 32 of dS by diagonals: lane l walks down the rows from column l on, modulo 32, and so
-            // over two diagonals that are 32 apart.
+          if (KV && (MODE == 1 || (MODE == 2 && !far))) {
+            // 16 x 16 of dS by diagonals, one for each half of the warp: lane l walks down the rows from column l on, modulo
+            // 16, and so over two diagonals that are 16 apart.
             __syncwarp();
-            const float* from = ds + warp * 32 * TB_DS_PITCH + lane;
             float ahead = 0.f, wrapped = 0.f;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const bool past = k + lane >= 32;
-              const float v = from[k * (TB_DS_PITCH + 1) - (past ? 32 : 0)];
+            for (int k = 0; k < TB_COLS; ++k) {
+              const bool past = k + (lane & 15) >= TB_COLS;
+              const float v = ds_walk[k * (TB_DS_PITCH + 1) - (past ? TB_COLS : 0)];
               ahead += past ? 0.f : v;
               wrapped += past ? v : 0.f;
             }
-            float* to = dacc + warp * span + (b0 + c / TB_HALF * TB_HALF) - (a0 + warp * 32) + side + lane;
+            float* to = dacc + warp * span + (a0 + warp * 32 + (lane & 16)) - (b0 + c) + side - (lane & 15);
             to[0] += ahead;
-            to[-32] += wrapped;
+            __syncwarp();  // the other half's offsets are 16 further on
+            to[TB_COLS] += wrapped;
             __syncwarp();
           }
         }
@@ -359,12 +404,12 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
-      if (!KV) {
-        const float2 f = both(sum);
-        const float tile_sum = f.x + f.y;
-        r += tile_sum;
-        if (far > 0) after += tile_sum;
-        else if (far < 0) before += tile_sum;
+      const float2 f = both(sum);
+      if (!KV) r += f.x + f.y;
+      else {
+        if (far > 0) after += f.x + f.y;
+        else if (far < 0) before += f.x + f.y;
+        if (tile == n_tiles - 1) finish_table(head_of(n / n_tiles));
       }
     }
     ok = ok && wait(done, (steps - 1) & 1, ERR_TC_O);
@@ -389,39 +434,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) k_rel_tc_bwd(const __grid_const
         }
       }
       if (in) g.delta[((int64_t)w.b * g.heads + w.head) * g.tokens + row] = ok ? d + r : NAN;
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, m);
-        after += __shfl_xor_sync(0xffffffffu, after, m);
-      }
-      if (lane == 0) { far_sum[0][warp] = before; far_sum[1][warp] = after; }
-      softmax_sync();
-      auto by_offset_sum = [&](int i) { return (dacc[i] + dacc[span + i]) + (dacc[2 * span + i] + dacc[3 * span + i]); };
-      if (warp < 2) {  // offsets past the reach join its ends
-        float rim = 0.f;
-        for (int i = lane; i < TB_RIM; i += 32) rim += by_offset_sum(warp ? span - 1 - i : i);
-#pragma unroll
-        for (int m = 16; m > 0; m >>= 1) rim += __shfl_xor_sync(0xffffffffu, rim, m);
-        if (lane == 0) far_all[warp] = rim + (far_sum[warp][0] + far_sum[warp][1]) + (far_sum[warp][2] + far_sum[warp][3]);
-      }
-      softmax_sync();
-      float* sorted = ds;  // the sums in the order of their buckets
-      static_assert(TC_Q * TB_DS_PITCH >= 2 * 1024 + 1, "the largest reach fits");
-      for (int n = threadIdx.x; n < 2 * g.reach + 1; n += 128) {
-        const int i = order[n];
-        sorted[n] = by_offset_sum(i + TB_RIM) + (i == 0 ? far_all[0] : i == 2 * g.reach ? far_all[1] : 0.f);
-      }
-      softmax_sync();
-      for (int base = 0; base < g.buckets; base += 32) {  // four lanes per bucket
-        const int b = base + threadIdx.x / 4;
-        float all = 0.f;
-        if (b < g.buckets)
-#pragma unroll 4
-          for (int n = begin[b] + (lane & 3); n < begin[b + 1]; n += 4) all += sorted[n];
-        all += __shfl_xor_sync(0xffffffffu, all, 1);
-        all += __shfl_xor_sync(0xffffffffu, all, 2);
-        if (b < g.buckets && (lane & 3) == 0) partial[b] = ok ? all : NAN;
-      }
     } else {
       constexpr int SP = D + 4;
       static_assert(2 * TC_Q * SP * 4 <= tb_operands<D, true>(), "the sums fit the operands");

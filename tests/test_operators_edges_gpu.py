@@ -141,3 +141,93 @@ def test_relative_attention_huge_values_behind_a_mask(tokens, d, closed):
     p = torch.where(index == 31, 0.0, p)  # exp(-1e4 + a few) is 0 in any format that holds 1e38 finite
     want, size = torch.einsum("bhij,bjhd->bihd", p, v.double()), torch.einsum("bhij,bjhd->bihd", p, v.double().abs())
     assert ((out - want).abs() <= (2 * u + 2.0 ** -14) * size).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# The table's gradient where the values have a common mean
+# ---------------------------------------------------------------------------------------------------------------
+
+
+def definition(q, k, v, table, plan, lengths, dout):
+    """Output and gradients in 64 bits, by differentiation."""
+    b, t, h, d = q.shape
+    off = torch.arange(t, device="cuda")[None] - torch.arange(t, device="cuda")[:, None]
+    index = plan.map.long()[off.clamp(-plan.max_distance, plan.max_distance) + plan.max_distance]
+    live = torch.ones(b, t, dtype=torch.bool, device="cuda") if lengths is None else torch.arange(t, device="cuda") < lengths[:, None]
+    seen = live[:, None, :, None] & live[:, None, None, :]
+    if plan.causal:
+        seen = seen & (off <= 0)
+    leaves = [x.detach().double().requires_grad_(True) for x in (q, k, v, table)]
+    share = h // k.shape[2]
+    qd, kd, vd = leaves[0].transpose(1, 2), *(x.transpose(1, 2).repeat_interleave(share, 1) for x in leaves[1:3])
+    s = qd @ kd.transpose(-1, -2) * d ** -0.5 + leaves[3][index].permute(2, 0, 1)
+    s = torch.where(seen, s, -1e300)
+    p = torch.exp(s - s.amax(-1, keepdim=True).clamp_min(-1e290).detach())  # 0 all along a row without keys
+    p = p / p.sum(-1, keepdim=True).clamp_min(1e-290)
+    out = (p @ vd).transpose(1, 2)
+    return [out.detach(), *torch.autograd.grad(out, leaves, dout.double() * live[:, :, None, None])]
+
+
+MEAN_CASES = [
+    # batch, tokens, heads, key heads, head_dim, type, causal, ragged, buckets, reach, mean of v
+    (3, 54, 8, 8, 32, "bf16", False, False, 32, 128, 4.0),
+    (2, 65, 4, 4, 64, "bf16", False, False, 32, 128, 4.0),
+    (2, 40, 4, 2, 64, "f16", False, False, 32, 128, 4.0),
+    (2, 63, 8, 1, 32, "bf16", True, True, 32, 40, 2.0),
+    (2, 300, 2, 2, 64, "f16", False, True, 32, 128, 4.0),
+    (1, 1001, 2, 2, 64, "bf16", False, False, 32, 128, 4.0),
+    (1, 1001, 2, 2, 64, "f16", False, False, 32, 1024, 4.0),
+    (1, 1001, 2, 1, 64, "f16", False, False, 4, 2, 4.0),
+    (2, 777, 4, 2, 32, "f16", True, True, 32, 128, 1.0),
+    (1, 1001, 11, 1, 32, "bf16", False, True, 8, 5, 3.0),
+    (1, 1501, 4, 2, 64, "bf16", True, False, 32, 128, 0.0),
+    (2, 449, 2, 2, 32, "bf16", False, False, 32, 128, 0.0),
+    (1, 640, 2, 2, 32, "bf16", False, True, 32, 128, 0.0),
+    (2, 321, 4, 2, 64, "bf16", True, True, 32, 128, 0.0),
+    (9, 33, 8, 4, 32, "f16", False, False, 32, 128, 0.0),
+    (30, 54, 8, 8, 32, "bf16", False, True, 32, 128, 0.0),
+]
+
+
+def mean_inputs(case, seed, broadcast=False):
+    b, t, h, hk, d, dtype, causal, ragged, buckets, reach, mean = case
+    gen, dt = generator(seed), TYPES[dtype]
+    q, k, v = normal(gen, b, t, h, d, dtype=dt), normal(gen, b, t, hk, d, dtype=dt), normal(gen, b, t, hk, d, dtype=dt, mean=mean)
+    plan = ops.RelativeBuckets(buckets, reach, causal=causal)
+    lengths = torch.randint(t // 2, t + 1, (b,), generator=gen, device="cuda", dtype=torch.int32) if ragged else None
+    return q, k, v, normal(gen, buckets, h, dtype=dt), plan, lengths, normal(gen, b, t, h, d, dtype=dt)
+
+
+def check_gradients(q, k, v, table, plan, lengths, dout):
+    u = torch.finfo(q.dtype).eps / 2
+    want = definition(q, k, v, table, plan, lengths, dout)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, table)]
+    out = ops.relative_attention(*leaves, plan, lengths=lengths)
+    got = torch.autograd.grad(out, leaves, dout)
+    # The table's gradient is a float32 sum, rounded once: u of each entry.  A pair's P (dP - delta) is off by some 2^-20 of
+    # P (|dP| + |delta|), each below 8 (1 + mean) of the spread sqrt(head_dim) that dP - delta has, and pair for pair on its
+    # own: 2^-20 * 80 < 2^-13 of what the pairs add up to, in an entry that is not small beside the largest one.
+    off, size = (got[3].double() - want[4]).abs(), want[4].abs()
+    assert (off <= u * size + 2.0 ** -12 * size.max()).all(), ("dtable", float((off / size.max()).max() / u))
+    assert off.norm() <= 2 * u * size.norm(), ("dtable", float(off.norm() / size.norm() / u))
+    # dq, dk, dv: P and dS are rounded before their products, each term on its own (u / sqrt(3) of it, in quadrature), and the
+    # results once more: 2 u of the 2-norm with room, where the terms of dS k and dS^T q do not cancel.
+    for name, g, w in zip(("dq", "dk", "dv"), got, want[1:]):
+        error = (g.double() - w).norm() / w.norm()
+        assert error <= 2 * u, (name, float(error / u))
+
+
+@pytest.mark.parametrize("case", MEAN_CASES, ids=str)
+def test_relative_attention_gradients_with_a_mean(case):
+    check_gradients(*mean_inputs(case, seed=1))
+
+
+@pytest.mark.parametrize("case", [MEAN_CASES[4], MEAN_CASES[5], MEAN_CASES[9]], ids=str)
+def test_relative_attention_gradients_with_a_mean_broadcast(case):
+    """One sequence's keys for several (a stride of 0, which the tile form takes)."""
+    q, k, v, table, plan, lengths, dout = mean_inputs(case, seed=2)
+    gen = generator(3)
+    b, t, h, d = q.shape
+    q, dout = (normal(gen, 2 * b, t, h, d, dtype=q.dtype) for _ in range(2))
+    k, v = (x[:1].expand(2 * b, -1, -1, -1) for x in (k, v))
+    check_gradients(q, k, v, table, plan, None if lengths is None else lengths.repeat(2), dout)
