@@ -4,10 +4,12 @@
 * ``relative_attention``: softmax attention with a learned bias per head and distance bucket.
 * ``distill_top_logits`` / ``distill_top_logits_step``: how far a student's logits are from a teacher's top entries.
 
-All three run hand-written kernels of libmgbs_b200.so and take part in autograd (first derivatives).  Wrong shapes, types
-or devices raise RuntimeError before anything is enqueued; there is no CPU fallback.  Nothing is kept between calls,
-outputs and workspaces come from torch's allocator, equal calls give equal bits, and every call may be captured in a
-CUDA graph (a backward pass only while no eager autograd graph of the same leaves is alive, a rule of autograd's own).  TransformerValueScorer, TransformerValueNet and MLPActionScorer.distillation_loss call them.
+All three run hand-written kernels of libmgbs_b200.so and take part in autograd (first derivatives, in reverse mode; forward
+mode, tracing and torch.func transforms are refused).  Wrong shapes, types or devices raise RuntimeError before anything is
+enqueued; there is no CPU fallback.  Nothing is kept between calls, outputs and workspaces come from torch's allocator, equal
+calls give equal bits, and every call may be captured in a CUDA graph (a backward pass only while no eager autograd graph of
+the same leaves is alive, a rule of autograd's own).  TransformerValueScorer, TransformerValueNet and
+MLPActionScorer.distillation_loss call them.
 """
 
 from __future__ import annotations
@@ -17,6 +19,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -125,6 +128,14 @@ def _once(backward):
     return run
 
 
+def _refuse_unseen(what: str, *tensors) -> None:
+    """Refuse the transforms that would not see the kernel, and go on without its work or its tangent."""
+    if torch.jit.is_tracing() or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        _refuse(what, "cannot be recorded by torch.jit.trace or make_fx")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse(what, "has no forward-mode derivative")
+
+
 def _same_device(what: str, device: torch.device, *tensors) -> None:
     for t in tensors:
         if t is not None and t.device != device:
@@ -216,6 +227,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dq_out, dk_out):
+        _refuse_unseen("qk_norm_rope backward", dq_out, dk_out)
         q, k, q_gain, k_gain, positions = ctx.saved_tensors
         lib = _load()
         a = _qk_args(q, k, q_gain, k_gain, ctx.rotary, positions, ctx.eps, ctx.interleaved)
@@ -241,6 +253,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: torch.Tensor, k_gain:
     token's index.  Pairs are (i, i + head_dim / 2), or (2 i, 2 i + 1) with ``interleaved``.  Statistics and rotation are
     in float32, rounded once.  Differentiable in q, k and the gains."""
     what, dtype, device = "qk_norm_rope", q.dtype, q.device
+    _refuse_unseen(what, q, k, q_gain, k_gain)
     if not q.is_cuda or q.dim() != 4 or k.dim() != 4:
         _refuse(what, "q and k must be [batch, tokens, heads, head_dim] CUDA tensors")
     if dtype not in DTYPES or k.dtype != dtype:
@@ -363,6 +376,7 @@ class _RelativeAttention(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dout):
+        _refuse_unseen("relative_attention backward", dout)
         q, k, v, table, lengths, out, stats = ctx.saved_tensors
         lib = _load()
         a = _rel_args(q, k, v, table, ctx.buckets, lengths, ctx.scale)
@@ -390,6 +404,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     P (dP - delta) are rounded to the inputs' type on the way, so with float16 a loss scale has to keep the latter below
     65504."""
     what, dtype, device = "relative_attention", q.dtype, q.device
+    _refuse_unseen(what, q, k, v, table)
     if not q.is_cuda or q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         _refuse(what, "q, k and v must be [batch, tokens, heads, head_dim] CUDA tensors")
     if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype != dtype or v.dtype != dtype or table.dtype != dtype:
@@ -425,6 +440,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
 
 
 def _distill_check(what, logits, teacher, index, temperature):
+    _refuse_unseen(what, logits)
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in DTYPES or logits.shape[1] < 1:
         _refuse(what, "logits must be a [rows, width] CUDA tensor with one column at least: bfloat16, float16 or float32")
     if teacher.dim() != 2 or teacher.shape != index.shape or teacher.shape[0] != logits.shape[0]:
@@ -472,6 +488,7 @@ class _DistillTopLogits(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dloss):
+        _refuse_unseen("distill_top_logits backward", dloss)
         logits, teacher, index = ctx.saved_tensors
         weight = dloss.to(torch.float32).contiguous()
         return _distill_run("distill_top_logits backward", logits, teacher, index, ctx.temperature, weight, True)[1], None, None, None

@@ -6,6 +6,9 @@ import re
 from pathlib import Path
 
 import pytest
+import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from multigpubeamsearch_b200 import operators as ops
 
@@ -49,3 +52,47 @@ def test_shared_arrays_declare_their_alignment(name):
 def test_sums_sent_between_blocks_are_aligned():
     text = (Path(ops.__file__).parent / "csrc" / "mgbs_distill.cu").read_text()
     assert "st.shared::cluster.v2.b32" in text and "struct __align__(8) Sum" in text
+
+
+def calls():
+    """Each function on CPU tensors, as (call, its differentiable arguments): refused for a reason that comes before the device's."""
+    q = torch.zeros(1, 2, 1, 32, dtype=torch.bfloat16)
+    gain, table = torch.ones(32), torch.zeros(32, 1, dtype=torch.bfloat16)
+    logits, teacher, index = torch.zeros(2, 4), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int64)
+    rotary, plan = ops.RotaryFrequencies(32, device="cpu"), ops.RelativeBuckets(device="cpu")
+    return {
+        "qk_norm_rope": (lambda q, k, g, h: ops.qk_norm_rope(q, k, g, h, rotary), (q, q, gain, gain)),
+        "relative_attention": (lambda q, k, v, t: ops.relative_attention(q, k, v, t, plan), (q, q, q, table)),
+        "distill_top_logits": (lambda z: ops.distill_top_logits(z, teacher, index), (logits,)),
+        "distill_top_logits_step": (lambda z: ops.distill_top_logits_step(z, teacher, index), (logits,)),
+    }
+
+
+@pytest.mark.parametrize("name", calls())
+def test_forward_mode_is_refused(name):
+    call, leaves = calls()[name]
+    for n in range(len(leaves)):
+        with forward_ad.dual_level():
+            args = [x.clone() for x in leaves]
+            args[n] = forward_ad.make_dual(args[n], torch.ones_like(args[n]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*args)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="CUDA"):  # a level without a tangent is none of its business
+        call(*leaves)
+
+
+@pytest.mark.parametrize("name", calls())
+def test_tracing_is_refused(name):
+    call, leaves = calls()[name]
+    with pytest.raises(RuntimeError, match="recorded"):
+        torch.jit.trace(call, leaves, check_trace=False)
+    with pytest.raises(RuntimeError, match="recorded"):
+        make_fx(call)(*leaves)
+
+
+@pytest.mark.parametrize("function,count", [(ops._QkNormRope, 2), (ops._RelativeAttention, 1), (ops._DistillTopLogits, 1)])
+def test_forward_mode_over_a_backward_is_refused(function, count):
+    with forward_ad.dual_level():
+        grads = [forward_ad.make_dual(torch.zeros(3), torch.ones(3)) for _ in range(count)]
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            function.backward(None, *grads)
