@@ -503,12 +503,12 @@ typedef struct MgbsTfConfig {
   float* q;     /* f32 [max_states] */
   int32_t* err;
   int32_t dtype; /* GEMM operand type: 0 = bf16, 1 = e4m3 (float32 accumulation, residual stream and softmax either way) */
-  float qk_eps;  /* of the layers' query and key norm */
+  float qk_eps;  /* of the layers' query and key norm, >= 0 */
   const uint64_t* rotary_phase[MGBS_TF_MAX_ENCODERS]; /* [16], with q_gain; zeros turn nothing */
   const int32_t* rel_map;    /* with rel_table: bucket_map, bucket_order and bucket_start of MgbsRelAttentionArgs */
   const int32_t* rel_order;
   const int32_t* rel_start;
-  int32_t rel_buckets, rel_distance;
+  int32_t rel_buckets, rel_distance; /* 1 .. 512, 1 .. 1024 */
 } MgbsTfConfig;
 typedef struct MgbsTf MgbsTf;
 int mgbs_sizeof_tf_config(void);

@@ -595,6 +595,22 @@ extern "C" {
 
 int mgbs_sizeof_tf_config(void) { return (int)sizeof(MgbsTfConfig); }
 
+// What the query/key norm and the attention with a relative bias would refuse: known here, because a call of
+// mgbs_tf_enqueue has other kernels on the stream before it comes to them.
+static int tf_relative_check(const MgbsTfConfig& c) {
+  for (int e = 0; e < c.encoders; ++e)
+    for (int l = 0; l < c.layers; ++l) {
+      const MgbsTfLayer& L = c.layer[e][l];
+      if (!L.q_gain != !L.k_gain) return MGBS_ERR_ARG;
+      if (L.q_gain && (!c.rotary_phase[e] || !(c.qk_eps >= 0.f) || isinf(c.qk_eps))) return MGBS_ERR_ARG;
+      if (!L.rel_table) continue;
+      if (c.dtype != 0) return MGBS_ERR_UNSUPPORTED;
+      if (!c.rel_map || !c.rel_order || !c.rel_start) return MGBS_ERR_ARG;
+      if (c.rel_buckets < 1 || c.rel_buckets > 512 || c.rel_distance < 1 || c.rel_distance > 1024) return MGBS_ERR_ARG;
+    }
+  return 0;
+}
+
 int mgbs_tf_create(const MgbsTfConfig* cfg, MgbsTf** out) {
   if (!cfg || !out) return MGBS_ERR_ARG;
   const MgbsTfConfig& c = *cfg;
@@ -604,6 +620,8 @@ int mgbs_tf_create(const MgbsTfConfig* cfg, MgbsTf** out) {
   if (c.layers < 1 || c.layers > MGBS_TF_MAX_LAYERS || c.encoders < 1 || c.encoders > MGBS_TF_MAX_ENCODERS) return MGBS_ERR_ARG;
   if (c.max_states < 1 || c.micro_batch < 1) return MGBS_ERR_ARG;
   if (!c.x || !c.y || !c.qkv || !c.att || !c.hid || !c.q || !c.err) return MGBS_ERR_ARG;
+  const int relative = tf_relative_check(c);
+  if (relative) return relative;
   MgbsTf* t = new (std::nothrow) MgbsTf();
   if (!t) return MGBS_ERR_STATE;
   t->cfg = c;
@@ -632,9 +650,6 @@ int mgbs_tf_create(const MgbsTfConfig* cfg, MgbsTf** out) {
       if (!L.ln1_g || !L.ln1_b || !L.wqkv || !L.bqkv || !L.wo || !L.bo || !L.ln2_g || !L.ln2_b || !L.w1 || !L.b1 ||
           !L.w2 || !L.b2)
         rc = MGBS_ERR_ARG;
-      if (!rc && ((!L.q_gain != !L.k_gain) || (L.q_gain && !c.rotary_phase[e]))) rc = MGBS_ERR_ARG;
-      if (!rc && L.rel_table && c.dtype != 0) rc = MGBS_ERR_UNSUPPORTED;
-      if (!rc && L.rel_table && (!c.rel_map || !c.rel_order || !c.rel_start)) rc = MGBS_ERR_ARG;
       if (!rc && c.dtype == 1 && (!L.cs_qkv || !L.cs_o || !L.cs_1 || !L.cs_2)) rc = MGBS_ERR_ARG;
       if (!rc) rc = mgbs::make_map(&t->tm_wqkv[e][l], L.wqkv, 768, 256, mgbs::BN, eb);
       if (!rc) rc = mgbs::make_map(&t->tm_wo[e][l], L.wo, 256, 256, mgbs::BN, eb);

@@ -10,7 +10,7 @@ import torch
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from multigpubeamsearch_b200 import operators as ops
+from multigpubeamsearch_b200 import operators as ops, scorers
 
 ERR_ARG, ERR_UNSUPPORTED = -1, -2
 SOME = 1 << 20  # an address that is aligned and never read: no call below enqueues anything
@@ -96,3 +96,39 @@ def test_forward_mode_over_a_backward_is_refused(function, count):
         grads = [forward_ad.make_dual(torch.zeros(3), torch.ones(3)) for _ in range(count)]
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             function.backward(None, *grads)
+
+
+def encoder_config(**more):
+    """A transformer scorer's configuration with relative positions in layer 1, its pointers never read."""
+    c = scorers.MgbsTfConfig(state_len=54, state_stride=64, num_values=6, d_model=256, heads=8, ffn=1024, layers=2, encoders=1, max_states=8,
+                             micro_batch=8, qk_eps=1e-6, rel_buckets=32, rel_distance=128)
+    for n in ("x", "y", "qkv", "att", "hid", "q", "err", "rel_map", "rel_order", "rel_start"):
+        setattr(c, n, SOME)
+    c.rotary_phase[0] = SOME
+    for n in ("q_gain", "k_gain", "rel_table"):
+        setattr(c.layer[0][1], n, SOME)
+    for n, v in more.items():
+        if n in ("q_gain", "k_gain", "rel_table"):
+            setattr(c.layer[0][1], n, v)
+        elif n == "rotary_phase":
+            c.rotary_phase[0] = v
+        else:
+            setattr(c, n, v)
+    return c
+
+
+@pytest.mark.parametrize("bad,code", [(dict(rel_buckets=0), ERR_ARG), (dict(rel_buckets=513), ERR_ARG), (dict(rel_distance=0), ERR_ARG),
+                                      (dict(rel_distance=1025), ERR_ARG), (dict(qk_eps=-1.0), ERR_ARG), (dict(qk_eps=float("nan")), ERR_ARG),
+                                      (dict(qk_eps=float("inf")), ERR_ARG), (dict(q_gain=None), ERR_ARG), (dict(rotary_phase=None), ERR_ARG),
+                                      (dict(rel_start=None), ERR_ARG), (dict(dtype=1), ERR_UNSUPPORTED)])
+def test_transformer_with_relative_positions_is_refused_when_created(bad, code):
+    """Not by a call of its own kernels later on: nothing of the rest of this configuration is looked at before."""
+    c, handle, made = encoder_config(**bad), C.c_void_p(), False
+    lib = ops._load()
+    try:
+        rc = lib.mgbs_tf_create(C.byref(c), C.byref(handle))
+        made = rc == 0
+    finally:
+        if made:
+            lib.mgbs_tf_destroy(handle)
+    assert rc == code
