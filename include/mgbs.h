@@ -597,9 +597,11 @@ int mgbs_qk_norm_rope_backward(const MgbsQkNormArgs* args, void* stream);
 /* Softmax attention with a learned bias per head and distance bucket:
  *   out_i = sum_j softmax_j(scale q_i . k_j + table[bucket(j - i), head]) v_j.
  * Query heads share key heads in runs of heads / heads_kv.  With lengths, tokens of a sequence from its length on are
- * no keys, are never read, and their outputs and gradients are 0; causal leaves only keys j <= i.  Strides in
- * elements (batch, token, head), the last dimension 1; q, k, v, dout on 16-byte boundaries (base and strides).
- * out, dq, dk, dv are contiguous. */
+ * no keys, what they hold has no influence, and their outputs and gradients are 0; they are memory that can be read over
+ * the whole of [batch, tokens] all the same, and that nothing writes during the call (tiles that straddle a length are
+ * loaded whole).  causal leaves only keys j <= i; a NaN or an infinity in the v (k in the backward) of a key that causal
+ * or a bias of -inf hides may still reach rows of its tile, as 0 times it.  Strides in elements (batch, token, head), the
+ * last dimension 1; q, k, v, dout on 16-byte boundaries (base and strides).  out, dq, dk, dv are contiguous. */
 typedef struct MgbsRelAttentionArgs {
   int32_t dtype;     /* MGBS_DT_BF16 or MGBS_DT_F16: q, k, v, table, out and all gradients */
   int32_t head_dim;  /* 32 or 64 */
@@ -616,7 +618,7 @@ typedef struct MgbsRelAttentionArgs {
   const int32_t* lengths;    /* [batch] or null */
   void* out;
   float* stats;      /* [batch, heads, tokens, 2] softmax statistics, or null: needed for a backward call when tokens > 64 or
-                      * heads != heads_kv, written by the forward and read by the backward */
+                      * heads != heads_kv, and only then written by the forward and read by the backward */
   int32_t num_buckets, max_distance; /* 1 .. 512, 1 .. 1024 */
   int32_t causal;
   float scale;       /* > 0 */

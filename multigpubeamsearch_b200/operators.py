@@ -5,11 +5,11 @@
 * ``distill_top_logits`` / ``distill_top_logits_step``: how far a student's logits are from a teacher's top entries.
 
 All three run hand-written kernels of libmgbs_b200.so and take part in autograd (first derivatives, in reverse mode; forward
-mode, tracing and torch.func transforms are refused).  Wrong shapes, types or devices raise RuntimeError before anything is
-enqueued; there is no CPU fallback.  Nothing is kept between calls, outputs and workspaces come from torch's allocator, equal
-calls give equal bits, and every call may be captured in a CUDA graph (a backward pass only while no eager autograd graph of
-the same leaves is alive, a rule of autograd's own).  TransformerValueScorer, TransformerValueNet and
-MLPActionScorer.distillation_loss call them.
+mode, tracing and torch.func transforms are refused, and torch.compile wants the call inside torch.compiler.disable).
+Wrong shapes, types or devices raise RuntimeError before anything is enqueued; there is no CPU fallback.  Nothing is kept
+between calls, outputs and workspaces come from torch's allocator, equal calls give equal bits, and every call may be
+captured in a CUDA graph (a backward pass only while no eager autograd graph of the same leaves is alive, a rule of
+autograd's own).  TransformerValueScorer, TransformerValueNet and MLPActionScorer.distillation_loss call them.
 """
 
 from __future__ import annotations
@@ -399,10 +399,13 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     ``q`` [batch, tokens, heads, head_dim], ``k`` and ``v`` [batch, tokens, key heads, head_dim], ``table`` [num_buckets,
     heads]: bfloat16 or float16 (one type), head_dim 32 or 64, heads a multiple of the key heads.  Any strides (a copy
     is made only where rows do not lie on 16-byte boundaries).  ``lengths`` (int32 [batch]): tokens of a sequence from
-    its length on are padding: never read, their outputs and gradients are 0.  ``scale``: head_dim ** -0.5 by default.
-    A row whose biases leave no key (all -inf) gives 0.  Differentiable in q, k, v and table; P and the scores' gradients
-    P (dP - delta) are rounded to the inputs' type on the way, so with float16 a loss scale has to keep the latter below
-    65504."""
+    its length on are padding: what they hold has no influence (nothing may write there during the call all the same, as
+    tiles are loaded whole), their outputs and gradients are 0.  ``scale``: head_dim ** -0.5 by default.  A row whose
+    biases leave no key (all -inf) gives 0.  A NaN or an infinity in the values of a key that only a causal mask or a bias
+    hides may reach rows beside it, as 0 times it.  Sums over the keys are in float32 before a row is divided by its
+    weights' total: values up to 1e28 are safe.  Differentiable in q, k, v and table; P and the scores' gradients
+    P (dP - delta) are rounded to the inputs' type on the way, so with float16 a loss scale has to keep the latter within
+    the type's range, 6e-8 to 65504."""
     what, dtype, device = "relative_attention", q.dtype, q.device
     _refuse_unseen(what, q, k, v, table)
     if not q.is_cuda or q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
