@@ -231,3 +231,46 @@ def test_relative_attention_gradients_with_a_mean_broadcast(case):
     q, dout = (normal(gen, 2 * b, t, h, d, dtype=q.dtype) for _ in range(2))
     k, v = (x[:1].expand(2 * b, -1, -1, -1) for x in (k, v))
     check_gradients(q, k, v, table, plan, None if lengths is None else lengths.repeat(2), dout)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Transforms
+# ---------------------------------------------------------------------------------------------------------------
+
+
+def small_calls():
+    gen, rotary, plan = generator(50), ops.RotaryFrequencies(32), ops.RelativeBuckets()
+    q, gain, table = normal(gen, 2, 70, 2, 32, dtype=torch.bfloat16), torch.ones(32, device="cuda"), normal(gen, 32, 2, dtype=torch.bfloat16)
+    logits, teacher, index = normal(gen, 3, 2000), normal(gen, 3, 4), torch.randint(0, 2000, (3, 4), generator=gen, device="cuda")
+    return {
+        "qk_norm_rope": (lambda x: ops.qk_norm_rope(x, x, gain, gain, rotary)[0], q),
+        "relative_attention": (lambda x: ops.relative_attention(x, x, x, table, plan), q),
+        "distill_top_logits": (lambda x: ops.distill_top_logits(x, teacher, index), logits),
+    }
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "relative_attention", "distill_top_logits"])
+def test_transforms_do_not_pass_a_kernel_by(name):
+    call, x = small_calls()[name]
+    for bad in (lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.vmap(call)(x[None]),
+                lambda: torch.func.grad(lambda y: call(y).float().sum())(x), lambda: torch.jit.trace(call, x, check_trace=False)):
+        with pytest.raises(RuntimeError):
+            bad()
+    y = x.clone().requires_grad_(True)
+    once, = torch.autograd.grad(call(y).float().square().sum(), y, create_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivatives
+        torch.autograd.grad(once.float().sum(), y)
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "relative_attention", "distill_top_logits"])
+def test_inside_a_compiled_function(name):
+    """Kept out of the compiled graph, a call does there what it does elsewhere."""
+    call, x = small_calls()[name]
+    apart = torch.compiler.disable(call)
+    both = [lambda y: call(y * 0.5) + 1.0, torch.compile(lambda y: apart(y * 0.5) + 1.0, backend="eager")]
+    results = []
+    for f in both:
+        y = x.clone().requires_grad_(True)
+        out = f(y)
+        results.append((out.detach(), *torch.autograd.grad(out, y, torch.ones_like(out))))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
