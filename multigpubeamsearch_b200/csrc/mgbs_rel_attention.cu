@@ -5,11 +5,12 @@
 //   dtable[b, h] = sum over sequences and pairs with bucket(j - i) = b of dS_ij
 //
 // Long sequences are in the files of the tcgen05 forms; the rest is here, on the warp-level matrix instruction (m16n8k16,
-// 16-bit operands, float32 accumulators): short sequences, and strides that TMA cannot describe.  For the scorer's 54 tokens the bytes of q, k, v bound the pass and
-// not the products: 749 us at 32768 x 54 tokens, 8 heads of 32, against 560 us for the bytes.  Scores, softmax
-// statistics, delta and all sums stay in float32; P and dS are rounded to the operands' 16 bits only as inputs of the next
-// product (the rounding errors of a row's terms are independent, so a sum over a row keeps more than the output's own 16
-// bits).
+// 16-bit operands, float32 accumulators): short sequences, and strides that TMA cannot describe.  The scorer's 54 tokens
+// take 749 us at 32768 sequences, 8 heads of 32, against 560 us for their bytes; what bounds them is the fixed latency of a
+// warp's chain of products and exponentials with 16 warps on a multiprocessor (memory is busy for half of the time), so
+// the time follows the clock: 880 us where it drops under load.  Scores, softmax statistics, delta and all sums stay in
+// float32; P and dS are rounded to the operands' 16 bits as inputs of the next product, because that product takes 16
+// bits (1.7e-3 -> 2.0e-3 of the output's norm in bfloat16, 2.1e-4 -> 2.9e-4 in float16 against products in 32 bits).
 //
 // Sequences of up to 64 tokens are one tile: a warp owns 16 query rows of one (sequence, head), a group of warps walks
 // over the sequences of ONE head, so that the head's biases live in registers as the products' initial accumulators,
@@ -1112,6 +1113,8 @@ template <typename T> int sum_table(const RelArgs& g, int tile, void* dtable, fl
 //   heads of 64:  T = 65: 1419 us against 1580 us, 256: 868 against 1267, 512: 1158 against 2220
 //   heads of 32:  T = 65: 1355 against 947, 256: 785 against 712, 384: 932 against 972, 512: 1056 against 1233 (half the
 //                 products per exponential, so that a block's fixed costs weigh more)
+// The rule asks for the number of tokens alone, while tiles are padded to 128 rows on one side and 64 on the other: just
+// past a tile's end the other form is ahead by a little, 2 % at 129 tokens (64) and at 448 (32).
 template <int D> constexpr int rel_tc_tokens() { return D == 64 ? 65 : 321; }
 // The backward is on tcgen05 from 65 tokens on for every head size: 221184 tokens, 8 heads of 64 in sequences of T = 65:
 // 1776 us against 3447 us, 129: 2250 against 3418, 192: 1526 against 2182, 1000: 3397 against 8488; heads of 32: 65: 1569
