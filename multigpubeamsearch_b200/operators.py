@@ -251,7 +251,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: torch.Tensor, k_gain:
     type), any strides (a copy is made only if the last dimension is not dense), head_dim even up to 256.  Gains:
     float32 [head_dim].  ``positions``: int32 or int64 [tokens] or [batch, tokens], negative ones included; by default a
     token's index.  Pairs are (i, i + head_dim / 2), or (2 i, 2 i + 1) with ``interleaved``.  Statistics and rotation are
-    in float32, rounded once.  Differentiable in q, k and the gains."""
+    in float32 (a head's sum of squares has to stay below 3e38), rounded once.  Differentiable in q, k and the gains."""
     what, dtype, device = "qk_norm_rope", q.dtype, q.device
     _refuse_unseen(what, q, k, q_gain, k_gain)
     if not q.is_cuda or q.dim() != 4 or k.dim() != 4:
