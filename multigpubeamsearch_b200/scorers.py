@@ -934,12 +934,12 @@ class TransformerValueScorer:
 
 
 class TransformerValueNet(torch.nn.Module):
-    """Trainable form of one encoder of TransformerValueScorer with relative positions: uint8 states [B, >= state_len] ->
-    float32 values [B]; states hold whole numbers below num_values.  Per layer x += W_o attention(LN1 x), x += W2 gelu(W1 LN2 x), where queries and keys are
-    normalised per head and rotated by position (operators.qk_norm_rope) and the attention has a learned bias per head
-    and distance bucket (operators.relative_attention); d_model 256, 8 heads.  The residual stream and all norms are
-    float32, the matrix products and the attention take bfloat16.  CUDA only.  ``encoder_weights()`` is the dictionary
-    that TransformerValueScorer loads."""
+    """Trainable form of one encoder of TransformerValueScorer with relative positions: uint8 states [B, >= state_len] of
+    whole numbers below num_values -> float32 values [B].  Per layer x += W_o attention(LN1 x), x += W2 gelu(W1 LN2 x),
+    where queries and keys are normalised per head and rotated by position (operators.qk_norm_rope) and the attention has
+    a learned bias per head and distance bucket (operators.relative_attention); d_model 256, 8 heads.  The residual stream
+    and all norms are float32, the matrix products and the attention take bfloat16.  CUDA only.  ``encoder_weights()`` is
+    the dictionary that TransformerValueScorer loads."""
 
     D, HEADS, EPS = 256, 8, 1e-6
 
