@@ -401,11 +401,11 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     is made only where rows do not lie on 16-byte boundaries).  ``lengths`` (int32 [batch]): tokens of a sequence from
     its length on are padding: what they hold has no influence (nothing may write there during the call all the same, as
     tiles are loaded whole), their outputs and gradients are 0.  ``scale``: head_dim ** -0.5 by default.  A row whose
-    biases leave no key (all -inf) gives 0.  A NaN or an infinity in the values of a key that only a causal mask or a bias
-    hides may reach rows beside it, as 0 times it.  Sums over the keys are in float32 before a row is divided by its
-    weights' total: values up to 1e28 are safe.  Differentiable in q, k, v and table; P and the scores' gradients
-    P (dP - delta) are rounded to the inputs' type on the way, so with float16 a loss scale has to keep the latter within
-    the type's range, 6e-8 to 65504."""
+    biases leave no key (all -inf) gives 0; finite biases beyond 1e38 * min(1, scale) in size are masks alike.  A NaN or
+    an infinity in the values of a key that only a causal mask or a bias hides may reach rows beside it, as 0 times it.
+    Sums over the keys are in float32 before a row is divided by its weights' total: values up to 1e28 are safe.
+    Differentiable in q, k, v and table; P and the scores' gradients P (dP - delta) are rounded to the inputs' type on the
+    way, so with float16 a loss scale has to keep the latter within the type's range, 6e-8 to 65504."""
     what, dtype, device = "relative_attention", q.dtype, q.device
     _refuse_unseen(what, q, k, v, table)
     if not q.is_cuda or q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
